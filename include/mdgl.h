@@ -43,6 +43,10 @@ extern "C" {
 
 #define MDGL_FLOAT32 0
 #define MDGL_FLOAT64 1
+/* the row operators at the end of this file (layer norm, the segment scan,
+ * routing) also take, with sums, statistics and states in float32: */
+#define MDGL_BFLOAT16 2
+#define MDGL_FLOAT16 3
 
 /* flags of mdgl_gspmm / mdgl_segment_reduce */
 #define MDGL_REPLACE_INF 1 /* +-inf results become 0 (heterograph.py:232-239) */
@@ -593,6 +597,50 @@ int mdgl_keep_where(const void* mask, const void* src, void* dst, int64_t n, int
 
 /* dst[i] = alpha * src[i]. */
 int mdgl_scale(const void* src, void* dst, int64_t n, double alpha, int dtype, void* stream);
+
+/* ---- Operators over packed rows. No counterparts in the reference. ----
+ * "State" below is float32, or float64 for MDGL_FLOAT64. Rows are contiguous. */
+
+/* What mdgl_segment_scan walks by: ids[r] = the segment of row r, and bit r % 64
+ * of starts[r / 64] / ends[r / 64]: row r is the first / last row of its segment
+ * (ceil(n / 64) words each). offsets: num_seg + 1 entries from 0 to n,
+ * non-decreasing (not checked). */
+int mdgl_segment_marks(const int32_t* offsets, int64_t num_seg, int64_t n, int32_t* ids,
+                       uint64_t* starts, uint64_t* ends, void* stream);
+
+/* Gated linear recurrence along each segment, per column:
+ *   h[t] = gate[t] * h[t-1] + value[t],  h[-1] = initial[segment] (state; null: 0)
+ * for rows of d columns. gate has the values' dtype, or MDGL_FLOAT32 with values
+ * of 16 bits. dst: h in the values' dtype; last (state, [num_seg][d], nullable):
+ * each segment's state behind its last row, its initial one for an empty segment
+ * (has_empty: whether there are any). marks (state, [ceil(n / 16)][d], nullable)
+ * is what mdgl_segment_scan_grad needs of the forward pass. ids, starts, ends:
+ * mdgl_segment_marks; longest: the longest segment's rows. Where a segment's rows
+ * are split (mdgl_segment_scan_workspace_bytes > 0), products of the gates over
+ * up to 1,024 rows are formed: they must not overflow the state's type (gates in
+ * [-1, 1] never do). */
+int mdgl_segment_scan(const void* gate, const void* value, const void* initial,
+                      const int32_t* offsets, const int32_t* ids, const uint64_t* starts,
+                      const uint64_t* ends, void* dst, void* last, void* marks, int64_t num_seg,
+                      int64_t n, int64_t d, int64_t longest, int has_empty, void* workspace,
+                      int64_t workspace_bytes, int dtype, int gate_dtype, void* stream);
+int64_t mdgl_segment_scan_workspace_bytes(int64_t n, int64_t d, int64_t longest, int dtype);
+
+/* Gradients of mdgl_segment_scan from those of h (grad, the values' dtype) and of
+ * `last` (grad_last, state, nullable): dgate (the gates' dtype; needs value and
+ * marks), dvalue and dinitial (state, [num_seg][d]), each nullable. */
+int mdgl_segment_scan_grad(const void* gate, const void* value, const void* initial,
+                           const void* marks, const void* grad, const void* grad_last,
+                           const int32_t* offsets, const int32_t* ids, const uint64_t* starts,
+                           const uint64_t* ends, void* dgate, void* dvalue, void* dinitial,
+                           int64_t num_seg, int64_t n, int64_t d, int64_t longest, int has_empty,
+                           void* workspace, int64_t workspace_bytes, int dtype, int gate_dtype,
+                           void* stream);
+
+/* One row of every sequence: next = gate * state + value (state), dst = next in
+ * the values' dtype, for `count` values. `next` may be `state`. */
+int mdgl_segment_scan_step(const void* gate, const void* value, const void* state, void* dst,
+                           void* next, int64_t count, int dtype, int gate_dtype, void* stream);
 
 #ifdef __cplusplus
 }

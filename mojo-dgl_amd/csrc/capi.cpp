@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "../../include/mdgl.h"
+#include "mdgl_half.h"
 #include "mdgl_kernels.h"
 
 using namespace mdgl;
@@ -90,6 +91,10 @@ int hip_status(hipError_t e, const char* what) {
 bool dtype_ok(int dtype) { return dtype == MDGL_FLOAT32 || dtype == MDGL_FLOAT64; }
 int64_t dsize(int dtype) { return dtype == MDGL_FLOAT32 ? 4 : 8; }
 int vec_width(int dtype) { return dtype == MDGL_FLOAT32 ? 4 : 2; }
+
+// The row operators (layer norm, scan, routing) also take the 16-bit types.
+bool row_dtype_ok(int dtype) { return dtype >= MDGL_FLOAT32 && dtype <= MDGL_FLOAT16; }
+bool half_dtype(int dtype) { return dtype == MDGL_BFLOAT16 || dtype == MDGL_FLOAT16; }
 
 bool aligned(const void* p, int64_t bytes) {
   return (reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes) == 0;
@@ -1553,3 +1558,153 @@ extern "C" int mdgl_gspmm_noalloc(const int32_t* indptr, const int32_t* indices,
                       num_chunks, chunk_len, heavy_rows, heavy_ptr, num_heavy, ws,
                       need > 0 ? MDGL_NOALLOC_SCRATCH_BYTES : 0, flags, dtype, stream);
 }
+
+extern "C" {
+
+int mdgl_segment_marks(const int32_t* offsets, int64_t num_seg, int64_t n, int32_t* ids,
+                       uint64_t* starts, uint64_t* ends, void* stream) {
+  MDGL_RANGE();
+  if (num_seg < 0 || n < 0) return fail(MDGL_EINVAL, "segment_marks: negative size");
+  if (n >= (int64_t(1) << 31) || num_seg >= (int64_t(1) << 31))
+    return fail(MDGL_EINVAL, "segment_marks: 2**31 or more rows or segments");
+  if (n == 0) return MDGL_OK;
+  if (num_seg == 0) return fail(MDGL_EINVAL, "segment_marks: rows but no segments");
+  if (!offsets || !ids || !starts || !ends) return fail(MDGL_EINVAL, "segment_marks: null buffer");
+  return hip_status(
+      launch_segment_marks(offsets, num_seg, n, ids, starts, ends, (hipStream_t)stream),
+      "segment_marks");
+}
+
+namespace {
+
+int scan_sizes(const char* what, int64_t num_seg, int64_t n, int64_t d, int64_t longest,
+               int dtype, int gate_dtype) {
+  if (!row_dtype_ok(dtype)) return fail(MDGL_EINVAL, "%s: bad dtype %d", what, dtype);
+  if (gate_dtype != dtype && !(gate_dtype == MDGL_FLOAT32 && half_dtype(dtype)))
+    return fail(MDGL_EINVAL, "%s: gates of dtype %d with values of %d", what, gate_dtype, dtype);
+  if (num_seg < 0 || n < 0 || d < 0 || longest < 0)
+    return fail(MDGL_EINVAL, "%s: negative size", what);
+  if (n >= (int64_t(1) << 31) || num_seg >= (int64_t(1) << 31))
+    return fail(MDGL_EINVAL, "%s: 2**31 or more rows or segments", what);
+  if (!row_widths_fit(d, dtype_bytes(dtype)))
+    return fail(MDGL_EINVAL, "%s: rows of 2 GiB or more", what);
+  if (longest > n) return fail(MDGL_EINVAL, "%s: a segment longer than the rows", what);
+  if (n > 0 && (num_seg == 0 || longest == 0))
+    return fail(MDGL_EINVAL, "%s: rows but no segments", what);
+  return MDGL_OK;
+}
+
+int scan_workspace(const char* what, void* workspace, int64_t have, int64_t n, int64_t d,
+                   int64_t longest, int dtype) {
+  const int64_t need = n > 0 ? scan_workspace_bytes(n, d, longest, dtype) : 0;
+  if (need > 0 && workspace && !aligned(workspace, WS_ALIGN))
+    return fail(MDGL_EINVAL, "workspace must be %lld-byte aligned", (long long)WS_ALIGN);
+  if (need > 0 && (!workspace || have < need))
+    return fail(MDGL_EWORKSPACE, "%s: workspace of %lld bytes needed, %lld given", what,
+                (long long)need, (long long)have);
+  return MDGL_OK;
+}
+
+}  // namespace
+
+int64_t mdgl_segment_scan_workspace_bytes(int64_t n, int64_t d, int64_t longest, int dtype) {
+  if (n < 0 || d < 0 || longest < 0 || !row_dtype_ok(dtype)) return -1;
+  return n == 0 || d == 0 ? 0 : scan_workspace_bytes(n, d, longest, dtype);
+}
+
+int mdgl_segment_scan(const void* gate, const void* value, const void* initial,
+                      const int32_t* offsets, const int32_t* ids, const uint64_t* starts,
+                      const uint64_t* ends, void* dst, void* last, void* marks, int64_t num_seg,
+                      int64_t n, int64_t d, int64_t longest, int has_empty, void* workspace,
+                      int64_t workspace_bytes, int dtype, int gate_dtype, void* stream) {
+  MDGL_RANGE();
+  int rc = scan_sizes("segment_scan", num_seg, n, d, longest, dtype, gate_dtype);
+  if (rc) return rc;
+  if (d == 0 || (n == 0 && !(has_empty && last))) return MDGL_OK;
+  if (n > 0 && (!gate || !value || !ids || !starts || !ends || !dst))
+    return fail(MDGL_EINVAL, "segment_scan: null buffer");
+  if (has_empty && last && !offsets) return fail(MDGL_EINVAL, "segment_scan: null buffer");
+  if ((rc = scan_workspace("segment_scan", workspace, workspace_bytes, n, d, longest, dtype)))
+    return rc;
+  ScanParams q{};
+  q.gate = gate;
+  q.value = value;
+  q.initial = initial;
+  q.offsets = offsets;
+  q.ids = ids;
+  q.starts = starts;
+  q.ends = ends;
+  q.out = dst;
+  q.last = last;
+  q.marks = marks;
+  q.n = n;
+  q.d = d;
+  q.num_seg = num_seg;
+  q.has_empty = has_empty;
+  q.gate_f32 = gate_dtype == MDGL_FLOAT32;
+  q.workspace = workspace;
+  q.stream = (hipStream_t)stream;
+  return hip_status(launch_scan(q, false, longest, dtype), "segment_scan");
+}
+
+int mdgl_segment_scan_grad(const void* gate, const void* value, const void* initial,
+                           const void* marks, const void* grad, const void* grad_last,
+                           const int32_t* offsets, const int32_t* ids, const uint64_t* starts,
+                           const uint64_t* ends, void* dgate, void* dvalue, void* dinitial,
+                           int64_t num_seg, int64_t n, int64_t d, int64_t longest, int has_empty,
+                           void* workspace, int64_t workspace_bytes, int dtype, int gate_dtype,
+                           void* stream) {
+  MDGL_RANGE();
+  int rc = scan_sizes("segment_scan_grad", num_seg, n, d, longest, dtype, gate_dtype);
+  if (rc) return rc;
+  if (d == 0 || (n == 0 && !(has_empty && dinitial))) return MDGL_OK;
+  if (n > 0 && (!gate || !grad || !ids || !starts || !ends || (dgate && (!value || !marks))))
+    return fail(MDGL_EINVAL, "segment_scan_grad: null buffer");
+  if (has_empty && dinitial && !offsets)
+    return fail(MDGL_EINVAL, "segment_scan_grad: null buffer");
+  if ((rc = scan_workspace("segment_scan_grad", workspace, workspace_bytes, n, d, longest, dtype)))
+    return rc;
+  ScanParams q{};
+  q.gate = gate;
+  q.value = value;
+  q.initial = initial;
+  q.grad = grad;
+  q.grad_last = grad_last;
+  q.offsets = offsets;
+  q.ids = ids;
+  q.starts = starts;
+  q.ends = ends;
+  q.marks = const_cast<void*>(marks);
+  q.dgate = dgate;
+  q.dvalue = dvalue;
+  q.dinitial = dinitial;
+  q.n = n;
+  q.d = d;
+  q.num_seg = num_seg;
+  q.has_empty = has_empty;
+  q.gate_f32 = gate_dtype == MDGL_FLOAT32;
+  q.workspace = workspace;
+  q.stream = (hipStream_t)stream;
+  return hip_status(launch_scan(q, true, longest, dtype), "segment_scan_grad");
+}
+
+int mdgl_segment_scan_step(const void* gate, const void* value, const void* state, void* dst,
+                           void* next, int64_t count, int dtype, int gate_dtype, void* stream) {
+  MDGL_RANGE();
+  if (!row_dtype_ok(dtype)) return fail(MDGL_EINVAL, "segment_scan_step: bad dtype %d", dtype);
+  if (gate_dtype != dtype && !(gate_dtype == MDGL_FLOAT32 && half_dtype(dtype)))
+    return fail(MDGL_EINVAL, "segment_scan_step: gates of dtype %d with values of %d", gate_dtype,
+                dtype);
+  if (count < 0) return fail(MDGL_EINVAL, "segment_scan_step: negative size");
+  // one workgroup per BLOCK * 2 values at least
+  if (count > MAX_LAUNCH_BLOCKS * BLOCK)
+    return fail(MDGL_EINVAL, "segment_scan_step: too many values for one launch");
+  if (count == 0) return MDGL_OK;
+  if (!gate || !value || !state || !dst || !next)
+    return fail(MDGL_EINVAL, "segment_scan_step: null buffer");
+  const ScanStepParams q{gate, value, state, dst, next, count, gate_dtype == MDGL_FLOAT32,
+                         (hipStream_t)stream};
+  return hip_status(launch_scan_step(q, dtype), "segment_scan_step");
+}
+
+}  // extern "C"

@@ -1,0 +1,50 @@
+// Element types of the row operators (layer norm, the segment scan, routing):
+// float, double, bfloat16 and float16 in memory; sums, statistics and states in
+// float (double for double). A result is rounded to its type once, to nearest.
+#pragma once
+
+#include "mdgl_common.h"
+
+namespace mdgl {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+template <class T> struct AccOf { using type = float; };
+template <> struct AccOf<double> { using type = double; };
+template <class T> using acc_t = typename AccOf<T>::type;
+
+// Dtype codes of include/mdgl.h.
+enum DType { DT_F32 = 0, DT_F64 = 1, DT_BF16 = 2, DT_F16 = 3 };
+inline int64_t dtype_bytes(int dtype) { return dtype == DT_F64 ? 8 : dtype == DT_F32 ? 4 : 2; }
+
+// Values per 16 bytes of the accumulator type: the columns a lane of the
+// scan or of the row movers holds.
+template <class T> constexpr int acc_vec() { return 16 / (int)sizeof(acc_t<T>); }
+
+__device__ __forceinline__ float fma_of(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fma_of(double a, double b, double c) { return __builtin_fma(a, b, c); }
+
+// N consecutive elements, at element alignment, in the accumulator type.
+template <class T, class A, int N, bool STREAM = false>
+__device__ __forceinline__ void load_acc(const T* p, A (&out)[N]) {
+  T raw[N];
+  load_any<STREAM>(p, raw);
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = (A)raw[i];
+}
+
+template <class T, class A, int N>
+__device__ __forceinline__ void store_acc(T* p, const A (&in)[N]) {
+  if constexpr (N == 1) {
+    *p = (T)in[0];
+  } else {
+    typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    V v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (T)in[i];
+    *reinterpret_cast<V*>(p) = v;
+  }
+}
+
+}  // namespace mdgl

@@ -307,4 +307,58 @@ int64_t segment_offsets_workspace_bytes(int64_t num);
 hipError_t launch_segment_offsets(const int64_t* len, int64_t num, int64_t chunk_len,
                                   int32_t* offsets, int64_t* stats, void* ws, hipStream_t s);
 
+// Gated linear recurrence over segments and its gradients (scan_impl.h;
+// scan_plan.hip for the marks and the geometry).
+struct ScanParams {
+  const void* gate;
+  const void* value;
+  const void* initial;
+  const void* grad;
+  const void* grad_last;
+  const int32_t* offsets;
+  const int32_t* ids;
+  const uint64_t* starts;
+  const uint64_t* ends;
+  void* out;
+  void* last;
+  void* marks;
+  void* dgate;
+  void* dvalue;
+  void* dinitial;
+  int64_t n, d, num_seg;
+  int has_empty, gate_f32;
+  void* workspace;
+  hipStream_t stream;
+};
+// How the rows are cut: walks of `len` rows (a multiple of 16), owning the
+// segments that start in them, or chunks with a carry.
+struct ScanGeometry {
+  bool owners;
+  int64_t len;
+};
+ScanGeometry scan_geometry(int64_t n, int64_t d, int64_t longest, int dtype);
+int64_t scan_workspace_bytes(int64_t n, int64_t d, int64_t longest, int dtype);
+hipError_t launch_scan(const ScanParams& q, bool back, int64_t longest, int dtype);
+hipError_t launch_scan_f32(const ScanParams& q, const ScanGeometry& geo, bool back);
+hipError_t launch_scan_f64(const ScanParams& q, const ScanGeometry& geo, bool back);
+hipError_t launch_scan_bf16(const ScanParams& q, const ScanGeometry& geo, bool back);
+hipError_t launch_scan_f16(const ScanParams& q, const ScanGeometry& geo, bool back);
+struct ScanStepParams {
+  const void* gate;
+  const void* value;
+  const void* state;
+  void* out;
+  void* next;
+  int64_t n;
+  int gate_f32;
+  hipStream_t stream;
+};
+hipError_t launch_scan_step(const ScanStepParams& q, int dtype);
+hipError_t launch_scan_step_f32(const ScanStepParams& q);
+hipError_t launch_scan_step_f64(const ScanStepParams& q);
+hipError_t launch_scan_step_bf16(const ScanStepParams& q);
+hipError_t launch_scan_step_f16(const ScanStepParams& q);
+hipError_t launch_segment_marks(const int32_t* offsets, int64_t num_seg, int64_t n, int32_t* ids,
+                                uint64_t* starts, uint64_t* ends, hipStream_t s);
+
 }  // namespace mdgl

@@ -50,6 +50,7 @@ REDUCERS = {"sum": REDUCE_SUM, "max": REDUCE_MAX, "min": REDUCE_MIN, "mean": RED
 TARGETS = {"u": SRC_CODE, "v": DST_CODE, "e": EDGE_CODE}
 
 FLOAT32, FLOAT64 = 0, 1
+BFLOAT16, FLOAT16 = 2, 3  # row operators only (layer norm, the segment scan, routing)
 REPLACE_INF = 1
 RHS_CSR_ORDER = 2
 LHS_LINE_ROWS = 8  # mdgl_gspmm: lhs rows copied to start on 128-byte lines
@@ -139,6 +140,13 @@ _SIGNATURES = {
     "mdgl_gather_rows": ([_P, _P, _P, _I64, _I64, _C, _P], _C),
     "mdgl_scatter_rows": ([_P, _P, _P, _I64, _I64, _C, _P], _C),
     "mdgl_edge_softmax_grad": ([_P, _P, _P, _P, _P, _I64, _I64, _C, _P], _C),
+    "mdgl_segment_marks": ([_P, _I64, _I64, _P, _P, _P, _P], _C),
+    "mdgl_segment_scan": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _C, _P,
+                           _I64, _C, _C, _P], _C),
+    "mdgl_segment_scan_workspace_bytes": ([_I64, _I64, _I64, _C], _I64),
+    "mdgl_segment_scan_grad": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64,
+                                _I64, _I64, _C, _P, _I64, _C, _C, _P], _C),
+    "mdgl_segment_scan_step": ([_P, _P, _P, _P, _P, _I64, _C, _C, _P], _C),
 }
 
 
@@ -428,6 +436,62 @@ def give_back(t: torch.Tensor, as_torch: bool, dev):
     if as_torch:
         return t if dev is None or t.device == dev else t.to(dev)
     return t.cpu().numpy()
+
+
+# ------------------------------------------------------------------ rows
+# The row operators (layer norm, the segment scan, routing) keep 16-bit types
+# too, with their sums and states in float32.
+ROW_CODES = {torch.float32: FLOAT32, torch.float64: FLOAT64, torch.bfloat16: BFLOAT16,
+             torch.float16: FLOAT16}
+
+
+class Rows:
+    """A validated operand of a row operator: a float32, float64, bfloat16 or
+    float16 tensor (or numpy array, without bfloat16); `dtype` is torch's."""
+
+    __slots__ = ("data", "is_torch", "device", "shape", "dtype")
+
+    def __init__(self, data, is_torch, dev, dtype):
+        self.data = data
+        self.is_torch = is_torch
+        self.device = dev
+        self.shape = tuple(data.shape)
+        self.dtype = dtype
+
+    @property
+    def ndim(self):
+        return len(self.shape)
+
+
+def rows(a) -> Rows:
+    """Validate an operand of a row operator: `feature`, but float16 and
+    bfloat16 stay as they are."""
+    if isinstance(a, torch.Tensor):
+        if a.dtype in ROW_CODES:
+            return Rows(a, True, a.device, a.dtype)
+    else:
+        a = np.asanyarray(a)
+        if a.dtype == np.float16:
+            return Rows(np.ascontiguousarray(a), False, None, torch.float16)
+    f = feature(a)
+    return Rows(f.data, f.is_torch, f.device, torch_dtype(f.dtype))
+
+
+def rows_on_device(r: Rows, dtype: torch.dtype) -> torch.Tensor:
+    """The operand as a contiguous tensor of `dtype` on the current GPU."""
+    dev = device()
+    t = r.data
+    if not r.is_torch:
+        t = torch.from_numpy(t)
+    elif t.dtype == dtype and t.is_cuda and t.get_device() == current_device() \
+            and t.is_contiguous():
+        return t
+    return t.detach().to(device=dev, dtype=dtype).contiguous()
+
+
+def state_dtype(dtype: torch.dtype) -> torch.dtype:
+    """What the row operators keep sums and states of `dtype` values in."""
+    return torch.float64 if dtype == torch.float64 else torch.float32
 
 
 # ------------------------------------------------------------------ ids

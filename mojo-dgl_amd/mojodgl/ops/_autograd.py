@@ -39,7 +39,8 @@ these follow the calculus of the forward ops and run on the same kernels:
 * segment_reduce / segment_softmax: the segments are CSR rows over the value
   rows themselves (``mdgl_segment_ids`` maps rows to segments): sum / mean /
   max / min as gspmm copy_rhs (max / min through the arg row of
-  ``mdgl_segment_reduce_arg``), softmax as edge_softmax.
+  ``mdgl_segment_reduce_arg``), softmax as edge_softmax;
+* segment_scan: the reverse recurrence (``mdgl_segment_scan_grad``).
 
 The backward passes run on the library's kernels, outside torch's graph, so
 they are differentiable once: a second derivative through them raises.
@@ -62,7 +63,7 @@ from .. import _lib
 from ..base import DGLError
 
 __all__ = ["needs_grad", "GSpMM", "GSDDMM", "EdgeSoftmax", "SegmentReduce", "SegmentSoftmax",
-           "SegmentMM", "GatherMM"]
+           "SegmentMM", "GatherMM", "SegmentScan"]
 
 
 def needs_grad(*xs) -> bool:
@@ -633,3 +634,38 @@ class GatherMM(torch.autograd.Function):
         da, db = _grouped_grad(a, b, grad_out, None, ctx.idx, a.shape[0],
                                ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return _back(da, a), _back(db, b), None
+
+
+def _save_some(ctx, *xs):
+    """`_save_operands` for any number of operands."""
+    ctx.save_for_backward(*(x if isinstance(x, torch.Tensor) else None for x in xs))
+    ctx.host = tuple(None if isinstance(x, torch.Tensor) else x for x in xs)
+
+
+def _saved_some(ctx):
+    return tuple(h if t is None else t for t, h in zip(ctx.saved_tensors, ctx.host))
+
+
+class SegmentScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, seglen, gate, value, initial, return_state):
+        from .scan import _scan
+
+        # the states in front of every 16th row serve the gates' gradient
+        h, last, marks, plan, back = _scan(seglen, gate, value, initial, return_state, True)
+        ctx.plan, ctx.marks = plan, marks
+        ctx.set_materialize_grads(False)
+        _save_some(ctx, gate, value, initial)
+        return back(h), back(last) if return_state else None
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, grad_last):
+        from .scan import _scan_grad
+
+        gate, value, initial = _saved_some(ctx)
+        if grad is None and grad_last is None:
+            return None, None, None, None, None
+        dg, dv, di = _scan_grad(ctx.plan, gate, value, initial, ctx.marks, grad, grad_last,
+                                ctx.needs_input_grad[1:4])
+        return None, _back(dg, gate), _back(dv, value), _back(di, initial), None

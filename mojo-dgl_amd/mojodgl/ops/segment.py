@@ -51,7 +51,7 @@ class _Segments:
     were a GPU tensor, whose offsets are formed and checked on the GPU with
     one small read back), `heavy` the number of chunks of `chunk_len` rows
     the segments longer than `chunk_len` split into (GPU lengths only),
-    `longest` the largest length.
+    `longest` the largest length, `shortest` the smallest (0 without any).
 
     With `defer` the checks of GPU lengths come back later: the caller may
     queue kernels that read the offsets (they clamp every offset into the
@@ -96,6 +96,7 @@ class _Segments:
             self.num = sl.size
             _check_lengths(sl, n)
             self.longest = int(sl.max()) if sl.size else 0
+            self.shortest = int(sl.min()) if sl.size else 0
             self.host = _offsets(sl)
             _check_offsets(self.host, n)
             self.off = None
@@ -110,7 +111,7 @@ class _Segments:
                 "[{}, {}] summing to {}".format(n, low, high, total))
         if self._chunked:
             self.heavy = heavy
-        self.longest = high
+        self.longest, self.shortest = high, low
 
     def start_check(self):
         """Start the read back of a deferred check (after the caller queued
