@@ -14,7 +14,10 @@ from .convert import graph  # noqa: F401
 from .function import *  # noqa: F401,F403
 from .heterograph import DGLGraph  # noqa: F401
 from .ops import *  # noqa: F401,F403
+from .ops import row_ops as _row_ops
 from .udf import EdgeBatch, NodeBatch  # noqa: F401
+
+globals().update({name: getattr(ops, name) for name in _row_ops})
 
 __version__ = "0.1.0"
 
@@ -22,4 +25,4 @@ __all__ = [
     "DGLGraph", "graph", "DGLError", "ALL", "EID", "ETYPE", "NID", "NTYPE",
     "EdgeBatch", "NodeBatch", "build",
     "function", "ops", "nn",
-] + ops.__all__
+] + ops.__all__ + _row_ops

@@ -22,5 +22,8 @@ __all__ = (
     + _sddmm_mod.__all__
     + _seg_mod.__all__
     + _spmm_mod.__all__
-    + _scan_mod.__all__
 )
+
+# Operators over packed rows without a counterpart in the reference: `__all__`
+# above keeps to its names.
+row_ops = list(_scan_mod.__all__)
