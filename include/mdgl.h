@@ -642,6 +642,25 @@ int mdgl_segment_scan_grad(const void* gate, const void* value, const void* init
 int mdgl_segment_scan_step(const void* gate, const void* value, const void* state, void* dst,
                            void* next, int64_t count, int dtype, int gate_dtype, void* stream);
 
+/* Layer norm over the d columns of each of n rows:
+ *   dst = (value - mean) * rstd * weight + bias,
+ *   rstd = 1 / sqrt(mean((value - mean)^2) + eps)
+ * weight / bias: d values in the rows' dtype, or MDGL_FLOAT32 with rows of 16
+ * bits; null: 1 / 0. mean, rstd (state, n each, both or neither) receive the
+ * statistics that the gradient takes. */
+int mdgl_layer_norm(const void* value, const void* weight, const void* bias, void* dst, void* mean,
+                    void* rstd, int64_t n, int64_t d, double eps, int dtype, int weight_dtype,
+                    void* stream);
+
+/* Gradients of mdgl_layer_norm from that of dst: dvalue (rows' dtype), dweight
+ * and dbias (weight_dtype), each nullable; the workspace is needed for the last
+ * two (summed over the rows in a fixed order). Nothing is written when n is 0. */
+int mdgl_layer_norm_grad(const void* value, const void* weight, const void* mean, const void* rstd,
+                         const void* grad, void* dvalue, void* dweight, void* dbias, int64_t n,
+                         int64_t d, void* workspace, int64_t workspace_bytes, int dtype,
+                         int weight_dtype, void* stream);
+int64_t mdgl_layer_norm_grad_workspace_bytes(int64_t n, int64_t d, int dtype);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1707,4 +1707,81 @@ int mdgl_segment_scan_step(const void* gate, const void* value, const void* stat
   return hip_status(launch_scan_step(q, dtype), "segment_scan_step");
 }
 
+namespace {
+
+int norm_common(const char* what, int64_t n, int64_t d, int dtype, int weight_dtype) {
+  if (!row_dtype_ok(dtype)) return fail(MDGL_EINVAL, "%s: bad dtype %d", what, dtype);
+  if (weight_dtype != dtype && !(weight_dtype == MDGL_FLOAT32 && half_dtype(dtype)))
+    return fail(MDGL_EINVAL, "%s: weights of dtype %d with rows of %d", what, weight_dtype, dtype);
+  if (n < 0 || d < 0) return fail(MDGL_EINVAL, "%s: negative size", what);
+  if (!row_widths_fit(d, dtype_bytes(dtype)))
+    return fail(MDGL_EINVAL, "%s: rows of 2 GiB or more", what);
+  return MDGL_OK;
+}
+
+}  // namespace
+
+int mdgl_layer_norm(const void* value, const void* weight, const void* bias, void* dst, void* mean,
+                    void* rstd, int64_t n, int64_t d, double eps, int dtype, int weight_dtype,
+                    void* stream) {
+  MDGL_RANGE();
+  if (int rc = norm_common("layer_norm", n, d, dtype, weight_dtype)) return rc;
+  if (!(eps >= 0)) return fail(MDGL_EINVAL, "layer_norm: eps must be >= 0");
+  if (!mean != !rstd)
+    return fail(MDGL_EINVAL, "layer_norm: `mean` and `rstd` come together or not at all");
+  if (n == 0 || d == 0) return MDGL_OK;
+  if (!value || !dst) return fail(MDGL_EINVAL, "layer_norm: null buffer");
+  NormParams q{};
+  q.x = value;
+  q.w = weight;
+  q.b = bias;
+  q.y = dst;
+  q.mean = mean;
+  q.rstd = rstd;
+  q.n = n;
+  q.d = d;
+  q.eps = eps;
+  q.weight_f32 = weight_dtype == MDGL_FLOAT32;
+  q.stream = (hipStream_t)stream;
+  return hip_status(launch_norm(q, dtype), "layer_norm");
+}
+
+int64_t mdgl_layer_norm_grad_workspace_bytes(int64_t n, int64_t d, int dtype) {
+  if (n < 0 || d < 0 || !row_dtype_ok(dtype)) return -1;
+  return n == 0 || d == 0 ? 0 : norm_workspace_bytes(n, d, dtype);
+}
+
+int mdgl_layer_norm_grad(const void* value, const void* weight, const void* mean, const void* rstd,
+                         const void* grad, void* dvalue, void* dweight, void* dbias, int64_t n,
+                         int64_t d, void* workspace, int64_t workspace_bytes, int dtype,
+                         int weight_dtype, void* stream) {
+  MDGL_RANGE();
+  if (int rc = norm_common("layer_norm_grad", n, d, dtype, weight_dtype)) return rc;
+  if (n == 0 || d == 0) return MDGL_OK;
+  if (!dvalue && !dweight && !dbias) return MDGL_OK;
+  if (!value || !mean || !rstd || !grad)
+    return fail(MDGL_EINVAL, "layer_norm_grad: null buffer");
+  const int64_t need = dweight || dbias ? norm_workspace_bytes(n, d, dtype) : 0;
+  if (need > 0 && workspace && !aligned(workspace, WS_ALIGN))
+    return fail(MDGL_EINVAL, "workspace must be %lld-byte aligned", (long long)WS_ALIGN);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(MDGL_EWORKSPACE, "layer_norm_grad: workspace of %lld bytes needed, %lld given",
+                (long long)need, (long long)workspace_bytes);
+  NormParams q{};
+  q.x = value;
+  q.w = weight;
+  q.dy = grad;
+  q.dx = dvalue;
+  q.dw = dweight;
+  q.db = dbias;
+  q.mean = const_cast<void*>(mean);
+  q.rstd = const_cast<void*>(rstd);
+  q.n = n;
+  q.d = d;
+  q.weight_f32 = weight_dtype == MDGL_FLOAT32;
+  q.workspace = workspace;
+  q.stream = (hipStream_t)stream;
+  return hip_status(launch_norm(q, dtype), "layer_norm_grad");
+}
+
 }  // extern "C"

@@ -361,4 +361,38 @@ hipError_t launch_scan_step_f16(const ScanStepParams& q);
 hipError_t launch_segment_marks(const int32_t* offsets, int64_t num_seg, int64_t n, int32_t* ids,
                                 uint64_t* starts, uint64_t* ends, hipStream_t s);
 
+// Layer norm (norm_impl.h; norm_plan.hip for the geometry); the gradients when
+// `dy` is given.
+struct NormParams {
+  const void* x;
+  const void* w;
+  const void* b;
+  const void* dy;
+  void* y;
+  void* dx;
+  void* dw;
+  void* db;
+  void* mean;
+  void* rstd;
+  int64_t n, d;
+  double eps;
+  int weight_f32;
+  void* workspace;
+  hipStream_t stream;
+};
+// shape: the instance (threads a row, vectors a thread); parts: the gradient's
+// workgroups, whose sums of dw and db are added afterwards.
+struct NormGeometry {
+  int shape;
+  int64_t parts;
+};
+NormGeometry norm_geometry(int64_t n, int64_t d, int size);
+int64_t norm_most_blocks(int threads);
+int64_t norm_workspace_bytes(int64_t n, int64_t d, int dtype);
+hipError_t launch_norm(const NormParams& q, int dtype);
+hipError_t launch_norm_f32(const NormParams& q);
+hipError_t launch_norm_f64(const NormParams& q);
+hipError_t launch_norm_bf16(const NormParams& q);
+hipError_t launch_norm_f16(const NormParams& q);
+
 }  // namespace mdgl

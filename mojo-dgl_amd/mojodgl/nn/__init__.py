@@ -1,3 +1,4 @@
-"""Neural-network helpers (only `functional.edge_softmax`, as the reference)."""
+"""Neural-network helpers: `functional.edge_softmax`, as the reference, and
+`functional.layer_norm`."""
 
 from . import functional  # noqa: F401

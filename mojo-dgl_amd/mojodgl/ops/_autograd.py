@@ -40,7 +40,9 @@ these follow the calculus of the forward ops and run on the same kernels:
   rows themselves (``mdgl_segment_ids`` maps rows to segments): sum / mean /
   max / min as gspmm copy_rhs (max / min through the arg row of
   ``mdgl_segment_reduce_arg``), softmax as edge_softmax;
-* segment_scan: the reverse recurrence (``mdgl_segment_scan_grad``).
+* segment_scan: the reverse recurrence (``mdgl_segment_scan_grad``);
+* layer_norm: dx and the sums of the weights' gradients in one pass
+  (``mdgl_layer_norm_grad``).
 
 The backward passes run on the library's kernels, outside torch's graph, so
 they are differentiable once: a second derivative through them raises.
@@ -63,7 +65,7 @@ from .. import _lib
 from ..base import DGLError
 
 __all__ = ["needs_grad", "GSpMM", "GSDDMM", "EdgeSoftmax", "SegmentReduce", "SegmentSoftmax",
-           "SegmentMM", "GatherMM", "SegmentScan"]
+           "SegmentMM", "GatherMM", "SegmentScan", "LayerNorm"]
 
 
 def needs_grad(*xs) -> bool:
@@ -669,3 +671,24 @@ class SegmentScan(torch.autograd.Function):
         dg, dv, di = _scan_grad(ctx.plan, gate, value, initial, ctx.marks, grad, grad_last,
                                 ctx.needs_input_grad[1:4])
         return None, _back(dg, gate), _back(dv, value), _back(di, initial), None
+
+
+class LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, value, weight, bias, eps):
+        from .norm import _layer_norm
+
+        y, mean, rstd, back = _layer_norm(value, weight, bias, eps, True)
+        ctx.stats = mean, rstd
+        _save_some(ctx, value, weight, bias)
+        return back(y)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        from .norm import _layer_norm_grad
+
+        value, weight, bias = _saved_some(ctx)
+        dx, dw, db = _layer_norm_grad(value, weight, bias, *ctx.stats, grad,
+                                      ctx.needs_input_grad[:3])
+        return _back(dx, value), _back(dw, weight), _back(db, bias), None
