@@ -661,6 +661,59 @@ int mdgl_layer_norm_grad(const void* value, const void* weight, const void* mean
                          int weight_dtype, void* stream);
 int64_t mdgl_layer_norm_grad_workspace_bytes(int64_t n, int64_t d, int dtype);
 
+/* Routing rows to experts. For each of n rows of num_experts logits (at most
+ * 2048), the k (at most 32) experts of the largest keys, falling, the lowest index
+ * among equals, into ids, and their weights (state). Scores: softmax or sigmoid of
+ * the logits; keys: score + bias (state, num_experts; null: the order of the
+ * logits). With topk_groups < num_groups the experts of the best groups only
+ * (num_experts / num_groups neighbours each; num_groups at most 64), by the largest
+ * key of a group or the sum of its two largest. weights = scale * score, divided by
+ * the sum of the row's k scores with `renormalize`. A logit of -inf masks its
+ * expert: it is chosen only when nothing else is left, with a weight of 0. A row
+ * with a NaN or +inf has NaN among its weights, and ids in range. */
+#define MDGL_SCORE_SOFTMAX 0
+#define MDGL_SCORE_SIGMOID 1
+#define MDGL_GROUP_MAX 0
+#define MDGL_GROUP_TOP2 1
+int mdgl_topk_route(const void* logits, const void* bias, void* weights, int64_t* ids, int64_t n,
+                    int64_t num_experts, int64_t k, int score, int64_t num_groups,
+                    int64_t topk_groups, int group_score, int renormalize, double scale, int dtype,
+                    void* stream);
+
+/* Gradient of the weights (grad: state, [n][k]) in the logits; ids as
+ * mdgl_topk_route wrote them (others outside the experts are skipped). */
+int mdgl_topk_route_grad(const void* logits, const int64_t* ids, const void* grad, void* dlogits,
+                         int64_t n, int64_t num_experts, int64_t k, int score, int renormalize,
+                         double scale, int dtype, void* stream);
+
+/* num_entries ids (n rows times k experts, row by row) in the order of their
+ * experts, each expert's in entry order: seglen[e] the entries of expert e,
+ * order[p] the entry at place p, slot[i] the place of entry i. Entries whose id is
+ * outside [0, num_experts) come behind all others, and their slot is the
+ * complement (~) of their place. num_experts: at most 2048. */
+int mdgl_route_plan(const int64_t* ids, int64_t num_entries, int64_t num_experts, int64_t* seglen,
+                    int32_t* order, int32_t* slot, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+int64_t mdgl_route_plan_workspace_bytes(int64_t num_entries, int64_t num_experts);
+
+/* dst[slot[t][j]] = src[t] for the n rows of src (d columns) and their k slots; a
+ * complemented slot's row is zeros. dst has n * k rows, all of them written. */
+int mdgl_dispatch_rows(const void* src, const int32_t* slot, void* dst, int64_t n, int64_t k,
+                       int64_t d, int dtype, void* stream);
+
+/* dst[t] = sum over j of weights[t][j] * src[slot[t][j]], in j's order, in the
+ * state's type (weights: state, null: 1); complemented slots add nothing. Without
+ * weights it is the gradient of mdgl_dispatch_rows. */
+int mdgl_combine_rows(const void* src, const int32_t* slot, const void* weights, void* dst,
+                      int64_t n, int64_t k, int64_t d, int dtype, void* stream);
+
+/* Gradients of mdgl_combine_rows from that of dst: dsrc[slot] = weights * grad
+ * (zeros at complemented slots) and dweights = <grad[t], src[slot]> (0 there),
+ * each nullable. */
+int mdgl_combine_rows_grad(const void* src, const int32_t* slot, const void* weights,
+                           const void* grad, void* dsrc, void* dweights, int64_t n, int64_t k,
+                           int64_t d, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1784,4 +1784,154 @@ int mdgl_layer_norm_grad(const void* value, const void* weight, const void* mean
   return hip_status(launch_norm(q, dtype), "layer_norm_grad");
 }
 
+namespace {
+
+int route_common(const char* what, int64_t n, int64_t e, int64_t k, int score, int dtype) {
+  if (!row_dtype_ok(dtype)) return fail(MDGL_EINVAL, "%s: bad dtype %d", what, dtype);
+  if (n < 0) return fail(MDGL_EINVAL, "%s: negative size", what);
+  if (e < 1 || e > ROUTE_MAX_EXPERTS)
+    return fail(MDGL_EINVAL, "%s: 1 to %d experts, got %lld", what, ROUTE_MAX_EXPERTS,
+                (long long)e);
+  if (k < 1 || k > ROUTE_MAX_K || k > e)
+    return fail(MDGL_EINVAL, "%s: 1 to %d of the experts a row, got %lld of %lld", what,
+                ROUTE_MAX_K, (long long)k, (long long)e);
+  if (score != MDGL_SCORE_SOFTMAX && score != MDGL_SCORE_SIGMOID)
+    return fail(MDGL_EINVAL, "%s: bad score %d", what, score);
+  return MDGL_OK;
+}
+
+int move_common(const char* what, int64_t n, int64_t k, int64_t d, int dtype) {
+  if (!row_dtype_ok(dtype)) return fail(MDGL_EINVAL, "%s: bad dtype %d", what, dtype);
+  if (n < 0 || k < 0 || d < 0) return fail(MDGL_EINVAL, "%s: negative size", what);
+  if (n >= (int64_t(1) << 31) || k >= (int64_t(1) << 31) || n * k >= (int64_t(1) << 31))
+    return fail(MDGL_EINVAL, "%s: 2**31 or more entries", what);
+  if (!row_widths_fit(d, dtype_bytes(dtype)))
+    return fail(MDGL_EINVAL, "%s: rows of 2 GiB or more", what);
+  return MDGL_OK;
+}
+
+}  // namespace
+
+int mdgl_topk_route(const void* logits, const void* bias, void* weights, int64_t* ids, int64_t n,
+                    int64_t num_experts, int64_t k, int score, int64_t num_groups,
+                    int64_t topk_groups, int group_score, int renormalize, double scale, int dtype,
+                    void* stream) {
+  MDGL_RANGE();
+  if (int rc = route_common("topk_route", n, num_experts, k, score, dtype)) return rc;
+  if (num_groups < 1 || num_groups > ROUTE_MAX_GROUPS || num_experts % num_groups)
+    return fail(MDGL_EINVAL, "topk_route: 1 to %d groups that divide the experts, got %lld of %lld",
+                ROUTE_MAX_GROUPS, (long long)num_groups, (long long)num_experts);
+  if (topk_groups < 1 || topk_groups > num_groups)
+    return fail(MDGL_EINVAL, "topk_route: %lld of %lld groups", (long long)topk_groups,
+                (long long)num_groups);
+  if (k > topk_groups * (num_experts / num_groups))
+    return fail(MDGL_EINVAL, "topk_route: %lld experts a row of the %lld of its groups",
+                (long long)k, (long long)(topk_groups * (num_experts / num_groups)));
+  if (group_score != MDGL_GROUP_MAX && group_score != MDGL_GROUP_TOP2)
+    return fail(MDGL_EINVAL, "topk_route: bad group score %d", group_score);
+  if (n == 0) return MDGL_OK;
+  if (!logits || !weights || !ids) return fail(MDGL_EINVAL, "topk_route: null buffer");
+  RouteParams q{};
+  q.logits = logits;
+  q.bias = bias;
+  q.weights = weights;
+  q.ids = ids;
+  q.n = n;
+  q.e = (int)num_experts;
+  q.k = (int)k;
+  q.groups = (int)num_groups;
+  q.topk_groups = (int)topk_groups;
+  q.sigmoid = score == MDGL_SCORE_SIGMOID;
+  q.top2 = group_score == MDGL_GROUP_TOP2;
+  q.renorm = renormalize;
+  q.scale = scale;
+  q.stream = (hipStream_t)stream;
+  return hip_status(launch_route(q, dtype), "topk_route");
+}
+
+int mdgl_topk_route_grad(const void* logits, const int64_t* ids, const void* grad, void* dlogits,
+                         int64_t n, int64_t num_experts, int64_t k, int score, int renormalize,
+                         double scale, int dtype, void* stream) {
+  MDGL_RANGE();
+  if (int rc = route_common("topk_route_grad", n, num_experts, k, score, dtype)) return rc;
+  if (n == 0) return MDGL_OK;
+  if (!logits || !ids || !grad || !dlogits)
+    return fail(MDGL_EINVAL, "topk_route_grad: null buffer");
+  RouteParams q{};
+  q.logits = logits;
+  q.ids = const_cast<int64_t*>(ids);
+  q.dweights = grad;
+  q.dlogits = dlogits;
+  q.n = n;
+  q.e = (int)num_experts;
+  q.k = (int)k;
+  q.groups = q.topk_groups = 1;
+  q.sigmoid = score == MDGL_SCORE_SIGMOID;
+  q.renorm = renormalize;
+  q.scale = scale;
+  q.stream = (hipStream_t)stream;
+  return hip_status(launch_route(q, dtype), "topk_route_grad");
+}
+
+int64_t mdgl_route_plan_workspace_bytes(int64_t num_entries, int64_t num_experts) {
+  if (num_entries < 0 || num_entries >= (int64_t(1) << 31) || num_experts < 1 ||
+      num_experts > ROUTE_MAX_EXPERTS)
+    return -1;
+  return route_plan_workspace_bytes(num_entries, (int)num_experts);
+}
+
+int mdgl_route_plan(const int64_t* ids, int64_t num_entries, int64_t num_experts, int64_t* seglen,
+                    int32_t* order, int32_t* slot, void* workspace, int64_t workspace_bytes,
+                    void* stream) {
+  MDGL_RANGE();
+  if (num_entries < 0 || num_entries >= (int64_t(1) << 31))
+    return fail(MDGL_EINVAL, "route_plan: 0 to 2**31 - 1 entries");
+  if (num_experts < 1 || num_experts > ROUTE_MAX_EXPERTS)
+    return fail(MDGL_EINVAL, "route_plan: 1 to %d experts, got %lld", ROUTE_MAX_EXPERTS,
+                (long long)num_experts);
+  if (!seglen || (num_entries > 0 && (!ids || !order || !slot)))
+    return fail(MDGL_EINVAL, "route_plan: null buffer");
+  const int64_t need = route_plan_workspace_bytes(num_entries, (int)num_experts);
+  if (need > 0 && workspace && !aligned(workspace, WS_ALIGN))
+    return fail(MDGL_EINVAL, "workspace must be %lld-byte aligned", (long long)WS_ALIGN);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(MDGL_EWORKSPACE, "route_plan: workspace of %lld bytes needed, %lld given",
+                (long long)need, (long long)workspace_bytes);
+  return hip_status(launch_route_plan(ids, num_entries, (int)num_experts, seglen, order, slot,
+                                      workspace, (hipStream_t)stream),
+                    "route_plan");
+}
+
+int mdgl_dispatch_rows(const void* src, const int32_t* slot, void* dst, int64_t n, int64_t k,
+                       int64_t d, int dtype, void* stream) {
+  MDGL_RANGE();
+  if (int rc = move_common("dispatch_rows", n, k, d, dtype)) return rc;
+  if (n == 0 || k == 0 || d == 0) return MDGL_OK;
+  if (!src || !slot || !dst) return fail(MDGL_EINVAL, "dispatch_rows: null buffer");
+  const MoveParams q{src, slot, nullptr, nullptr, dst, nullptr, n, d, (int)k, (hipStream_t)stream};
+  return hip_status(launch_move(q, MOVE_DISPATCH, dtype), "dispatch_rows");
+}
+
+int mdgl_combine_rows(const void* src, const int32_t* slot, const void* weights, void* dst,
+                      int64_t n, int64_t k, int64_t d, int dtype, void* stream) {
+  MDGL_RANGE();
+  if (int rc = move_common("combine_rows", n, k, d, dtype)) return rc;
+  if (n == 0 || d == 0) return MDGL_OK;
+  if (!dst || (k > 0 && (!src || !slot))) return fail(MDGL_EINVAL, "combine_rows: null buffer");
+  const MoveParams q{src, slot, weights, nullptr, dst, nullptr, n, d, (int)k, (hipStream_t)stream};
+  return hip_status(launch_move(q, MOVE_COMBINE, dtype), "combine_rows");
+}
+
+int mdgl_combine_rows_grad(const void* src, const int32_t* slot, const void* weights,
+                           const void* grad, void* dsrc, void* dweights, int64_t n, int64_t k,
+                           int64_t d, int dtype, void* stream) {
+  MDGL_RANGE();
+  if (int rc = move_common("combine_rows_grad", n, k, d, dtype)) return rc;
+  if (n == 0 || k == 0 || d == 0 || (!dsrc && !dweights)) return MDGL_OK;
+  if (!slot || !weights || !grad || (dweights && !src))
+    return fail(MDGL_EINVAL, "combine_rows_grad: null buffer");
+  const MoveParams q{src, slot, weights, grad, dsrc, dweights, n, d, (int)k, (hipStream_t)stream};
+  return hip_status(launch_move(q, MOVE_COMBINE_GRAD, dtype), "combine_rows_grad");
+}
+
 }  // extern "C"

@@ -34,17 +34,26 @@ __device__ __forceinline__ void load_acc(const T* p, A (&out)[N]) {
   for (int i = 0; i < N; ++i) out[i] = (A)raw[i];
 }
 
-template <class T, class A, int N>
-__device__ __forceinline__ void store_acc(T* p, const A (&in)[N]) {
+// N consecutive elements at element alignment.
+template <class T, int N>
+__device__ __forceinline__ void store_any(T* p, const T (&in)[N]) {
   if constexpr (N == 1) {
-    *p = (T)in[0];
+    *p = in[0];
   } else {
     typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
     V v;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = (T)in[i];
+    for (int i = 0; i < N; ++i) v[i] = in[i];
     *reinterpret_cast<V*>(p) = v;
   }
+}
+
+template <class T, class A, int N>
+__device__ __forceinline__ void store_acc(T* p, const A (&in)[N]) {
+  T out[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = (T)in[i];
+  store_any(p, out);
 }
 
 }  // namespace mdgl

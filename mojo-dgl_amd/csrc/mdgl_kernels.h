@@ -395,4 +395,45 @@ hipError_t launch_norm_f64(const NormParams& q);
 hipError_t launch_norm_bf16(const NormParams& q);
 hipError_t launch_norm_f16(const NormParams& q);
 
+// Routing to experts (route_impl.h); the weights' gradient when `dlogits` is given.
+constexpr int ROUTE_MAX_EXPERTS = 2048;
+constexpr int ROUTE_MAX_K = 32;
+constexpr int ROUTE_MAX_GROUPS = 64;
+struct RouteParams {
+  const void* logits;
+  const void* bias;
+  void* weights;
+  int64_t* ids;
+  const void* dweights;
+  void* dlogits;
+  int64_t n;
+  int e, k, groups, topk_groups, sigmoid, top2, renorm;
+  double scale;
+  hipStream_t stream;
+};
+hipError_t launch_route(const RouteParams& q, int dtype);
+hipError_t launch_route_f32(const RouteParams& q);
+hipError_t launch_route_f64(const RouteParams& q);
+hipError_t launch_route_bf16(const RouteParams& q);
+hipError_t launch_route_f16(const RouteParams& q);
+
+// Entries (n rows times k experts) put in the order of their experts, and rows
+// moved there and back (experts.hip).
+int64_t route_plan_workspace_bytes(int64_t m, int experts);
+hipError_t launch_route_plan(const int64_t* ids, int64_t m, int experts, int64_t* seglen,
+                             int32_t* order, int32_t* slot, void* workspace, hipStream_t s);
+enum MoveKind { MOVE_DISPATCH, MOVE_COMBINE, MOVE_COMBINE_GRAD };
+struct MoveParams {
+  const void* src;
+  const int32_t* slot;
+  const void* weights;
+  const void* grad;
+  void* dst;
+  void* dweights;
+  int64_t n, d;
+  int k;
+  hipStream_t stream;
+};
+hipError_t launch_move(const MoveParams& q, MoveKind kind, int dtype);
+
 }  // namespace mdgl

@@ -1,0 +1,403 @@
+// Routing rows to experts (included once per type): scores, the choice of k
+// experts a row, their weights, and the weights' gradient.
+//
+//   s = softmax(x) or sigmoid(x) over a row's E logits x
+//   key = s + bias, or x itself without a bias (both scores grow with x)
+//   groups of E / groups neighbouring experts: the topk_groups best by their
+//   largest key, or by the sum of their two largest, stay
+//   ids = the k largest keys in falling order, the lowest index among equals
+//   w = scale * s[ids], divided by their sum when renormalised
+//
+// A logit of -inf masks its expert: its key is below every other (as is that of a
+// NaN), and its weight is 0. A row needs G lanes (16, or 32 and 64 for many
+// experts or choices), each holding R neighbouring experts, so the lowest index
+// among equals is the lowest lane's. A round of the choice is a maximum over the
+// lane, over the group by DPP, and the lowest index that has it; lane j keeps the
+// j-th choice.
+//
+// With a bias the order of two keys can hang on their last bits. The float pass
+// therefore makes one choice more than asked for, and a row two of whose
+// neighbouring keys (or whose last kept and first dropped group) lie closer than
+// the float keys can be wrong is chosen again in double, as a whole wavefront.
+// Keys of equal logits and biases need no second look: they are equal however
+// they are formed.
+#pragma once
+
+#include "mdgl_half.h"
+#include "mdgl_kernels.h"
+
+namespace mdgl {
+
+template <class T>
+struct RouteArgs {
+  using A = acc_t<T>;
+  const T* logits;  // [n][e]
+  const A* bias;    // [e], may be null
+  A* weights;       // [n][k]
+  int64_t* ids;     // [n][k]
+  int64_t n;
+  int e, k, groups, topk_groups;  // groups = 1: no choice of groups
+  int sigmoid, top2, renorm;
+  A scale;
+  const A* dweights;  // backward
+  T* dlogits;
+};
+
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ float abs_of(float x) { return fabsf(x); }
+__device__ __forceinline__ double abs_of(double x) { return fabs(x); }
+template <class K> __device__ __forceinline__ K lowest() { return -K(__builtin_huge_val()); }
+
+template <class K>
+__device__ __forceinline__ K sigmoid_of(K x) { return K(1) / (K(1) + exp_of(-x)); }
+
+// Maximum / minimum over G lanes, in all of them. No value is NaN.
+template <int G, class K>
+__device__ __forceinline__ K lanes_max(K v) {
+  auto up = [](K a, K b) { return a > b ? a : b; };
+  v = up(v, lane_xor_dpp(v, 0));
+  v = up(v, lane_xor_dpp(v, 1));
+  v = up(v, lane_xor_dpp(v, 2));
+  v = up(v, lane_xor_dpp(v, 3));
+  if constexpr (G > 16) v = up(v, __shfl_xor(v, 16));
+  if constexpr (G > 32) v = up(v, __shfl_xor(v, 32));
+  return v;
+}
+
+template <int G>
+__device__ __forceinline__ int lanes_min(int v) { return -lanes_max<G>(-v); }
+
+// The larger two of two pairs (a >= b in each).
+template <class K>
+__device__ __forceinline__ void join_two(K& a, K& b, K c, K d) {
+  const K lo = a < c ? a : c;
+  a = a > c ? a : c;
+  b = b > d ? b : d;
+  b = b > lo ? b : lo;
+}
+
+template <class K>
+struct Choice {
+  int id;    // lane j: the j-th choice
+  K key;     // and its key
+  K top, sum;  // softmax: the row's largest logit, the sum of exp(x - top)
+  bool near;   // the choice of groups hangs on the last bits
+};
+
+// The first `count` choices of a row (count <= G), keys formed in K.
+template <class K, class T, int G, int R>
+__device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T* x, int count) {
+  const int lane = threadIdx.x % G;
+  const int per = (p.e + G - 1) / G, base = lane * per;
+  const int have = base >= p.e ? 0 : (p.e - base < per ? p.e - base : per);
+  K key[R];
+  uint32_t gone = 0;  // experts not to be chosen (any more)
+#pragma unroll
+  for (int i = 0; i < R; i += 4) {
+    if (i + 4 <= have) {
+      T v[4];
+      load_any<false>(x + base + i, v);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) key[i + q] = (K)v[q];
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        key[i + q] = i + q < have ? (K)x[base + i + q] : lowest<K>();
+        if (i + q >= have) gone |= 1u << (i + q);
+      }
+    }
+  }
+  Choice<K> c;
+  c.top = lowest<K>();
+  c.sum = K(0);
+  c.near = false;
+  c.id = 0;
+  c.key = lowest<K>();
+  if (!p.sigmoid && (p.bias || !p.renorm)) {
+    // the row's softmax statistics; a NaN goes into the sum
+#pragma unroll
+    for (int i = 0; i < R; ++i) c.top = key[i] > c.top ? key[i] : c.top;
+    c.top = lanes_max<G>(c.top);
+    if (c.top > lowest<K>()) {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (!(gone >> i & 1)) c.sum += exp_of(key[i] - c.top);
+      c.sum = group_sum(c.sum, G);
+    }
+  }
+  K most = K(1);  // no score is larger
+  if (p.bias) {
+    const K part = c.sum > K(0) ? K(1) / c.sum : K(0);
+    if (!p.sigmoid) most = part;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (gone >> i & 1 || key[i] == lowest<K>()) continue;
+      const K s = p.sigmoid ? sigmoid_of(key[i]) : exp_of(key[i] - c.top) * part;
+      key[i] = s + (K)p.bias[base + i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) key[i] = key[i] != key[i] ? lowest<K>() : key[i];
+
+  if (p.groups > 1) {
+    const int size = p.e / p.groups;
+    K mark = lowest<K>();  // lane j: the mark of group j
+    K big = K(0);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      big = key[i] > lowest<K>() && abs_of(key[i]) > big ? abs_of(key[i]) : big;
+    big = lanes_max<G>(big);
+    auto grade = [&](K a, K b) { return p.top2 && b > lowest<K>() ? a + b : a; };
+    const int span = size / per;  // lanes a group, when its border is a lane's
+    const bool whole = size == span * per && (span & (span - 1)) == 0;
+    int mine = lane / (whole ? span : 1);  // the group of all of the lane's experts
+    if (whole) {
+      K a = lowest<K>(), b = lowest<K>();
+#pragma unroll
+      for (int i = 0; i < R; ++i) join_two(a, b, key[i], lowest<K>());
+      for (int off = 1; off < span; off <<= 1) {
+        const K oa = __shfl_xor(a, off), ob = __shfl_xor(b, off);
+        join_two(a, b, oa, ob);
+      }
+      mark = grade(a, b);
+      mark = __shfl(mark, lane * span < G ? lane * span : 0, G);
+      if (lane >= p.groups) mark = lowest<K>();
+    } else {
+      for (int g = 0; g < p.groups; ++g) {
+        K a = lowest<K>(), b = lowest<K>();
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const int e = base + i - g * size;
+          join_two(a, b, i < have && e >= 0 && e < size ? key[i] : lowest<K>(), lowest<K>());
+        }
+#pragma unroll
+        for (int off = 1; off < G; off <<= 1) {
+          const K oa = __shfl_xor(a, off), ob = __shfl_xor(b, off);
+          join_two(a, b, oa, ob);
+        }
+        if (lane == g) mark = grade(a, b);
+      }
+    }
+    uint64_t kept = 0;
+    bool open = lane < p.groups;
+    K last = K(0);
+    for (int j = 0; j <= p.topk_groups; ++j) {  // one more: the first that is dropped
+      const K top = lanes_max<G>(open ? mark : lowest<K>());
+      const int g = lanes_min<G>(open && mark == top ? lane : G);
+      if (j == p.topk_groups) {
+        // marks are sums of up to two keys as large as `big`, of scores up to `most`
+        const K wrong = (p.bias ? K(p.sigmoid ? 64 : 512) * most : K(0)) + K(16) * big;
+        c.near = last - top <= wrong * K(0x1p-24) && top > lowest<K>();
+        break;
+      }
+      last = top;
+      if (g < G) kept |= uint64_t(1) << g;
+      if (lane == g) open = false;
+    }
+    if (whole) {
+      if (!(kept >> mine & 1)) gone = ~0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (i < have && !(kept >> ((base + i) / size) & 1)) gone |= 1u << i;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) key[i] = gone >> i & 1 ? lowest<K>() : key[i];
+  }
+
+  for (int j = 0; j < count; ++j) {
+    K top = lowest<K>();
+#pragma unroll
+    for (int i = 0; i < R; ++i) top = key[i] > top ? key[i] : top;
+    top = lanes_max<G>(top);
+    int at = p.e;
+#pragma unroll
+    for (int i = R - 1; i >= 0; --i) at = key[i] == top && !(gone >> i & 1) ? base + i : at;
+    at = lanes_min<G>(at);
+    if (lane == j) {
+      c.id = at;
+      c.key = top;
+    }
+    const int t = at - base;
+#pragma unroll
+    for (int i = 0; i < R; ++i) key[i] = t == i ? lowest<K>() : key[i];
+    if (t >= 0 && t < R) gone |= 1u << t;
+  }
+  return c;
+}
+
+// A chosen expert's weight before scaling, on lane j < k with its logit x:
+// normalised over the row's choices, or its score.
+template <int G, class A>
+__device__ __forceinline__ A route_weight(A x, bool live, bool sigmoid, bool renorm, A top, A sum) {
+  if (!renorm) {
+    if (sigmoid) return sigmoid_of(x);
+    return top > lowest<A>() ? exp_of(x - top) / sum : A(0);
+  }
+  const A most = lanes_max<G>(live && x == x ? x : lowest<A>());
+  // scores that would underflow are in the ratio of exp(x) in any case
+  A v = sigmoid && most > A(-60) ? sigmoid_of(x) : exp_of(x - most);
+  if (most == lowest<A>() && x == x) v = A(0);
+  const A total = group_sum(live ? v : A(0), G);
+  return total == A(0) ? A(0) : v / total;
+}
+
+template <class T, int G, int R>
+__global__ void __launch_bounds__(BLOCK) route_kernel(RouteArgs<T> p) {
+  using A = acc_t<T>;
+  const int lane = threadIdx.x % G;
+  const int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G;
+  const int64_t row = r < p.n ? r : p.n - 1;  // the last rows' spare lanes go along
+  const T* x = p.logits + row * p.e;
+  int id;
+  A logit, top, sum;
+  if constexpr (sizeof(A) == 8) {
+    const Choice<double> c = route_choose<double, T, G, R>(p, x, p.k);
+    id = c.id;
+    top = c.top;
+    sum = c.sum;
+    logit = lane < p.k && id < p.e ? (A)x[id] : lowest<A>();
+  } else {
+    const bool more = p.bias && p.k < p.e;  // the first that is not chosen, too
+    const Choice<float> c = route_choose<float, T, G, R>(p, x, p.k + (more ? 1 : 0));
+    const bool kept = lane < p.k + (more ? 1 : 0) && c.id < p.e;
+    id = c.id;
+    top = c.top;
+    sum = c.sum;
+    logit = kept ? (A)x[id] : lowest<A>();
+    bool again = false;
+    if (p.bias) {
+      const A bias = kept ? p.bias[id] : A(0);
+      A s = p.sigmoid ? sigmoid_of(logit) : exp_of(logit - top) / sum;
+      const A key1 = __shfl_up(c.key, 1, G), x1 = __shfl_up(logit, 1, G);
+      const A b1 = __shfl_up(bias, 1, G), s1 = __shfl_up(s, 1, G);
+      const A wrong = A(p.sigmoid ? 16 : 128) * (s + s1) + A(2) * (abs_of(c.key) + abs_of(key1));
+      const bool near = lane > 0 && kept && c.key > lowest<A>() &&
+                        key1 - c.key <= wrong * A(0x1p-24) && !(x1 == logit && b1 == bias);
+      again = near;
+    }
+    // without a bias only sums of two logits can round
+    if (__any(again || (c.near && (p.bias || p.top2)))) {
+      id = route_choose<double, T, G, R>(p, x, p.k).id;
+      logit = lane < p.k && id < p.e ? (A)x[id] : lowest<A>();
+    }
+  }
+  const bool live = lane < p.k;
+  const A w = route_weight<G, A>(logit, live, p.sigmoid, p.renorm, top, sum);
+  if (live && r < p.n) {
+    p.ids[row * p.k + lane] = id;
+    p.weights[row * p.k + lane] = w * p.scale;
+  }
+}
+
+// dlogits of a row, formed in LDS: zeros (or, where every score counts, the
+// softmax's share) with the choices' terms added, then written as vectors.
+template <class T, int G>
+__global__ void __launch_bounds__(BLOCK) route_grad_kernel(RouteArgs<T> p) {
+  using A = acc_t<T>;
+  extern __shared__ __align__(16) char route_lds[];
+  const int lane = threadIdx.x % G;
+  const int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G;
+  const int64_t row = r < p.n ? r : p.n - 1;
+  A* buf = reinterpret_cast<A*>(route_lds) + (int64_t)(threadIdx.x / G) * p.e;
+  const T* x = p.logits + row * p.e;
+  const bool live = lane < p.k;
+  const int64_t id = live ? p.ids[row * p.k + lane] : -1;
+  const bool ok = id >= 0 && id < p.e;
+  const A logit = ok ? (A)x[id] : lowest<A>();
+  const A dw = ok ? p.dweights[row * p.k + lane] * p.scale : A(0);
+  const bool full = !p.sigmoid && !p.renorm;
+  A top = lowest<A>(), sum = A(0);
+  if (full) {
+    for (int i = lane; i < p.e; i += G) {
+      const A v = (A)x[i];
+      buf[i] = v;
+      top = v > top ? v : top;
+    }
+    top = lanes_max<G>(top);
+    for (int i = lane; i < p.e; i += G) {
+      const A v = top > lowest<A>() ? exp_of(buf[i] - top) : A(0);
+      buf[i] = v;
+      sum += v;
+    }
+    sum = group_sum(sum, G);
+  }
+  const A w = route_weight<G, A>(logit, ok, p.sigmoid, p.renorm, top, sum);
+  const A inner = group_sum(ok ? dw * w : A(0), G);
+  A dx;
+  if (full) {
+    const A part = sum == A(0) ? A(0) : A(1) / sum;
+    for (int i = lane; i < p.e; i += G) buf[i] = -(buf[i] * part) * inner;
+    dx = w * (dw - inner);
+  } else {
+    for (int i = lane; i < p.e; i += G) buf[i] = A(0);
+    dx = w * (p.renorm ? dw - inner : dw);
+    if (p.sigmoid) dx *= sigmoid_of(-logit);
+    if (logit == lowest<A>()) dx = A(0);
+  }
+  __syncthreads();
+  if (ok) buf[id] = dx;
+  __syncthreads();
+  if (r >= p.n) return;
+  for (int i = lane; i < p.e; i += G) p.dlogits[row * p.e + i] = (T)buf[i];
+}
+
+// Rows [at, at + n) of a call.
+template <class T>
+hipError_t run_route_rows(RouteArgs<T> p, int64_t at, int64_t n, hipStream_t s) {
+  using A = acc_t<T>;
+  p.logits += at * p.e;
+  p.ids += at * p.k;
+  p.n = n;
+  auto grid = [&](int g) { return (n + BLOCK / g - 1) / (BLOCK / g); };
+  if (p.dlogits) {
+    p.dlogits += at * p.e;
+    p.dweights += at * p.k;
+    const int g = p.k <= 16 && p.e <= 256 ? 16 : 64;
+    const size_t lds = (size_t)(BLOCK / g) * p.e * sizeof(A);
+    if (g == 16) route_grad_kernel<T, 16><<<grid(16), BLOCK, lds, s>>>(p);
+    else route_grad_kernel<T, 64><<<grid(64), BLOCK, lds, s>>>(p);
+    return hipGetLastError();
+  }
+  p.weights += at * p.k;
+  // lanes for the choices (and the one more), and for the groups' marks
+  const int need = p.k + 1 > p.groups ? p.k + 1 : p.groups;
+  if (need <= 16 && p.e <= 64) route_kernel<T, 16, 4><<<grid(16), BLOCK, 0, s>>>(p);
+  else if (need <= 16 && p.e <= 256) route_kernel<T, 16, 16><<<grid(16), BLOCK, 0, s>>>(p);
+  else if (need <= 32 && p.e <= 512) route_kernel<T, 32, 16><<<grid(32), BLOCK, 0, s>>>(p);
+  else if (p.e <= 1024) route_kernel<T, 64, 16><<<grid(64), BLOCK, 0, s>>>(p);
+  else route_kernel<T, 64, 32><<<grid(64), BLOCK, 0, s>>>(p);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t run_route(const RouteParams& q) {
+  using A = acc_t<T>;
+  RouteArgs<T> p{};
+  p.logits = (const T*)q.logits;
+  p.bias = (const A*)q.bias;
+  p.weights = (A*)q.weights;
+  p.ids = q.ids;
+  p.n = q.n;
+  p.e = q.e;
+  p.k = q.k;
+  p.groups = q.topk_groups == q.groups ? 1 : q.groups;
+  p.topk_groups = q.topk_groups;
+  p.sigmoid = q.sigmoid;
+  p.top2 = q.top2;
+  p.renorm = q.renorm;
+  p.scale = (A)q.scale;
+  p.dweights = (const A*)q.dweights;
+  p.dlogits = (T*)q.dlogits;
+  hipStream_t s = q.stream;
+  // a launch takes MAX_LAUNCH_BLOCKS workgroups of four rows at least
+  for (int64_t at = 0; at < q.n; at += 4 * MAX_LAUNCH_BLOCKS) {
+    const hipError_t e = run_route_rows(p, at, q.n - at < 4 * MAX_LAUNCH_BLOCKS
+                                                   ? q.n - at : 4 * MAX_LAUNCH_BLOCKS, s);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace mdgl

@@ -151,6 +151,15 @@ _SIGNATURES = {
     "mdgl_layer_norm_grad": ([_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _C, _C, _P],
                              _C),
     "mdgl_layer_norm_grad_workspace_bytes": ([_I64, _I64, _C], _I64),
+    "mdgl_topk_route": ([_P, _P, _P, _P, _I64, _I64, _I64, _C, _I64, _I64, _C, _C,
+                         ctypes.c_double, _C, _P], _C),
+    "mdgl_topk_route_grad": ([_P, _P, _P, _P, _I64, _I64, _I64, _C, _C, ctypes.c_double, _C, _P],
+                             _C),
+    "mdgl_route_plan": ([_P, _I64, _I64, _P, _P, _P, _P, _I64, _P], _C),
+    "mdgl_route_plan_workspace_bytes": ([_I64, _I64], _I64),
+    "mdgl_dispatch_rows": ([_P, _P, _P, _I64, _I64, _I64, _C, _P], _C),
+    "mdgl_combine_rows": ([_P, _P, _P, _P, _I64, _I64, _I64, _C, _P], _C),
+    "mdgl_combine_rows_grad": ([_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _C, _P], _C),
 }
 
 

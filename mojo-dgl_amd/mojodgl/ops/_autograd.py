@@ -42,7 +42,11 @@ these follow the calculus of the forward ops and run on the same kernels:
   ``mdgl_segment_reduce_arg``), softmax as edge_softmax;
 * segment_scan: the reverse recurrence (``mdgl_segment_scan_grad``);
 * layer_norm: dx and the sums of the weights' gradients in one pass
-  (``mdgl_layer_norm_grad``).
+  (``mdgl_layer_norm_grad``);
+* topk_route: the chosen experts' weights back to the logits
+  (``mdgl_topk_route_grad``); dispatch_rows: the sum of a row's copies
+  (``mdgl_combine_rows`` without weights); combine_rows:
+  ``mdgl_combine_rows_grad``.
 
 The backward passes run on the library's kernels, outside torch's graph, so
 they are differentiable once: a second derivative through them raises.
@@ -65,7 +69,8 @@ from .. import _lib
 from ..base import DGLError
 
 __all__ = ["needs_grad", "GSpMM", "GSDDMM", "EdgeSoftmax", "SegmentReduce", "SegmentSoftmax",
-           "SegmentMM", "GatherMM", "SegmentScan", "LayerNorm"]
+           "SegmentMM", "GatherMM", "SegmentScan", "LayerNorm",
+           "TopkRoute", "DispatchRows", "CombineRows"]
 
 
 def needs_grad(*xs) -> bool:
@@ -692,3 +697,65 @@ class LayerNorm(torch.autograd.Function):
         dx, dw, db = _layer_norm_grad(value, weight, bias, *ctx.stats, grad,
                                       ctx.needs_input_grad[:3])
         return _back(dx, value), _back(dw, weight), _back(db, bias), None
+
+
+class TopkRoute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, score, bias, num_groups, topk_groups, group_score, renormalize,
+                scale):
+        from .route import _topk_route
+
+        w, ids, back = _topk_route(logits, k, score, bias, num_groups, topk_groups, group_score,
+                                   renormalize, scale)
+        # a copy of the ids the caller cannot write to
+        ctx.ids, ctx.how = ids.clone(), (score, renormalize, scale)
+        ctx.save_for_backward(logits)
+        w, ids = back(w), back(ids)
+        ctx.mark_non_differentiable(ids)
+        return w, ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _):
+        from .route import _topk_route_grad
+
+        (logits,) = ctx.saved_tensors
+        return (_back(_topk_route_grad(logits, ctx.ids, grad, *ctx.how), logits),) + (None,) * 8
+
+
+class DispatchRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, value, plan):
+        from .route import _dispatch_rows
+
+        out, back = _dispatch_rows(value, plan)
+        ctx.plan = plan
+        ctx.like = torch.empty(0, dtype=value.dtype, device=value.device)
+        return back(out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        from .route import _sum_rows
+
+        return _back(_sum_rows(_gpu(grad).contiguous(), None, ctx.plan), ctx.like), None
+
+
+class CombineRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, value, weights, plan):
+        from .route import _combine_rows
+
+        out, back = _combine_rows(value, weights, plan)
+        ctx.plan = plan
+        _save_some(ctx, value, weights)
+        return back(out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        from .route import _combine_rows_grad
+
+        value, weights = _saved_some(ctx)
+        dx, dw = _combine_rows_grad(value, weights, ctx.plan, grad, ctx.needs_input_grad[:2])
+        return _back(dx, value), _back(dw, weights), None
