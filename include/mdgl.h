@@ -615,16 +615,14 @@ int mdgl_segment_marks(const int32_t* offsets, int64_t num_seg, int64_t n, int32
  * each segment's state behind its last row, its initial one for an empty segment
  * (has_empty: whether there are any). marks (state, [ceil(n / 16)][d], nullable)
  * is what mdgl_segment_scan_grad needs of the forward pass. ids, starts, ends:
- * mdgl_segment_marks; longest: the longest segment's rows. Where a segment's rows
- * are split (mdgl_segment_scan_workspace_bytes > 0), products of the gates over
- * up to 1,024 rows are formed: they must not overflow the state's type (gates in
- * [-1, 1] never do). */
+ * mdgl_segment_marks. Products of neighbouring rows' gates within a segment are
+ * formed: they must not overflow the state's type (gates in [-1, 1] never do). */
 int mdgl_segment_scan(const void* gate, const void* value, const void* initial,
                       const int32_t* offsets, const int32_t* ids, const uint64_t* starts,
                       const uint64_t* ends, void* dst, void* last, void* marks, int64_t num_seg,
-                      int64_t n, int64_t d, int64_t longest, int has_empty, void* workspace,
+                      int64_t n, int64_t d, int has_empty, void* workspace,
                       int64_t workspace_bytes, int dtype, int gate_dtype, void* stream);
-int64_t mdgl_segment_scan_workspace_bytes(int64_t n, int64_t d, int64_t longest, int dtype);
+int64_t mdgl_segment_scan_workspace_bytes(int64_t n, int64_t d, int dtype);
 
 /* Gradients of mdgl_segment_scan from those of h (grad, the values' dtype) and of
  * `last` (grad_last, state, nullable): dgate (the gates' dtype; needs value and
@@ -633,7 +631,7 @@ int mdgl_segment_scan_grad(const void* gate, const void* value, const void* init
                            const void* marks, const void* grad, const void* grad_last,
                            const int32_t* offsets, const int32_t* ids, const uint64_t* starts,
                            const uint64_t* ends, void* dgate, void* dvalue, void* dinitial,
-                           int64_t num_seg, int64_t n, int64_t d, int64_t longest, int has_empty,
+                           int64_t num_seg, int64_t n, int64_t d, int has_empty,
                            void* workspace, int64_t workspace_bytes, int dtype, int gate_dtype,
                            void* stream);
 

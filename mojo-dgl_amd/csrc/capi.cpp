@@ -1577,26 +1577,23 @@ int mdgl_segment_marks(const int32_t* offsets, int64_t num_seg, int64_t n, int32
 
 namespace {
 
-int scan_sizes(const char* what, int64_t num_seg, int64_t n, int64_t d, int64_t longest,
-               int dtype, int gate_dtype) {
+int scan_sizes(const char* what, int64_t num_seg, int64_t n, int64_t d, int dtype,
+               int gate_dtype) {
   if (!row_dtype_ok(dtype)) return fail(MDGL_EINVAL, "%s: bad dtype %d", what, dtype);
   if (gate_dtype != dtype && !(gate_dtype == MDGL_FLOAT32 && half_dtype(dtype)))
     return fail(MDGL_EINVAL, "%s: gates of dtype %d with values of %d", what, gate_dtype, dtype);
-  if (num_seg < 0 || n < 0 || d < 0 || longest < 0)
-    return fail(MDGL_EINVAL, "%s: negative size", what);
+  if (num_seg < 0 || n < 0 || d < 0) return fail(MDGL_EINVAL, "%s: negative size", what);
   if (n >= (int64_t(1) << 31) || num_seg >= (int64_t(1) << 31))
     return fail(MDGL_EINVAL, "%s: 2**31 or more rows or segments", what);
   if (!row_widths_fit(d, dtype_bytes(dtype)))
     return fail(MDGL_EINVAL, "%s: rows of 2 GiB or more", what);
-  if (longest > n) return fail(MDGL_EINVAL, "%s: a segment longer than the rows", what);
-  if (n > 0 && (num_seg == 0 || longest == 0))
-    return fail(MDGL_EINVAL, "%s: rows but no segments", what);
+  if (n > 0 && num_seg == 0) return fail(MDGL_EINVAL, "%s: rows but no segments", what);
   return MDGL_OK;
 }
 
 int scan_workspace(const char* what, void* workspace, int64_t have, int64_t n, int64_t d,
-                   int64_t longest, int dtype) {
-  const int64_t need = n > 0 ? scan_workspace_bytes(n, d, longest, dtype) : 0;
+                   int dtype) {
+  const int64_t need = scan_workspace_bytes(n, d, dtype);
   if (need > 0 && workspace && !aligned(workspace, WS_ALIGN))
     return fail(MDGL_EINVAL, "workspace must be %lld-byte aligned", (long long)WS_ALIGN);
   if (need > 0 && (!workspace || have < need))
@@ -1607,24 +1604,24 @@ int scan_workspace(const char* what, void* workspace, int64_t have, int64_t n, i
 
 }  // namespace
 
-int64_t mdgl_segment_scan_workspace_bytes(int64_t n, int64_t d, int64_t longest, int dtype) {
-  if (n < 0 || d < 0 || longest < 0 || !row_dtype_ok(dtype)) return -1;
-  return n == 0 || d == 0 ? 0 : scan_workspace_bytes(n, d, longest, dtype);
+int64_t mdgl_segment_scan_workspace_bytes(int64_t n, int64_t d, int dtype) {
+  if (n < 0 || d < 0 || !row_dtype_ok(dtype)) return -1;
+  return d == 0 ? 0 : scan_workspace_bytes(n, d, dtype);
 }
 
 int mdgl_segment_scan(const void* gate, const void* value, const void* initial,
                       const int32_t* offsets, const int32_t* ids, const uint64_t* starts,
                       const uint64_t* ends, void* dst, void* last, void* marks, int64_t num_seg,
-                      int64_t n, int64_t d, int64_t longest, int has_empty, void* workspace,
+                      int64_t n, int64_t d, int has_empty, void* workspace,
                       int64_t workspace_bytes, int dtype, int gate_dtype, void* stream) {
   MDGL_RANGE();
-  int rc = scan_sizes("segment_scan", num_seg, n, d, longest, dtype, gate_dtype);
+  int rc = scan_sizes("segment_scan", num_seg, n, d, dtype, gate_dtype);
   if (rc) return rc;
   if (d == 0 || (n == 0 && !(has_empty && last))) return MDGL_OK;
   if (n > 0 && (!gate || !value || !ids || !starts || !ends || !dst))
     return fail(MDGL_EINVAL, "segment_scan: null buffer");
   if (has_empty && last && !offsets) return fail(MDGL_EINVAL, "segment_scan: null buffer");
-  if ((rc = scan_workspace("segment_scan", workspace, workspace_bytes, n, d, longest, dtype)))
+  if ((rc = scan_workspace("segment_scan", workspace, workspace_bytes, n, d, dtype)))
     return rc;
   ScanParams q{};
   q.gate = gate;
@@ -1644,25 +1641,25 @@ int mdgl_segment_scan(const void* gate, const void* value, const void* initial,
   q.gate_f32 = gate_dtype == MDGL_FLOAT32;
   q.workspace = workspace;
   q.stream = (hipStream_t)stream;
-  return hip_status(launch_scan(q, false, longest, dtype), "segment_scan");
+  return hip_status(launch_scan(q, false, dtype), "segment_scan");
 }
 
 int mdgl_segment_scan_grad(const void* gate, const void* value, const void* initial,
                            const void* marks, const void* grad, const void* grad_last,
                            const int32_t* offsets, const int32_t* ids, const uint64_t* starts,
                            const uint64_t* ends, void* dgate, void* dvalue, void* dinitial,
-                           int64_t num_seg, int64_t n, int64_t d, int64_t longest, int has_empty,
+                           int64_t num_seg, int64_t n, int64_t d, int has_empty,
                            void* workspace, int64_t workspace_bytes, int dtype, int gate_dtype,
                            void* stream) {
   MDGL_RANGE();
-  int rc = scan_sizes("segment_scan_grad", num_seg, n, d, longest, dtype, gate_dtype);
+  int rc = scan_sizes("segment_scan_grad", num_seg, n, d, dtype, gate_dtype);
   if (rc) return rc;
   if (d == 0 || (n == 0 && !(has_empty && dinitial))) return MDGL_OK;
   if (n > 0 && (!gate || !grad || !ids || !starts || !ends || (dgate && (!value || !marks))))
     return fail(MDGL_EINVAL, "segment_scan_grad: null buffer");
   if (has_empty && dinitial && !offsets)
     return fail(MDGL_EINVAL, "segment_scan_grad: null buffer");
-  if ((rc = scan_workspace("segment_scan_grad", workspace, workspace_bytes, n, d, longest, dtype)))
+  if ((rc = scan_workspace("segment_scan_grad", workspace, workspace_bytes, n, d, dtype)))
     return rc;
   ScanParams q{};
   q.gate = gate;
@@ -1685,7 +1682,7 @@ int mdgl_segment_scan_grad(const void* gate, const void* value, const void* init
   q.gate_f32 = gate_dtype == MDGL_FLOAT32;
   q.workspace = workspace;
   q.stream = (hipStream_t)stream;
-  return hip_status(launch_scan(q, true, longest, dtype), "segment_scan_grad");
+  return hip_status(launch_scan(q, true, dtype), "segment_scan_grad");
 }
 
 int mdgl_segment_scan_step(const void* gate, const void* value, const void* state, void* dst,

@@ -56,4 +56,35 @@ __device__ __forceinline__ void store_acc(T* p, const A (&in)[N]) {
   store_any(p, out);
 }
 
+// N consecutive elements held as they came from memory: 16-bit values stay two
+// to a register until they are used.
+template <class T, int N>
+struct Held {
+  static constexpr int WORDS = (N * (int)sizeof(T) + 3) / 4;
+  static constexpr int ALIGN = sizeof(T) < 4 ? (int)sizeof(T) : 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (sizeof(T) * N < 4) {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    } else if constexpr (WORDS == 1) {
+      __builtin_memcpy(w, p, 4);
+    } else {
+      typedef uint32_t V __attribute__((ext_vector_type(WORDS), aligned(ALIGN)));
+      const V v = *reinterpret_cast<const V*>(p);
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) w[i] = v[i];
+    }
+  }
+  __device__ __forceinline__ acc_t<T> at(int k) const {
+    if constexpr (sizeof(T) == 8) {
+      return __builtin_bit_cast(double, (uint64_t)w[2 * k + 1] << 32 | w[2 * k]);
+    } else if constexpr (sizeof(T) == 4) {
+      return __builtin_bit_cast(float, w[k]);
+    } else {
+      const uint16_t h = (uint16_t)(k % 2 ? w[k / 2] >> 16 : w[k / 2]);
+      return (float)__builtin_bit_cast(T, h);
+    }
+  }
+};
+
 }  // namespace mdgl

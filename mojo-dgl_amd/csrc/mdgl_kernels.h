@@ -308,7 +308,7 @@ hipError_t launch_segment_offsets(const int64_t* len, int64_t num, int64_t chunk
                                   int32_t* offsets, int64_t* stats, void* ws, hipStream_t s);
 
 // Gated linear recurrence over segments and its gradients (scan_impl.h;
-// scan_plan.hip for the marks and the geometry).
+// scan_plan.hip for the marks).
 struct ScanParams {
   const void* gate;
   const void* value;
@@ -330,19 +330,14 @@ struct ScanParams {
   void* workspace;
   hipStream_t stream;
 };
-// How the rows are cut: walks of `len` rows (a multiple of 16), owning the
-// segments that start in them, or chunks with a carry.
-struct ScanGeometry {
-  bool owners;
-  int64_t len;
-};
-ScanGeometry scan_geometry(int64_t n, int64_t d, int64_t longest, int dtype);
-int64_t scan_workspace_bytes(int64_t n, int64_t d, int64_t longest, int dtype);
-hipError_t launch_scan(const ScanParams& q, bool back, int64_t longest, int dtype);
-hipError_t launch_scan_f32(const ScanParams& q, const ScanGeometry& geo, bool back);
-hipError_t launch_scan_f64(const ScanParams& q, const ScanGeometry& geo, bool back);
-hipError_t launch_scan_bf16(const ScanParams& q, const ScanGeometry& geo, bool back);
-hipError_t launch_scan_f16(const ScanParams& q, const ScanGeometry& geo, bool back);
+constexpr int64_t SCAN_TICKET_BYTES = 256;  // the ticket, in front of what chunks publish
+hipError_t launch_scan_reset(uint32_t* ticket, uint32_t* words, int64_t n, hipStream_t s);
+int64_t scan_workspace_bytes(int64_t n, int64_t d, int dtype);
+hipError_t launch_scan(const ScanParams& q, bool back, int dtype);
+hipError_t launch_scan_f32(const ScanParams& q, bool back);
+hipError_t launch_scan_f64(const ScanParams& q, bool back);
+hipError_t launch_scan_bf16(const ScanParams& q, bool back);
+hipError_t launch_scan_f16(const ScanParams& q, bool back);
 struct ScanStepParams {
   const void* gate;
   const void* value;

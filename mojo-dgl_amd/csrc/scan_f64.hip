@@ -1,8 +1,8 @@
 #include "scan_impl.h"
 
 namespace mdgl {
-hipError_t launch_scan_f64(const ScanParams& q, const ScanGeometry& geo, bool back) {
-  return run_scan_width<double, double>(q, geo, back);
+hipError_t launch_scan_f64(const ScanParams& q, bool back) {
+  return run_scan<double, double>(q, back);
 }
 hipError_t launch_scan_step_f64(const ScanStepParams& q) { return run_scan_step<double, double>(q); }
 }  // namespace mdgl

@@ -9,29 +9,28 @@
 //   dvalue[t] = D[t],  dgate[t] = D[t] * h[t-1],  dinitial = gate[0] * D[0]
 //
 // Both are chains of affine maps x -> A x + B, which compose: (A1, B1) then
-// (A2, B2) is (A1 A2, A2 B1 + B2). No column needs another one, so a lane holds
-// 16 bytes' worth of accumulators (4 columns, 2 of double) and walks down its
-// rows. The rows of all segments are one axis; bit r of `starts` / `ends` says
-// that row r is the first / last of its segment, so a walk resets its state
-// there and lengths never leave lanes idle. Two ways to cut that axis, by a rule
-// of scan_geometry:
+// (A2, B2) is (A1 A2, A2 B1 + B2). The rows of all segments are one axis, cut into
+// chunks of equal size whatever the lengths: bit r of `starts` / `ends` says that
+// row r is the first / last of its segment, and a walk replaces its state there
+// (nothing is multiplied by zero, so an infinity or a NaN stays in its segment).
 //
-//  * owners: a walk takes the segments that start in its `len` rows, to the
-//    end of the last one. It needs nothing from another walk: one launch, and
-//    each row is read once;
-//  * chunks, where a segment is too long for that: scan_fold_kernel reads the
-//    rows and leaves each chunk's (A, B), scan_carry_kernel composes them along
-//    the chunks, and the walk starts from its chunk's carry.
+// scan_pass_kernel reads each row once. A workgroup holds its chunk's rows in
+// registers, 16 rows of two columns a thread, composes their maps (in the thread,
+// then over the threads of a column in LDS), publishes the chunk's map, and looks
+// back along the chunks in front of it, composing maps until it meets one whose
+// final state is already there. With that state it goes over its registers again
+// and writes. A chunk that holds a segment's border knows its final state at once,
+// so short segments wait for nobody; the one other launch resets what chunks
+// publish, and a single chunk needs neither.
 //
-// The gradient walks 16 rows at a time: forward to have h again, in float
-// whatever the rows' type (a float gate's gradient would otherwise carry the
-// rounding of bfloat16 rows), from the state that the forward pass left in
-// `marks` in front of every 16th row (1/16 float a value, where the states h
-// themselves would be a whole one), then backward with both in registers.
-//
-// Across a segment's border nothing is multiplied by zero: the state is replaced,
-// so an infinity or a NaN stays in its segment.
+// The gradient's walk runs the other way. It has h again from gate and value, in
+// float whatever the rows' type (a float gate's gradient would otherwise carry the
+// rounding of bfloat16 rows), and from the state that the forward pass left in
+// `marks` in front of every 16th row: 1/16 float a value, where h itself would be
+// a whole one.
 #pragma once
+
+#include <type_traits>
 
 #include "mdgl_half.h"
 #include "mdgl_kernels.h"
@@ -51,218 +50,18 @@ struct ScanArgs {
   const int32_t* ids;
   const uint16_t* starts;
   const uint16_t* ends;
-  const A* carry;  // [chunks][d] state in front of a chunk (behind it, backward); null for owners
   T* out;
   A* last;
   A* marks;  // [ceil(n / 16)][d]: written forward (may be null), read backward
   G* dgate;
   T* dvalue;
   A* dinitial;
-  A* fold_a;
-  A* fold_b;
-  int64_t n, d, lanes, len, walks;
+  int64_t n, d, lanes, chunks;
+  uint32_t* ticket;
+  A* words;       // [chunks][3][d]: A, B, and the state behind the chunk
+  int64_t tiles;  // of `wide` lanes of columns
+  int wide;       // a power of two, 1 to 64
 };
-
-// First segment start at or behind row p (n when there is none).
-__device__ __forceinline__ int64_t next_start(const uint16_t* starts, int64_t p, int64_t n) {
-  if (p >= n) return n;
-  int64_t b = p / SCAN_BLOCK;
-  uint32_t w = starts[b] & (0xffffu << (p % SCAN_BLOCK));
-  const int64_t blocks = (n + SCAN_BLOCK - 1) / SCAN_BLOCK;
-  while (w == 0 && ++b < blocks) w = starts[b];
-  return b < blocks ? b * SCAN_BLOCK + __builtin_ctz(w) : n;
-}
-
-// The rows [r0, r1) of a lane's walk and its first column.
-template <class X, int V>
-__device__ __forceinline__ bool scan_walk(const X& p, int64_t* walk, int64_t* col, int64_t* r0,
-                                          int64_t* r1, bool owners) {
-  const int64_t t = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
-  const int64_t w = t / p.lanes;
-  if (w >= p.walks) return false;
-  const int64_t c = (t - w * p.lanes) * V;
-  *walk = w;
-  // the last lane of a row ends with it, sharing columns with the lane before
-  // (both compute and write the same values)
-  *col = c + V <= p.d ? c : p.d - V;
-  *r0 = w * p.len;
-  *r1 = *r0 + p.len < p.n ? *r0 + p.len : p.n;
-  if (owners) {
-    *r0 = next_start(p.starts, *r0, p.n);
-    *r1 = next_start(p.starts, *r1, p.n);
-  }
-  return true;
-}
-
-// The block of rows from `base` that lies in [r0, r1): reads are kept inside by
-// repeating the walk's first or last row.
-__device__ __forceinline__ int64_t scan_row(int64_t row, int64_t r0, int64_t r1) {
-  return row < r0 ? r0 : row >= r1 ? r1 - 1 : row;
-}
-
-template <class T, class G, int V>
-__global__ void __launch_bounds__(BLOCK) scan_kernel(ScanArgs<T, G> p) {
-  using A = acc_t<T>;
-  int64_t walk, col, r0, r1;
-  if (!scan_walk<ScanArgs<T, G>, V>(p, &walk, &col, &r0, &r1, !p.carry)) return;
-  A h[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) h[k] = A(0);
-  if (p.carry && r0 < r1) load_acc<A, A, V>(p.carry + walk * p.d + col, h);
-  constexpr int U = SCAN_BLOCK / 2;  // rows in flight
-  for (int64_t base = r0 / SCAN_BLOCK * SCAN_BLOCK; base < r1; base += SCAN_BLOCK) {
-    const uint32_t first = p.starts[base / SCAN_BLOCK], end = p.ends[base / SCAN_BLOCK];
-    if (p.marks && base >= r0) store_acc<A, A, V>(p.marks + base / SCAN_BLOCK * p.d + col, h);
-#pragma unroll
-    for (int part = 0; part < SCAN_BLOCK; part += U) {
-      if (base + part >= r1 || base + part + U <= r0) continue;
-      A a[U][V], v[U][V];
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int64_t at = scan_row(base + part + i, r0, r1) * p.d + col;
-        load_acc<G, A, V>(p.gate + at, a[i]);
-        load_acc<T, A, V>(p.value + at, v[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int64_t row = base + part + i;
-        if (row < r0 || row >= r1) continue;
-        if (first >> (part + i) & 1) {
-          if (p.initial) load_acc<A, A, V>(p.initial + (int64_t)p.ids[row] * p.d + col, h);
-          else
-#pragma unroll
-            for (int k = 0; k < V; ++k) h[k] = A(0);
-        }
-#pragma unroll
-        for (int k = 0; k < V; ++k) h[k] = fma_of(a[i][k], h[k], v[i][k]);
-        store_acc<T, A, V>(p.out + row * p.d + col, h);
-        if (p.last && (end >> (part + i) & 1))
-          store_acc<A, A, V>(p.last + (int64_t)p.ids[row] * p.d + col, h);
-      }
-    }
-  }
-}
-
-template <class T, class G, int V>
-__global__ void __launch_bounds__(BLOCK) scan_grad_kernel(ScanArgs<T, G> p) {
-  using A = acc_t<T>;
-  constexpr int U = SCAN_BLOCK;
-  int64_t walk, col, r0, r1;
-  if (!scan_walk<ScanArgs<T, G>, V>(p, &walk, &col, &r0, &r1, !p.carry)) return;
-  if (r0 >= r1) return;
-  A c[V];  // gate[t + 1] * D[t + 1]
-#pragma unroll
-  for (int k = 0; k < V; ++k) c[k] = A(0);
-  if (p.carry) load_acc<A, A, V>(p.carry + walk * p.d + col, c);
-  const int64_t lowest = r0 / SCAN_BLOCK * SCAN_BLOCK;
-  for (int64_t base = (r1 - 1) / SCAN_BLOCK * SCAN_BLOCK; base >= lowest; base -= SCAN_BLOCK) {
-    const uint32_t first = p.starts[base / SCAN_BLOCK], end = p.ends[base / SCAN_BLOCK];
-    A a[U][V], before[U][V], g[U][V];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int64_t at = scan_row(base + i, r0, r1) * p.d + col;
-      load_acc<G, A, V>(p.gate + at, a[i]);
-      load_acc<T, A, V>(p.grad + at, g[i]);
-      if (p.dgate) load_acc<T, A, V>(p.value + at, before[i]);
-    }
-    if (p.dgate) {  // the states in front of each row
-      A h[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) h[k] = A(0);
-      // a walk that does not hold the block's first row starts at a segment's
-      if (base >= r0) load_acc<A, A, V>(p.marks + base / SCAN_BLOCK * p.d + col, h);
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int64_t row = base + i;
-        if (row < r0 || row >= r1) continue;
-        if (first >> i & 1) {
-          if (p.initial) load_acc<A, A, V>(p.initial + (int64_t)p.ids[row] * p.d + col, h);
-          else
-#pragma unroll
-            for (int k = 0; k < V; ++k) h[k] = A(0);
-        }
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const A next = fma_of(a[i][k], h[k], before[i][k]);
-          before[i][k] = h[k];
-          h[k] = next;
-        }
-      }
-    }
-#pragma unroll
-    for (int i = U - 1; i >= 0; --i) {
-      const int64_t row = base + i;
-      if (row < r0 || row >= r1) continue;
-      if (end >> i & 1) {
-        if (p.grad_last) load_acc<A, A, V>(p.grad_last + (int64_t)p.ids[row] * p.d + col, c);
-        else
-#pragma unroll
-          for (int k = 0; k < V; ++k) c[k] = A(0);
-      }
-      A da[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        g[i][k] = g[i][k] + c[k];
-        c[k] = a[i][k] * g[i][k];
-      }
-      if (p.dvalue) store_acc<T, A, V>(p.dvalue + row * p.d + col, g[i]);
-      if (p.dgate) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) da[k] = g[i][k] * before[i][k];
-        store_acc<G, A, V>(p.dgate + row * p.d + col, da);
-      }
-      if (p.dinitial && (first >> i & 1))
-        store_acc<A, A, V>(p.dinitial + (int64_t)p.ids[row] * p.d + col, c);
-    }
-  }
-}
-
-// A chunk's map of the state in front of it to the state behind it (BACK: of the
-// gradient behind it to the one in front). A chunk that holds a segment's border
-// has a B only (its A is not read).
-template <class T, class G, int V, bool BACK>
-__global__ void __launch_bounds__(BLOCK) scan_fold_kernel(ScanArgs<T, G> p) {
-  using A = acc_t<T>;
-  constexpr int U = SCAN_BLOCK;
-  int64_t walk, col, r0, r1;
-  if (!scan_walk<ScanArgs<T, G>, V>(p, &walk, &col, &r0, &r1, false)) return;
-  A fa[V], fb[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) { fa[k] = A(1); fb[k] = A(0); }
-  const T* x = BACK ? p.grad : p.value;
-  const A* edge = BACK ? p.grad_last : p.initial;
-  const int64_t blocks = (r1 - r0 + SCAN_BLOCK - 1) / SCAN_BLOCK;
-  for (int64_t b = 0; b < blocks; ++b) {
-    const int64_t base = r0 + (BACK ? blocks - 1 - b : b) * SCAN_BLOCK;
-    const uint32_t edges = (BACK ? p.ends : p.starts)[base / SCAN_BLOCK];
-    A a[U][V], v[U][V];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int64_t at = scan_row(base + i, r0, r1) * p.d + col;
-      load_acc<G, A, V>(p.gate + at, a[i]);
-      load_acc<T, A, V>(x + at, v[i]);
-    }
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int i = BACK ? U - 1 - j : j;
-      const int64_t row = base + i;
-      if (row >= r1) continue;
-      if (edges >> i & 1) {
-        if (edge) load_acc<A, A, V>(edge + (int64_t)p.ids[row] * p.d + col, fb);
-        else
-#pragma unroll
-          for (int k = 0; k < V; ++k) fb[k] = A(0);
-      }
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        fa[k] = fa[k] * a[i][k];
-        fb[k] = BACK ? a[i][k] * (v[i][k] + fb[k]) : fma_of(a[i][k], fb[k], v[i][k]);
-      }
-    }
-  }
-  store_acc<A, A, V>(p.fold_a + walk * p.d + col, fa);
-  store_acc<A, A, V>(p.fold_b + walk * p.d + col, fb);
-}
 
 // x through the map (a, b): a state of 0 leaves b whatever a is (a product of
 // gates that overflowed stays out of a segment that starts from nothing).
@@ -271,59 +70,181 @@ __device__ __forceinline__ A scan_apply(A a, A b, A x) {
   return x == A(0) ? b : fma_of(a, x, b);
 }
 
-// carry[c] = the state in front of chunk c (BACK: the gradient behind it), from
-// the chunks' maps. A workgroup takes `wide` lanes of columns; its threads are
-// wide lanes times parts of the chunks. Each part composes its chunks' maps, the
-// parts' maps are scanned in LDS, and each part goes over its chunks again with
-// its carry, which replaces fold_a.
-constexpr int CARRY_BLOCK = 1024;
+// What chunks publish is one word a value, written and read whole and past the
+// caches that one XCD does not share with another (relaxed atomics of the agent's
+// scope). Every bit set means "not yet": a word says by itself that it is there, so
+// no flag and no fence orders it. A value with that pattern (a NaN) becomes
+// another NaN.
+template <class A> struct WordOf { using type = uint32_t; };
+template <> struct WordOf<double> { using type = unsigned long long; };
+
+template <class A>
+__device__ __forceinline__ void publish(A* p, A v) {
+  using W = typename WordOf<A>::type;
+  if (__builtin_bit_cast(W, v) == ~W(0)) v = A(__builtin_nan(""));
+  __hip_atomic_store(reinterpret_cast<W*>(p), __builtin_bit_cast(W, v), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <class A>
+__device__ __forceinline__ bool observe(const A* p, A* v) {
+  using W = typename WordOf<A>::type;
+  const W w = __hip_atomic_load(reinterpret_cast<const W*>(p), __ATOMIC_RELAXED,
+                                __HIP_MEMORY_SCOPE_AGENT);
+  *v = __builtin_bit_cast(A, w);
+  return w != ~W(0);
+}
+
+// The state in front of chunk `c` of the walk's order (BACK: from the last chunk
+// to the first). LOOK chunks are read at a time, which hides all but the first
+// one's latency. The wait ends: chunks are handed out by ticket in this order, so
+// the workgroups of all chunks in front have started, and each publishes its map
+// without waiting for anything; the first chunk holds a segment's border and
+// publishes its final state.
+constexpr int SCAN_LOOK = 2;
 
 template <class A, int V, bool BACK>
-__global__ void __launch_bounds__(CARRY_BLOCK) scan_carry_kernel(
-    A* fold_a, const A* fold_b, const uint16_t* edges, int64_t n, int64_t d, int64_t lanes,
-    int64_t chunks, int64_t len, int wide) {
-  __shared__ A sa[CARRY_BLOCK][V], sb[CARRY_BLOCK][V];
-  __shared__ uint8_t sk[CARRY_BLOCK];
-  const int parts = CARRY_BLOCK / wide, part = threadIdx.x / wide;
-  const int64_t lane = (int64_t)blockIdx.x * wide + threadIdx.x % wide;
-  const int64_t c0 = lane * V, col = c0 + V <= d ? c0 : d - V;
-  const bool live = lane < lanes;
-  const int64_t per = (chunks + parts - 1) / parts;
-  const int64_t lo = part * per < chunks ? part * per : chunks;
-  const int64_t hi = live ? (lo + per < chunks ? lo + per : chunks) : lo;
-  const int64_t blocks = (n + SCAN_BLOCK - 1) / SCAN_BLOCK, step = len / SCAN_BLOCK;
-  auto chunk = [&](int64_t i) { return BACK ? chunks - 1 - i : i; };
-  auto broken = [&](int64_t c) {
-    uint32_t any = 0;
-    for (int64_t b = c * step; b < (c + 1) * step && b < blocks; ++b) any |= edges[b];
-    return any != 0;
-  };
+__device__ __forceinline__ void look_back(const A* words, int64_t d, int64_t col, int64_t c,
+                                          int64_t chunks, A (&x)[V]) {
+  A ma[V], mb[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) { ma[k] = A(1); mb[k] = A(0); }
+  int64_t j = c - 1;
+  while (j >= 0) {
+    A a[SCAN_LOOK][V], b[SCAN_LOOK][V], s[SCAN_LOOK][V];
+    bool map[SCAN_LOOK], state[SCAN_LOOK];
+#pragma unroll
+    for (int q = 0; q < SCAN_LOOK; ++q) {
+      const int64_t at = j - q > 0 ? j - q : 0;
+      const A* w = words + (BACK ? chunks - 1 - at : at) * 3 * d + col;
+      map[q] = state[q] = true;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        map[q] &= observe(w + k, &a[q][k]);
+        map[q] &= observe(w + d + k, &b[q][k]);
+        state[q] &= observe(w + 2 * d + k, &s[q][k]);
+      }
+    }
+    bool stuck = false, found = false;
+#pragma unroll
+    for (int q = 0; q < SCAN_LOOK; ++q) {
+      const bool here = !stuck && !found && j >= 0;
+      const bool last = here && __all(state[q]);
+      const bool next = here && !last && __all(map[q]);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const A from = last ? s[q][k] : b[q][k];
+        mb[k] = last || next ? scan_apply(ma[k], mb[k], from) : mb[k];
+        ma[k] = next ? ma[k] * a[q][k] : ma[k];
+      }
+      found |= last;
+      stuck |= here && !last && !next;
+      j -= next;
+    }
+    if (found) break;
+    if (stuck) __builtin_amdgcn_s_sleep(1);
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) x[k] = mb[k];
+}
+
+// A chunk's rows, SCAN_BLOCK a thread: threads of `wide` lanes of columns form a
+// strip, the workgroup's strips lie one behind the other, and its maps are scanned
+// over the strips in LDS.
+//
+// Bound by memory; 32,768 rows of 2,048 bfloat16 values with float gates, in four
+// sequences: forward 122 us (570 MB, 4.7 TB/s), gradient 181 us (955 MB,
+// 5.3 TB/s), where a copy of 1 GiB runs at 5.1 TB/s. Two columns a lane: four took
+// 138 and 195 us, as registers then leave room for half the wavefronts. Rows that
+// are not used yet stay as they came, two 16-bit values to a register: 311 us ->
+// 260 us for the gradient. 512 threads: 256 make the chain of chunks twice as long
+// (100,000 rows of 1,024 float16 values in one sequence: 190 us against 139 us).
+constexpr int PASS_BLOCK = 512;
+
+template <class T, class G, int V, bool BACK>
+__global__ void __launch_bounds__(PASS_BLOCK) scan_pass_kernel(ScanArgs<T, G> p) {
+  using A = acc_t<T>;
+  constexpr int U = SCAN_BLOCK;
+  __shared__ A sa[PASS_BLOCK][V], sb[PASS_BLOCK][V];
+  __shared__ uint8_t sk[PASS_BLOCK];
+  __shared__ uint32_t turn;
+  const int me = threadIdx.x;
+  if (me == 0) turn = p.chunks > 1 ? atomicAdd(p.ticket, 1u) : blockIdx.x;
+  __syncthreads();
+  const int64_t order = turn / p.tiles, tile = turn % p.tiles;
+  const int64_t chunk = BACK ? p.chunks - 1 - order : order;
+  const int strips = PASS_BLOCK / p.wide, strip = me / p.wide;
+  int64_t lane = tile * p.wide + me % p.wide;
+  if (lane >= p.lanes) lane = p.lanes - 1;  // spare lanes do what the last one does
+  const int64_t c0 = lane * V, col = c0 + V <= p.d ? c0 : p.d - V;
+  const int64_t r0 = (chunk * strips + strip) * U;
+  const int64_t r1 = r0 + U < p.n ? r0 + U : p.n;
+  const bool any = r0 < r1;
+  const int64_t from = r0 * p.d + col;
+  const uint32_t first = any ? p.starts[r0 / U] : 0, end = any ? p.ends[r0 / U] : 0;
+  const T* x = BACK ? p.grad : p.value;
+  Held<G, V> a[U];
+  Held<T, V> v[U], value[BACK ? U : 1];
   A fa[V], fb[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) { fa[k] = A(1); fb[k] = A(0); }
   bool cut = false;
-  for (int64_t i = lo; i < hi; ++i) {
-    const int64_t c = chunk(i);
-    A a[V], b[V];
-    load_acc<A, A, V>(fold_a + c * d + col, a);
-    load_acc<A, A, V>(fold_b + c * d + col, b);
-    const bool k1 = broken(c);
-    cut |= k1;
+  const bool plain = __all(r0 + U <= p.n && (first | end) == 0);
+  auto read = [&](auto all) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      fa[k] = fa[k] * a[k];
-      fb[k] = k1 ? b[k] : scan_apply(a[k], b[k], fb[k]);
+    for (int i = 0; i < U; ++i) {
+      const int64_t at = from + (decltype(all)::value || r0 + i < r1 ? i : r1 - 1 - r0) * p.d;
+      a[i].load(p.gate + at);
+      v[i].load(x + at);
+      if (BACK && p.dgate) value[BACK ? i : 0].load(p.value + at);
     }
+  };
+  // the state that row i starts from where it is its segment's first
+  // (BACK: last), in `to`
+  const uint32_t edges = BACK ? end : first;
+  const A* edge = BACK ? p.grad_last : p.initial;
+  auto border = [&](int i, A (&to)[V]) {
+    if (edge) load_acc<A, A, V>(edge + (int64_t)p.ids[r0 + i] * p.d + col, to);
+    else
+#pragma unroll
+      for (int k = 0; k < V; ++k) to[k] = A(0);
+  };
+  auto fold = [&](auto all) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = BACK ? U - 1 - j : j;
+      if constexpr (!decltype(all)::value) {
+        if (r0 + i >= r1) continue;
+        if (edges >> i & 1) {
+          border(i, fb);
+          cut = true;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const A g = a[i].at(k), y = v[i].at(k);
+        fa[k] = fa[k] * g;
+        fb[k] = BACK ? g * (y + fb[k]) : fma_of(g, fb[k], y);
+      }
+    }
+  };
+  if (plain) {
+    read(std::true_type{});
+    fold(std::true_type{});
+  } else if (any) {
+    read(std::false_type{});
+    fold(std::false_type{});
   }
-  // inclusive scan of the parts' maps
-  const int me = threadIdx.x;
-  for (int off = 1; off < parts; off <<= 1) {
+
+  // inclusive scan of the strips' maps, in the order of the walk
+  const int pos = BACK ? strips - 1 - strip : strip;
+  for (int off = 1; off < strips; off <<= 1) {
 #pragma unroll
     for (int k = 0; k < V; ++k) { sa[me][k] = fa[k]; sb[me][k] = fb[k]; }
     sk[me] = cut;
     __syncthreads();
-    if (part >= off) {
-      const int o = me - off * wide;
+    if (pos >= off) {
+      const int o = BACK ? me + off * p.wide : me - off * p.wide;
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         fb[k] = cut ? fb[k] : scan_apply(fa[k], fb[k], sb[o][k]);
@@ -334,20 +255,118 @@ __global__ void __launch_bounds__(CARRY_BLOCK) scan_carry_kernel(
     __syncthreads();
   }
 #pragma unroll
-  for (int k = 0; k < V; ++k) sb[me][k] = fb[k];
+  for (int k = 0; k < V; ++k) { sa[me][k] = fa[k]; sb[me][k] = fb[k]; }
+  sk[me] = cut;
+  __shared__ A carry[WAVE][V];
+  // the last strip of the walk holds the chunk's map; its wavefront looks back
+  if (p.chunks == 1) {
+    if (me < p.wide)
+#pragma unroll
+      for (int k = 0; k < V; ++k) carry[me][k] = A(0);
+  } else if (me / WAVE == (BACK ? 0 : PASS_BLOCK / WAVE - 1)) {
+    const bool mine = pos == strips - 1;  // narrow rows: several strips a wavefront
+    A* w = p.words + chunk * 3 * p.d + col;
+    if (mine) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        if (cut) {
+          publish(w + 2 * p.d + k, fb[k]);
+        } else {
+          publish(w + k, fa[k]);
+          publish(w + p.d + k, fb[k]);
+        }
+      }
+    }
+    A s[V];
+    look_back<A, V, BACK>(p.words, p.d, col, order, p.chunks, s);
+    if (mine) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        if (!cut) publish(w + 2 * p.d + k, scan_apply(fa[k], fb[k], s[k]));
+        carry[me % p.wide][k] = s[k];
+      }
+    }
+  }
   __syncthreads();
-  A x[V];
+  if (!any) return;
+  A h[V];  // the state this strip starts from
 #pragma unroll
-  for (int k = 0; k < V; ++k) x[k] = part ? sb[me - wide][k] : A(0);
-  for (int64_t i = lo; i < hi; ++i) {
-    const int64_t c = chunk(i);
-    A a[V], b[V];
-    load_acc<A, A, V>(fold_a + c * d + col, a);
-    load_acc<A, A, V>(fold_b + c * d + col, b);
-    const bool k1 = broken(c);
-    store_acc<A, A, V>(fold_a + c * d + col, x);
+  for (int k = 0; k < V; ++k) h[k] = carry[me % p.wide][k];
+  if (pos) {
+    const int o = BACK ? me + p.wide : me - p.wide;
 #pragma unroll
-    for (int k = 0; k < V; ++k) x[k] = k1 ? b[k] : scan_apply(a[k], b[k], x[k]);
+    for (int k = 0; k < V; ++k) h[k] = sk[o] ? sb[o][k] : scan_apply(sa[o][k], sb[o][k], h[k]);
+  }
+
+  if constexpr (!BACK) {
+    if (p.marks) store_acc<A, A, V>(p.marks + r0 / U * p.d + col, h);
+    auto write = [&](auto all) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if constexpr (!decltype(all)::value) {
+          if (r0 + i >= r1) continue;
+          if (edges >> i & 1) border(i, h);
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) h[k] = fma_of(a[i].at(k), h[k], v[i].at(k));
+        store_acc<T, A, V>(p.out + from + i * p.d, h);
+        if constexpr (!decltype(all)::value)
+          if (p.last && (end >> i & 1))
+            store_acc<A, A, V>(p.last + (int64_t)p.ids[r0 + i] * p.d + col, h);
+      }
+    };
+    if (plain) write(std::true_type{});
+    else write(std::false_type{});
+  } else {
+    auto write = [&](auto all) {
+      constexpr bool ALL = decltype(all)::value;
+      A before[U][V];
+      if (p.dgate) {  // the states in front of each row
+        A f[V];
+        load_acc<A, A, V>(p.marks + r0 / U * p.d + col, f);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          if constexpr (!ALL) {
+            if (r0 + i >= r1) continue;
+            if (first >> i & 1) {
+              if (p.initial) load_acc<A, A, V>(p.initial + (int64_t)p.ids[r0 + i] * p.d + col, f);
+              else
+#pragma unroll
+                for (int k = 0; k < V; ++k) f[k] = A(0);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            before[i][k] = f[k];
+            f[k] = fma_of(a[i].at(k), f[k], value[BACK ? i : 0].at(k));
+          }
+        }
+      }
+#pragma unroll
+      for (int i = U - 1; i >= 0; --i) {
+        if constexpr (!ALL) {
+          if (r0 + i >= r1) continue;
+          if (edges >> i & 1) border(i, h);
+        }
+        A da[V], dv[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          dv[k] = v[i].at(k) + h[k];
+          h[k] = a[i].at(k) * dv[k];
+        }
+        if (p.dvalue) store_acc<T, A, V>(p.dvalue + from + i * p.d, dv);
+        if (p.dgate) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) da[k] = dv[k] * before[i][k];
+          store_acc<G, A, V>(p.dgate + from + i * p.d, da);
+        }
+        if constexpr (!ALL)
+          if (p.dinitial && (first >> i & 1))
+            store_acc<A, A, V>(p.dinitial + (int64_t)p.ids[r0 + i] * p.d + col, h);
+      }
+    };
+    if (plain) write(std::true_type{});
+    else write(std::false_type{});
   }
 }
 
@@ -391,7 +410,28 @@ __global__ void __launch_bounds__(BLOCK) scan_step_kernel(const G* gate, const T
 inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 template <class T, class G, int V>
-hipError_t run_scan(const ScanParams& q, const ScanGeometry& geo, bool back) {
+hipError_t run_scan_pass(ScanArgs<T, G> p, void* workspace, bool back, hipStream_t s) {
+  using A = acc_t<T>;
+  p.lanes = ceil_div64(p.d, V);
+  p.wide = WAVE;
+  while (p.wide > 1 && p.wide / 2 >= p.lanes) p.wide /= 2;
+  p.tiles = ceil_div64(p.lanes, p.wide);
+  p.chunks = ceil_div64(p.n, (int64_t)SCAN_BLOCK * (PASS_BLOCK / p.wide));
+  if (p.chunks > 1) {
+    p.ticket = (uint32_t*)workspace;
+    p.words = (A*)((char*)workspace + SCAN_TICKET_BYTES);
+    const int64_t words = p.chunks * 3 * p.d * (int64_t)(sizeof(A) / 4);
+    const hipError_t e = launch_scan_reset(p.ticket, (uint32_t*)p.words, words, s);
+    if (e != hipSuccess) return e;
+  }
+  const int64_t grid = p.chunks * p.tiles;
+  if (back) scan_pass_kernel<T, G, V, true><<<grid, PASS_BLOCK, 0, s>>>(p);
+  else scan_pass_kernel<T, G, V, false><<<grid, PASS_BLOCK, 0, s>>>(p);
+  return hipGetLastError();
+}
+
+template <class T, class G>
+hipError_t run_scan(const ScanParams& q, bool back) {
   using A = acc_t<T>;
   hipStream_t s = q.stream;
   ScanArgs<T, G> p{};
@@ -411,32 +451,14 @@ hipError_t run_scan(const ScanParams& q, const ScanGeometry& geo, bool back) {
   p.dinitial = (A*)q.dinitial;
   p.n = q.n;
   p.d = q.d;
-  p.lanes = ceil_div64(q.d, V);
-  p.len = geo.len;
-  p.walks = ceil_div64(q.n, geo.len);
+  hipError_t e = hipSuccess;
   if (q.n > 0) {
-    const int64_t grid = ceil_div64(p.walks * p.lanes, BLOCK);
-    if (!geo.owners) {
-      A* fa = (A*)q.workspace;
-      A* fb = fa + p.walks * p.d;
-      p.fold_a = fa;
-      p.fold_b = fb;
-      p.carry = fa;
-      int wide = 16;
-      while (wide > 1 && wide / 2 >= p.lanes) wide /= 2;
-      const int64_t cgrid = ceil_div64(p.lanes, wide);
-      if (back) {
-        scan_fold_kernel<T, G, V, true><<<grid, BLOCK, 0, s>>>(p);
-        scan_carry_kernel<A, V, true><<<cgrid, CARRY_BLOCK, 0, s>>>(
-            fa, fb, p.ends, p.n, p.d, p.lanes, p.walks, p.len, wide);
-      } else {
-        scan_fold_kernel<T, G, V, false><<<grid, BLOCK, 0, s>>>(p);
-        scan_carry_kernel<A, V, false><<<cgrid, CARRY_BLOCK, 0, s>>>(
-            fa, fb, p.starts, p.n, p.d, p.lanes, p.walks, p.len, wide);
-      }
-    }
-    if (back) scan_grad_kernel<T, G, V><<<grid, BLOCK, 0, s>>>(p);
-    else scan_kernel<T, G, V><<<grid, BLOCK, 0, s>>>(p);
+    // a lane's columns are 8 bytes of accumulators: 16 would halve the wavefronts
+    // that its registers leave room for
+    constexpr int V = acc_vec<T>() / 2;
+    e = q.d < V ? run_scan_pass<T, G, 1>(p, q.workspace, back, s)
+                : run_scan_pass<T, G, V>(p, q.workspace, back, s);
+    if (e != hipSuccess) return e;
   }
   A* edge_to = back ? p.dinitial : p.last;
   if (q.has_empty && edge_to) {
@@ -445,12 +467,6 @@ hipError_t run_scan(const ScanParams& q, const ScanGeometry& geo, bool back) {
         q.offsets, back ? p.grad_last : p.initial, edge_to, q.num_seg, q.d);
   }
   return hipGetLastError();
-}
-
-template <class T, class G>
-hipError_t run_scan_width(const ScanParams& q, const ScanGeometry& geo, bool back) {
-  if (q.d >= acc_vec<T>()) return run_scan<T, G, acc_vec<T>()>(q, geo, back);
-  return run_scan<T, G, 1>(q, geo, back);
 }
 
 template <class T, class G>

@@ -1,4 +1,4 @@
-// The segments' marks that the scan walks by, and how it cuts the rows.
+// The segments' marks that the scan walks by, and its dispatch by type.
 #include "mdgl_half.h"
 #include "mdgl_kernels.h"
 
@@ -32,7 +32,22 @@ __global__ void __launch_bounds__(BLOCK) segment_marks_kernel(const int32_t* off
   }
 }
 
+// The scan's ticket and the words its chunks publish: 0, and every bit set.
+__global__ void __launch_bounds__(BLOCK) scan_reset_kernel(uint32_t* ticket, uint32_t* words,
+                                                           int64_t n) {
+  const int64_t i = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) * 4;
+  if (i == 0) *ticket = 0;
+  if (i + 4 <= n) *reinterpret_cast<uint4*>(words + i) = make_uint4(~0u, ~0u, ~0u, ~0u);
+  else
+    for (int64_t j = i; j < n; ++j) words[j] = ~0u;
+}
+
 }  // namespace
+
+hipError_t launch_scan_reset(uint32_t* ticket, uint32_t* words, int64_t n, hipStream_t s) {
+  scan_reset_kernel<<<(n + 4 * BLOCK - 1) / (4 * BLOCK), BLOCK, 0, s>>>(ticket, words, n);
+  return hipGetLastError();
+}
 
 hipError_t launch_segment_marks(const int32_t* offsets, int64_t num_seg, int64_t n, int32_t* ids,
                                 uint64_t* starts, uint64_t* ends, hipStream_t s) {
@@ -42,28 +57,18 @@ hipError_t launch_segment_marks(const int32_t* offsets, int64_t num_seg, int64_t
   return hipGetLastError();
 }
 
-ScanGeometry scan_geometry(int64_t n, int64_t d, int64_t longest, int dtype) {
-  const int64_t vec = dtype == DT_F64 ? 2 : 4;
-  const int64_t lanes = d < vec ? d : (d + vec - 1) / vec;
-  // rows a walk: the most that leaves 2,048 wavefronts of them
-  int64_t len = 16;
-  while (len < 1024 && (n / (2 * len)) * lanes >= 2048 * WAVE) len *= 2;
-  return {longest <= 256, len};
+int64_t scan_workspace_bytes(int64_t n, int64_t d, int dtype) {
+  // chunks of 128 rows at least, three words a column; one chunk needs none
+  const int64_t chunks = (n + 127) / 128;
+  return chunks > 1 ? SCAN_TICKET_BYTES + chunks * 3 * d * (dtype == DT_F64 ? 8 : 4) : 0;
 }
 
-int64_t scan_workspace_bytes(int64_t n, int64_t d, int64_t longest, int dtype) {
-  const ScanGeometry geo = scan_geometry(n, d, longest, dtype);
-  if (geo.owners) return 0;
-  return (n + geo.len - 1) / geo.len * d * 2 * (dtype == DT_F64 ? 8 : 4);
-}
-
-hipError_t launch_scan(const ScanParams& q, bool back, int64_t longest, int dtype) {
-  const ScanGeometry geo = scan_geometry(q.n, q.d, longest, dtype);
+hipError_t launch_scan(const ScanParams& q, bool back, int dtype) {
   switch (dtype) {
-    case DT_F32: return launch_scan_f32(q, geo, back);
-    case DT_F64: return launch_scan_f64(q, geo, back);
-    case DT_BF16: return launch_scan_bf16(q, geo, back);
-    default: return launch_scan_f16(q, geo, back);
+    case DT_F32: return launch_scan_f32(q, back);
+    case DT_F64: return launch_scan_f64(q, back);
+    case DT_BF16: return launch_scan_bf16(q, back);
+    default: return launch_scan_f16(q, back);
   }
 }
 

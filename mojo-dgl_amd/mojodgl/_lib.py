@@ -141,11 +141,11 @@ _SIGNATURES = {
     "mdgl_scatter_rows": ([_P, _P, _P, _I64, _I64, _C, _P], _C),
     "mdgl_edge_softmax_grad": ([_P, _P, _P, _P, _P, _I64, _I64, _C, _P], _C),
     "mdgl_segment_marks": ([_P, _I64, _I64, _P, _P, _P, _P], _C),
-    "mdgl_segment_scan": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _C, _P,
+    "mdgl_segment_scan": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _C, _P,
                            _I64, _C, _C, _P], _C),
-    "mdgl_segment_scan_workspace_bytes": ([_I64, _I64, _I64, _C], _I64),
+    "mdgl_segment_scan_workspace_bytes": ([_I64, _I64, _C], _I64),
     "mdgl_segment_scan_grad": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64,
-                                _I64, _I64, _C, _P, _I64, _C, _C, _P], _C),
+                                _I64, _C, _P, _I64, _C, _C, _P], _C),
     "mdgl_segment_scan_step": ([_P, _P, _P, _P, _P, _I64, _C, _C, _P], _C),
     "mdgl_layer_norm": ([_P, _P, _P, _P, _P, _P, _I64, _I64, ctypes.c_double, _C, _C, _P], _C),
     "mdgl_layer_norm_grad": ([_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _C, _C, _P],

@@ -26,7 +26,7 @@ class SegmentPlan:
     """A batch's segments as the scan walks them, on the GPU: made once by
     `segment_plan` and used by every layer's scan of that batch.
 
-    num_rows, num_segments, longest : the rows, the segments, the longest one
+    num_rows, num_segments : its rows and segments
     """
 
     def __init__(self, seglen, num_rows=None):
@@ -40,7 +40,7 @@ class SegmentPlan:
         seg = _Segments(seglen, num_rows)  # raises for lengths that do not fit the rows
         dev = _lib.device()
         self.num_rows, self.num_segments = num_rows, seg.num
-        self.longest, self.has_empty = seg.longest, bool(seg.num) and seg.shortest == 0
+        self.has_empty = bool(seg.num) and seg.shortest == 0
         self.offsets = seg.device()
         self.device_index = _lib.current_device()
         words = (num_rows + 63) // 64
@@ -99,9 +99,9 @@ def segment_scan(seglen, gate, value, initial=None, return_state=False):
     ``h`` in the type of ``value``, and with ``return_state`` the states,
     (len(seglen), ...) in float32 (float64 for float64 values), which the next
     call takes as ``initial``. With torch tensors that require grad the results
-    take part in autograd. Segments of more than 256 rows are cut, and the
-    product of the gates of up to 1,024 rows is then formed: it must not
-    overflow (gates in [-1, 1] never do).
+    take part in autograd. Products of the gates of a segment's
+    neighbouring rows are formed: they must not overflow (gates in [-1, 1] never
+    do).
 
     Examples
     --------
@@ -146,12 +146,12 @@ def _scan(seglen, gate, value, initial, want_state, want_marks):
         marks = torch.empty((n + MARK_ROWS - 1) // MARK_ROWS, d, dtype=st, device=dev)
     L = _lib.lib()
     code = _lib.ROW_CODES[vt]
-    nbytes = L.mdgl_segment_scan_workspace_bytes(n, d, plan.longest, code)
+    nbytes = L.mdgl_segment_scan_workspace_bytes(n, d, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
     _lib.check(L.mdgl_segment_scan(
         g.data_ptr(), v.data_ptr(), _lib.ptr(i), plan.offsets.data_ptr(), plan.ids.data_ptr(),
         plan.starts.data_ptr(), plan.ends.data_ptr(), h.data_ptr(), _lib.ptr(last),
-        _lib.ptr(marks), plan.num_segments, n, d, plan.longest, plan.has_empty, _lib.ptr(ws),
+        _lib.ptr(marks), plan.num_segments, n, d, plan.has_empty, _lib.ptr(ws),
         nbytes, code, _lib.ROW_CODES[gt], _lib.stream()), "segment_scan")
     as_torch = _lib.wants_torch(G, V, I)
     where = _lib.out_device(V, G, I)
@@ -199,13 +199,13 @@ def _scan_grad(plan, gate, value, initial, marks, grad, grad_last, need):
         di = torch.empty((plan.num_segments,) + shape[1:], dtype=st, device=dev)
     L = _lib.lib()
     code = _lib.ROW_CODES[vt]
-    nbytes = L.mdgl_segment_scan_workspace_bytes(n, d, plan.longest, code)
+    nbytes = L.mdgl_segment_scan_workspace_bytes(n, d, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
     _lib.check(L.mdgl_segment_scan_grad(
         g.data_ptr(), v.data_ptr(), _lib.ptr(i), marks.data_ptr(), gh.data_ptr(), _lib.ptr(gl),
         plan.offsets.data_ptr(), plan.ids.data_ptr(), plan.starts.data_ptr(),
         plan.ends.data_ptr(), _lib.ptr(dg), _lib.ptr(dv), _lib.ptr(di), plan.num_segments, n, d,
-        plan.longest, plan.has_empty, _lib.ptr(ws), nbytes, code, _lib.ROW_CODES[gt],
+        plan.has_empty, _lib.ptr(ws), nbytes, code, _lib.ROW_CODES[gt],
         _lib.stream()), "segment_scan_grad")
     return dg, dv, di
 
