@@ -18,9 +18,10 @@
 // With a bias the order of two keys can hang on their last bits. The float pass
 // therefore makes one choice more than asked for, and a row two of whose
 // neighbouring keys (or whose last kept and first dropped group) lie closer than
-// the float keys can be wrong is chosen again in double, as a whole wavefront.
-// Keys of equal logits and biases need no second look: they are equal however
-// they are formed.
+// the float keys can be wrong is chosen again in double, by a whole wavefront.
+// Chosen keys of equal logits and biases need no second look: they are equal however
+// they are formed. (The last chosen and the first that is not do: a third may lie
+// as close.)
 #pragma once
 
 #include "mdgl_half.h"
@@ -85,6 +86,217 @@ struct Choice {
   bool near;   // the choice of groups hangs on the last bits
 };
 
+// The group of the lane's experts where every lane's lie in one, by its first
+// lanes; `span` lanes form a group (0: groups end inside lanes).
+__device__ __forceinline__ int route_span(int e, int groups, int per) {
+  const int size = e / groups, span = size / per;
+  return size == span * per && (span & (span - 1)) == 0 ? span : 0;
+}
+
+// Floats as integers of the same order; 0 is below all of them, NaN stands with
+// -inf.
+constexpr uint32_t KEY_LOWEST = 0x007fffffu;  // -inf
+
+__device__ __forceinline__ uint32_t ordered(float x) {  // not a NaN, not -0
+  const uint32_t b = __builtin_bit_cast(uint32_t, x);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+
+__device__ __forceinline__ float unordered(uint32_t k) {
+  return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+// Maximum over G lanes, in all of them; the moves inside 16 lanes are part of the
+// maximum's own instruction.
+template <int G>
+__device__ __forceinline__ uint32_t lanes_umax(uint32_t v) {
+  auto up = [](uint32_t a, int b) { return a > (uint32_t)b ? a : (uint32_t)b; };
+  v = up(v, __builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));   // quad [1,0,3,2]
+  v = up(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));   // quad [2,3,0,1]
+  v = up(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));  // row_half_mirror
+  v = up(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));  // row_mirror
+  if constexpr (G > 16) v = up(v, __shfl_xor((int)v, 16));
+  if constexpr (G > 32) v = up(v, __shfl_xor((int)v, 32));
+  return v;
+}
+
+// The first `count` choices of a row (count <= G) by float keys. An expert that
+// is not there, or no longer, has key 0. The keys' exponentials and reciprocals are
+// the hardware's: they are good to what the caller's bounds on keys allow, and a
+// closer call is chosen again in double.
+template <class T, int G, int R>
+__device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& p, const T* x,
+                                                            int count) {
+  constexpr float LOG2E = 1.44269504088896340736f;
+  const int lane = threadIdx.x % G;
+  const int per = (p.e + G - 1) / G, base = lane * per;
+  const int have = base >= p.e ? 0 : (p.e - base < per ? p.e - base : per);
+  float v[R];
+#pragma unroll
+  for (int i = 0; i < R; i += 4) {
+    if (i + 4 <= have) {
+      T raw[4];
+      load_any<false>(x + base + i, raw);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[i + q] = (float)raw[q];
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[i + q] = i + q < have ? (float)x[base + i + q] : -__builtin_huge_valf();
+    }
+  }
+  Choice<float> c;
+  c.top = lowest<float>();
+  c.sum = 0.0f;
+  c.near = false;
+  c.id = 0;
+  c.key = lowest<float>();
+  if (!p.sigmoid && (p.bias || !p.renorm)) {
+    // the row's softmax statistics; a NaN goes into the sum
+#pragma unroll
+    for (int i = 0; i < R; ++i) c.top = v[i] > c.top ? v[i] : c.top;
+    c.top = lanes_max<G>(c.top);
+    if (c.top > lowest<float>()) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) c.sum += expf(v[i] - c.top);  // 0 where none is
+      c.sum = group_sum(c.sum, G);
+    }
+  }
+  uint32_t key[R];
+  float most = 1.0f;  // no score is larger
+  if (p.bias) {
+    const float part = c.sum > 0.0f ? 1.0f / c.sum : 0.0f;
+    if (!p.sigmoid) most = part;
+#pragma unroll
+    for (int i = 0; i < R; i += 4) {
+      float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (i + 4 <= have) {
+        load_any<false>(p.bias + base + i, b);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (i + q < have) b[q] = p.bias[base + i + q];
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float y = v[i + q];
+        const float s = p.sigmoid
+                            ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * y))
+                            : __builtin_amdgcn_exp2f(LOG2E * (y - c.top)) * part;
+        const uint32_t k = ordered(s + b[q]);  // no -0: s is not negative
+        key[i + q] = i + q >= have ? 0u : y > lowest<float>() ? k : KEY_LOWEST;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const uint32_t k = v[i] == v[i] ? ordered(v[i] + 0.0f) : KEY_LOWEST;
+      key[i] = i < have ? k : 0u;
+    }
+  }
+
+  if (p.groups > 1) {
+    const int size = p.e / p.groups, span = route_span(p.e, p.groups, per);
+    auto grade = [&](uint32_t a, uint32_t b) {
+      const float f = unordered(a);
+      return p.top2 && b > KEY_LOWEST ? f + unordered(b) : f;
+    };
+    auto two = [](uint32_t& a, uint32_t& b, uint32_t k) {  // a >= b the larger two
+      const uint32_t lo = k < a ? k : a;
+      a = k > a ? k : a;
+      b = lo > b ? lo : b;
+    };
+    auto join = [](uint32_t& a, uint32_t& b, int off) {
+      const uint32_t oa = __shfl_xor(a, off), ob = __shfl_xor(b, off);
+      join_two(a, b, oa, ob);
+    };
+    // lane j: the mark of group j, and how large the keys summed in it are
+    float mark = lowest<float>(), size_of = 0.0f;
+    auto large = [&](uint32_t a, uint32_t b) {
+      const float f = a > KEY_LOWEST ? abs_of(unordered(a)) : 0.0f;
+      return p.top2 && b > KEY_LOWEST ? f + abs_of(unordered(b)) : f;
+    };
+    if (span) {
+      uint32_t a = KEY_LOWEST, b = KEY_LOWEST;
+#pragma unroll
+      for (int i = 0; i < R; ++i) two(a, b, key[i]);
+      for (int off = 1; off < span; off <<= 1) join(a, b, off);
+      const int from = lane * span < G ? lane * span : 0;
+      mark = __shfl(grade(a, b), from, G);
+      size_of = __shfl(large(a, b), from, G);
+    } else {
+      for (int g = 0; g < p.groups; ++g) {
+        uint32_t a = KEY_LOWEST, b = KEY_LOWEST;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const int e = base + i - g * size;
+          two(a, b, e >= 0 && e < size ? key[i] : 0u);
+        }
+#pragma unroll
+        for (int off = 1; off < G; off <<= 1) join(a, b, off);
+        if (lane == g) {
+          mark = grade(a, b);
+          size_of = large(a, b);
+        }
+      }
+    }
+    // a group stays when fewer than topk_groups are ranked before it
+    const bool real = lane < p.groups;
+    int before = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const float m = __shfl(mark, g, G);
+      before += m > mark || (m == mark && g < lane);
+    }
+    const bool stays = real && before < p.topk_groups;
+    const float kept_low = -lanes_max<G>(stays ? -mark : lowest<float>());
+    const float lost_top = lanes_max<G>(real && !stays ? mark : lowest<float>());
+    // marks are sums of up to two keys, of scores up to `most`
+    const float big = lanes_max<G>(real ? size_of : 0.0f);
+    const float wrong = (p.bias ? (p.sigmoid ? 64.0f : 512.0f) * most : 0.0f) + 8.0f * big;
+    c.near = kept_low - lost_top <= wrong * 0x1p-24f && lost_top > lowest<float>();
+    const uint64_t all = __ballot(stays) >> (threadIdx.x % WAVE / G * G);
+    if (span) {
+      const int mine = lane / span;
+      const bool out = mine >= p.groups || !(all >> mine & 1);
+#pragma unroll
+      for (int i = 0; i < R; ++i) key[i] = out ? 0u : key[i];
+    } else {
+      int g = base / size, at = base % size;
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (i < have && !(all >> g & 1)) key[i] = 0u;
+        if (++at == size) {
+          at = 0;
+          ++g;
+        }
+      }
+    }
+  }
+
+  for (int j = 0; j < count; ++j) {
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < R; ++i) top = key[i] > top ? key[i] : top;
+    top = lanes_umax<G>(top);
+    int at = p.e;
+    bool hit[R];
+#pragma unroll
+    for (int i = R - 1; i >= 0; --i) {
+      hit[i] = key[i] == top;
+      at = hit[i] ? base + i : at;
+    }
+    const int first = top ? (int)~lanes_umax<G>(~(uint32_t)at) : p.e;
+    if (lane == j) {
+      c.id = first;
+      c.key = top ? unordered(top) : lowest<float>();
+    }
+    // of equal keys only the first is taken
+    const int t = at == first ? first - base : -1;
+#pragma unroll
+    for (int i = 0; i < R; ++i) key[i] = t == i ? 0u : key[i];
+  }
+  return c;
+}
+
 // The first `count` choices of a row (count <= G), keys formed in K.
 template <class K, class T, int G, int R>
 __device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T* x, int count) {
@@ -143,14 +355,9 @@ __device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T
   if (p.groups > 1) {
     const int size = p.e / p.groups;
     K mark = lowest<K>();  // lane j: the mark of group j
-    K big = K(0);
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-      big = key[i] > lowest<K>() && abs_of(key[i]) > big ? abs_of(key[i]) : big;
-    big = lanes_max<G>(big);
     auto grade = [&](K a, K b) { return p.top2 && b > lowest<K>() ? a + b : a; };
-    const int span = size / per;  // lanes a group, when its border is a lane's
-    const bool whole = size == span * per && (span & (span - 1)) == 0;
+    const int span = route_span(p.e, p.groups, per);
+    const bool whole = span != 0;
     int mine = lane / (whole ? span : 1);  // the group of all of the lane's experts
     if (whole) {
       K a = lowest<K>(), b = lowest<K>();
@@ -181,17 +388,9 @@ __device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T
     }
     uint64_t kept = 0;
     bool open = lane < p.groups;
-    K last = K(0);
-    for (int j = 0; j <= p.topk_groups; ++j) {  // one more: the first that is dropped
+    for (int j = 0; j < p.topk_groups; ++j) {
       const K top = lanes_max<G>(open ? mark : lowest<K>());
       const int g = lanes_min<G>(open && mark == top ? lane : G);
-      if (j == p.topk_groups) {
-        // marks are sums of up to two keys as large as `big`, of scores up to `most`
-        const K wrong = (p.bias ? K(p.sigmoid ? 64 : 512) * most : K(0)) + K(16) * big;
-        c.near = last - top <= wrong * K(0x1p-24) && top > lowest<K>();
-        break;
-      }
-      last = top;
       if (g < G) kept |= uint64_t(1) << g;
       if (lane == g) open = false;
     }
@@ -250,6 +449,7 @@ __global__ void __launch_bounds__(BLOCK) route_kernel(RouteArgs<T> p) {
   const int64_t r = (int64_t)blockIdx.x * (BLOCK / G) + threadIdx.x / G;
   const int64_t row = r < p.n ? r : p.n - 1;  // the last rows' spare lanes go along
   const T* x = p.logits + row * p.e;
+  const bool live = lane < p.k;
   int id;
   A logit, top, sum;
   if constexpr (sizeof(A) == 8) {
@@ -260,7 +460,7 @@ __global__ void __launch_bounds__(BLOCK) route_kernel(RouteArgs<T> p) {
     logit = lane < p.k && id < p.e ? (A)x[id] : lowest<A>();
   } else {
     const bool more = p.bias && p.k < p.e;  // the first that is not chosen, too
-    const Choice<float> c = route_choose<float, T, G, R>(p, x, p.k + (more ? 1 : 0));
+    const Choice<float> c = route_choose_float<T, G, R>(p, x, p.k + (more ? 1 : 0));
     const bool kept = lane < p.k + (more ? 1 : 0) && c.id < p.e;
     id = c.id;
     top = c.top;
@@ -269,21 +469,28 @@ __global__ void __launch_bounds__(BLOCK) route_kernel(RouteArgs<T> p) {
     bool again = false;
     if (p.bias) {
       const A bias = kept ? p.bias[id] : A(0);
-      A s = p.sigmoid ? sigmoid_of(logit) : exp_of(logit - top) / sum;
+      const A s = abs_of(c.key - bias);  // the score, near enough
       const A key1 = __shfl_up(c.key, 1, G), x1 = __shfl_up(logit, 1, G);
       const A b1 = __shfl_up(bias, 1, G), s1 = __shfl_up(s, 1, G);
       const A wrong = A(p.sigmoid ? 16 : 128) * (s + s1) + A(2) * (abs_of(c.key) + abs_of(key1));
       const bool near = lane > 0 && kept && c.key > lowest<A>() &&
-                        key1 - c.key <= wrong * A(0x1p-24) && !(x1 == logit && b1 == bias);
+                        key1 - c.key <= wrong * A(0x1p-24) &&
+                        !(lane < p.k && x1 == logit && b1 == bias);
       again = near;
     }
     // without a bias only sums of two logits can round
-    if (__any(again || (c.near && (p.bias || p.top2)))) {
-      id = route_choose<double, T, G, R>(p, x, p.k).id;
-      logit = lane < p.k && id < p.e ? (A)x[id] : lowest<A>();
+    again = again || (c.near && (p.bias || p.top2));
+    for (uint64_t flags = __ballot(again); flags;) {
+      const int g = __builtin_ctzll(flags) / G;  // the wavefront's g-th row
+      const int64_t other = __shfl(row, g * G);
+      const int sure = route_choose<double, T, WAVE, R * G / WAVE < 4 ? 4 : R * G / WAVE>(
+                           p, p.logits + other * p.e, p.k).id;
+      const int mine = __shfl(sure, lane);
+      if ((int)(threadIdx.x % WAVE) / G == g) id = mine;
+      flags &= ~(~uint64_t(0) >> (WAVE - G) << (g * G));
     }
+    if (live) logit = id < p.e ? (A)x[id] : lowest<A>();
   }
-  const bool live = lane < p.k;
   const A w = route_weight<G, A>(logit, live, p.sigmoid, p.renorm, top, sum);
   if (live && r < p.n) {
     p.ids[row * p.k + lane] = id;
