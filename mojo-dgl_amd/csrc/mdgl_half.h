@@ -63,6 +63,17 @@ struct Held {
   static constexpr int WORDS = (N * (int)sizeof(T) + 3) / 4;
   static constexpr int ALIGN = sizeof(T) < 4 ? (int)sizeof(T) : 4;
   uint32_t w[WORDS];
+  // past the caches: for what is read once
+  __device__ __forceinline__ void load_stream(const T* p) {
+    if constexpr (WORDS > 1) {
+      typedef uint32_t V __attribute__((ext_vector_type(WORDS), aligned(ALIGN)));
+      const V v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) w[i] = v[i];
+    } else {
+      load(p);
+    }
+  }
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (sizeof(T) * N < 4) {
       w[0] = *reinterpret_cast<const uint16_t*>(p);

@@ -458,48 +458,36 @@ ROW_CODES = {torch.float32: FLOAT32, torch.float64: FLOAT64, torch.bfloat16: BFL
              torch.float16: FLOAT16}
 
 
-class Rows:
-    """A validated operand of a row operator: a float32, float64, bfloat16 or
-    float16 tensor (or numpy array, without bfloat16); `dtype` is torch's."""
-
-    __slots__ = ("data", "is_torch", "device", "shape", "dtype")
-
-    def __init__(self, data, is_torch, dev, dtype):
-        self.data = data
-        self.is_torch = is_torch
-        self.device = dev
-        self.shape = tuple(data.shape)
-        self.dtype = dtype
-
-    @property
-    def ndim(self):
-        return len(self.shape)
-
-
-def rows(a) -> Rows:
-    """Validate an operand of a row operator: `feature`, but float16 and
-    bfloat16 stay as they are."""
+def rows(a) -> torch.Tensor:
+    """An operand of a row operator as a tensor, where it is: `feature`, but
+    float16 and bfloat16 stay as they are."""
     if isinstance(a, torch.Tensor):
-        if a.dtype in ROW_CODES:
-            return Rows(a, True, a.device, a.dtype)
-    else:
-        a = np.asanyarray(a)
-        if a.dtype == np.float16:
-            return Rows(np.ascontiguousarray(a), False, None, torch.float16)
-    f = feature(a)
-    return Rows(f.data, f.is_torch, f.device, torch_dtype(f.dtype))
+        return a if a.dtype in ROW_CODES else feature(a).data
+    a = np.asanyarray(a)
+    a = np.ascontiguousarray(a) if a.dtype == np.float16 else feature(a).data
+    return torch.from_numpy(a)
 
 
-def rows_on_device(r: Rows, dtype: torch.dtype) -> torch.Tensor:
+def rows_on_device(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """The operand as a contiguous tensor of `dtype` on the current GPU."""
-    dev = device()
-    t = r.data
-    if not r.is_torch:
-        t = torch.from_numpy(t)
-    elif t.dtype == dtype and t.is_cuda and t.get_device() == current_device() \
+    if t.dtype is dtype and t.is_cuda and t.get_device() == current_device() \
             and t.is_contiguous():
         return t
-    return t.detach().to(device=dev, dtype=dtype).contiguous()
+    return t.detach().to(device=device(), dtype=dtype).contiguous()
+
+
+def caller_device(*operands):
+    """Where results go: the device of the first tensor among the operands as they
+    were given, None (numpy) without any."""
+    for x in operands:
+        if isinstance(x, torch.Tensor):
+            return x.device
+    return None
+
+
+def hand_back(t: torch.Tensor, where):
+    """A result on the current GPU as the caller's container (`caller_device`)."""
+    return t.cpu().numpy() if where is None else t if t.device == where else t.to(where)
 
 
 def state_dtype(dtype: torch.dtype) -> torch.dtype:

@@ -659,11 +659,12 @@ class SegmentScan(torch.autograd.Function):
         from .scan import _scan
 
         # the states in front of every 16th row serve the gates' gradient
-        h, last, marks, plan, back = _scan(seglen, gate, value, initial, return_state, True)
+        h, last, marks, plan = _scan(seglen, gate, value, initial, return_state, True)
         ctx.plan, ctx.marks = plan, marks
         ctx.set_materialize_grads(False)
         _save_some(ctx, gate, value, initial)
-        return back(h), back(last) if return_state else None
+        where = _lib.caller_device(value, gate, initial)
+        return _lib.hand_back(h, where), _lib.hand_back(last, where) if return_state else None
 
     @staticmethod
     @once_differentiable
@@ -683,10 +684,10 @@ class LayerNorm(torch.autograd.Function):
     def forward(ctx, value, weight, bias, eps):
         from .norm import _layer_norm
 
-        y, mean, rstd, back = _layer_norm(value, weight, bias, eps, True)
+        y, mean, rstd = _layer_norm(value, weight, bias, eps, True)
         ctx.stats = mean, rstd
         _save_some(ctx, value, weight, bias)
-        return back(y)
+        return _lib.hand_back(y, _lib.caller_device(value, weight, bias))
 
     @staticmethod
     @once_differentiable
@@ -705,12 +706,12 @@ class TopkRoute(torch.autograd.Function):
                 scale):
         from .route import _topk_route
 
-        w, ids, back = _topk_route(logits, k, score, bias, num_groups, topk_groups, group_score,
-                                   renormalize, scale)
+        w, ids = _topk_route(logits, k, score, bias, num_groups, topk_groups, group_score,
+                             renormalize, scale)
         # a copy of the ids the caller cannot write to
         ctx.ids, ctx.how = ids.clone(), (score, renormalize, scale)
         ctx.save_for_backward(logits)
-        w, ids = back(w), back(ids)
+        w, ids = (_lib.hand_back(t, logits.device) for t in (w, ids))
         ctx.mark_non_differentiable(ids)
         return w, ids
 
@@ -728,10 +729,9 @@ class DispatchRows(torch.autograd.Function):
     def forward(ctx, value, plan):
         from .route import _dispatch_rows
 
-        out, back = _dispatch_rows(value, plan)
         ctx.plan = plan
         ctx.like = torch.empty(0, dtype=value.dtype, device=value.device)
-        return back(out)
+        return _lib.hand_back(_dispatch_rows(value, plan), value.device)
 
     @staticmethod
     @once_differentiable
@@ -746,10 +746,10 @@ class CombineRows(torch.autograd.Function):
     def forward(ctx, value, weights, plan):
         from .route import _combine_rows
 
-        out, back = _combine_rows(value, weights, plan)
         ctx.plan = plan
         _save_some(ctx, value, weights)
-        return back(out)
+        return _lib.hand_back(_combine_rows(value, weights, plan),
+                              _lib.caller_device(value, weights))
 
     @staticmethod
     @once_differentiable

@@ -36,59 +36,61 @@ def layer_norm(value, weight=None, bias=None, eps=1e-5):
     """
     if _autograd.needs_grad(value, weight, bias):
         return _autograd.LayerNorm.apply(value, weight, bias, eps)
-    y, _, _, back = _layer_norm(value, weight, bias, eps, False)
-    return back(y)
+    y = _layer_norm(value, weight, bias, eps, False)[0]
+    return _lib.hand_back(y, _lib.caller_device(value, weight, bias))
 
 
 def _operands(value, weight, bias):
-    """Validated operands and the GPU types (rows, weights) of a call."""
-    V = _lib.rows(value)
-    W, B = (None if x is None else _lib.rows(x) for x in (weight, bias))
-    if V.ndim < 1:
+    """The operands and the types (rows, weights) of a call, checked."""
+    x = _lib.rows(value)
+    w = None if weight is None else _lib.rows(weight)
+    b = None if bias is None else _lib.rows(bias)
+    if x.ndim < 1:
         raise DGLError("layer_norm wants rows, got a value without axes")
-    d = V.shape[-1]
-    for name, x in (("weight", W), ("bias", B)):
-        if x is not None and x.shape != (d,):
-            raise DGLError("{} must have shape {}, got {}".format(name, (d,), x.shape))
-    given = {x.dtype for x in (W, B) if x is not None}
-    vt = torch.float64 if torch.float64 in given else V.dtype
-    wt = vt if given <= {vt} or vt == torch.float64 else torch.float32
-    return V, W, B, vt, wt
+    d = x.shape[-1]
+    vt = wt = x.dtype
+    for name, t in (("weight", w), ("bias", b)):
+        if t is None:
+            continue
+        if t.ndim != 1 or t.shape[0] != d:
+            raise DGLError("{} must have shape {}, got {}".format(name, (d,), tuple(t.shape)))
+        if t.dtype is torch.float64:
+            vt = wt = torch.float64
+        elif t.dtype is not vt and wt is not torch.float64:
+            wt = torch.float32
+    return x, w, b, vt, wt, d
 
 
 def _layer_norm(value, weight, bias, eps, want_stats):
-    """(y, mean, rstd, back): GPU tensors and the function that gives a result
-    back in the caller's container."""
-    V, W, B, vt, wt = _operands(value, weight, bias)
+    """(y, mean, rstd) on the GPU."""
+    x, w, b, vt, wt, d = _operands(value, weight, bias)
     eps = float(eps)
     if not eps >= 0.0:
         raise DGLError("eps must be >= 0, got {}".format(eps))
-    d = V.shape[-1]
-    dev = _lib.device()
-    x = _lib.rows_on_device(V, vt)
+    _lib.device()
+    x = _lib.rows_on_device(x, vt)
+    w = None if w is None else _lib.rows_on_device(w, wt)
+    b = None if b is None else _lib.rows_on_device(b, wt)
     n = x.numel() // d if d else 0
-    w, b = (None if t is None else _lib.rows_on_device(t, wt) for t in (W, B))
-    y = torch.empty(V.shape, dtype=vt, device=dev)
+    y = torch.empty_like(x)
     mean = rstd = None
     if want_stats:
-        mean, rstd = torch.empty(2, n, dtype=_lib.state_dtype(vt), device=dev).unbind(0)
+        mean, rstd = torch.empty(2, n, dtype=_lib.state_dtype(vt), device=x.device).unbind(0)
     _lib.check(_lib.lib().mdgl_layer_norm(
         x.data_ptr(), _lib.ptr(w), _lib.ptr(b), y.data_ptr(), _lib.ptr(mean), _lib.ptr(rstd), n, d,
         eps, _lib.ROW_CODES[vt], _lib.ROW_CODES[wt], _lib.stream()), "layer_norm")
-    as_torch, where = _lib.wants_torch(V, W, B), _lib.out_device(V, W, B)
-    return y, mean, rstd, lambda t: _lib.give_back(t, as_torch, where)
+    return y, mean, rstd
 
 
 def _layer_norm_grad(value, weight, bias, mean, rstd, grad, need):
     """(dvalue, dweight, dbias) on the GPU, those that `need` wants."""
-    V, W, B, vt, wt = _operands(value, weight, bias)
-    d = V.shape[-1]
-    dev = _lib.device()
-    x = _lib.rows_on_device(V, vt)
+    x, w, _, vt, wt, d = _operands(value, weight, bias)
+    x = _lib.rows_on_device(x, vt)
+    w = None if w is None else _lib.rows_on_device(w, wt)
+    g = _lib.rows_on_device(grad, vt)
+    dev = x.device
     n = x.numel() // d if d else 0
-    w = None if W is None else _lib.rows_on_device(W, wt)
-    g = grad.to(device=dev, dtype=vt).contiguous()
-    dx = torch.empty(V.shape, dtype=vt, device=dev) if need[0] else None
+    dx = torch.empty_like(x) if need[0] else None
     # no rows: the kernels write nothing
     make = torch.empty if n else torch.zeros
     dw = make(d, dtype=wt, device=dev) if need[1] else None

@@ -55,32 +55,34 @@ def topk_route(logits, k, score="softmax", bias=None, num_groups=1, topk_groups=
     if _autograd.needs_grad(logits):
         return _autograd.TopkRoute.apply(logits, k, score, bias, num_groups, topk_groups,
                                          group_score, renormalize, scale)
-    w, ids, back = _topk_route(logits, k, score, bias, num_groups, topk_groups, group_score,
-                               renormalize, scale)
-    return back(w), back(ids)
+    w, ids = _topk_route(logits, k, score, bias, num_groups, topk_groups, group_score,
+                         renormalize, scale)
+    where = _lib.caller_device(logits)
+    return _lib.hand_back(w, where), _lib.hand_back(ids, where)
 
 
 def _topk_route(logits, k, score, bias, num_groups, topk_groups, group_score, renormalize, scale):
-    """(weights, ids, back): GPU tensors and the function that gives a result back
-    in the caller's container."""
-    X = _lib.rows(logits)
-    if X.ndim != 2:
-        raise DGLError("topk_route wants logits of shape (N, E), got {}".format(X.shape))
-    for name, value, table in (("score", score, _SCORES),
-                               ("group_score", group_score, _GROUP_SCORES)):
-        if value not in table:
-            raise DGLError("{} must be one of {}, got {!r}".format(name, sorted(table), value))
-    n, e = X.shape
-    st = _lib.state_dtype(X.dtype)
-    B = None if bias is None else _lib.rows(bias)
-    if B is not None and B.shape != (e,):
-        raise DGLError("bias must have shape {}, got {}".format((e,), B.shape))
+    """(weights, ids) on the GPU."""
+    x = _lib.rows(logits)
+    if x.ndim != 2:
+        raise DGLError("topk_route wants logits of shape (N, E), got {}".format(tuple(x.shape)))
+    if score not in _SCORES:
+        raise DGLError("score must be one of {}, got {!r}".format(sorted(_SCORES), score))
+    if group_score not in _GROUP_SCORES:
+        raise DGLError("group_score must be one of {}, got {!r}".format(sorted(_GROUP_SCORES),
+                                                                        group_score))
+    n, e = x.shape
+    xt = x.dtype
+    st = _lib.state_dtype(xt)
+    b = None if bias is None else _lib.rows(bias)
+    if b is not None and tuple(b.shape) != (e,):
+        raise DGLError("bias must have shape {}, got {}".format((e,), tuple(b.shape)))
     scale = float(scale)
     if not math.isfinite(scale):
         raise DGLError("scale must be finite, got {}".format(scale))
     dev = _lib.device()
-    x = _lib.rows_on_device(X, X.dtype)
-    b = None if B is None else _lib.rows_on_device(B, st)
+    x = _lib.rows_on_device(x, xt)
+    b = None if b is None else _lib.rows_on_device(b, st)
     k, num_groups = int(k), int(num_groups)
     topk_groups = num_groups if topk_groups is None else int(topk_groups)
     w = torch.empty(n, max(k, 0), dtype=st, device=dev)
@@ -88,20 +90,20 @@ def _topk_route(logits, k, score, bias, num_groups, topk_groups, group_score, re
     _lib.check(_lib.lib().mdgl_topk_route(
         x.data_ptr(), _lib.ptr(b), w.data_ptr(), ids.data_ptr(), n, e, k, _SCORES[score],
         num_groups, topk_groups, _GROUP_SCORES[group_score], bool(renormalize), scale,
-        _lib.ROW_CODES[X.dtype], _lib.stream()), "topk_route")
-    return w, ids, lambda t: _lib.give_back(t, X.is_torch, X.device)
+        _lib.ROW_CODES[xt], _lib.stream()), "topk_route")
+    return w, ids
 
 
 def _topk_route_grad(logits, ids, grad, score, renormalize, scale):
-    X = _lib.rows(logits)
-    n, e = X.shape
-    dev = _lib.device()
-    x = _lib.rows_on_device(X, X.dtype)
-    g = grad.to(device=dev, dtype=_lib.state_dtype(X.dtype)).contiguous()
-    dx = torch.empty(n, e, dtype=X.dtype, device=dev)
+    x = _lib.rows(logits)
+    n, e = x.shape
+    xt = x.dtype
+    x = _lib.rows_on_device(x, xt)
+    g = _lib.rows_on_device(grad, _lib.state_dtype(xt))
+    dx = torch.empty_like(x)
     _lib.check(_lib.lib().mdgl_topk_route_grad(
         x.data_ptr(), ids.data_ptr(), g.data_ptr(), dx.data_ptr(), n, e, ids.shape[1],
-        _SCORES[score], bool(renormalize), float(scale), _lib.ROW_CODES[X.dtype], _lib.stream()),
+        _SCORES[score], bool(renormalize), float(scale), _lib.ROW_CODES[xt], _lib.stream()),
         "topk_route_grad")
     return dx
 
@@ -160,11 +162,9 @@ def route_plan(ids, num_experts) -> RoutePlan:
     return RoutePlan(ids, num_experts)
 
 
-def _check_plan(plan, what, rows, want):
+def _check_plan(plan, what):
     if not isinstance(plan, RoutePlan):
         raise DGLError("{} wants a plan made by route_plan".format(what))
-    if rows != want:
-        raise DGLError("{}: the plan is of {} rows, got {}".format(what, want, rows))
     if plan.device_index != _lib.current_device():
         raise DGLError("the plan lies on GPU {}, the current one is {}".format(
             plan.device_index, _lib.current_device()))
@@ -186,28 +186,29 @@ def dispatch_rows(value, plan):
     """
     if _autograd.needs_grad(value):
         return _autograd.DispatchRows.apply(value, plan)
-    out, back = _dispatch_rows(value, plan)
-    return back(out)
+    return _lib.hand_back(_dispatch_rows(value, plan), _lib.caller_device(value))
 
 
 def _dispatch_rows(value, plan):
-    X = _lib.rows(value)
-    if X.ndim < 1:
+    x = _lib.rows(value)
+    if x.ndim < 1:
         raise DGLError("dispatch_rows wants rows, got a value without axes")
-    _check_plan(plan, "dispatch_rows", X.shape[0], plan.num_rows if isinstance(
-        plan, RoutePlan) else None)
-    x = _lib.rows_on_device(X, X.dtype)
-    n, k, d = plan.num_rows, plan.k, int(math.prod(X.shape[1:]))
-    out = torch.empty((n * k,) + X.shape[1:], dtype=X.dtype, device=x.device)
+    _lib.device()
+    _check_plan(plan, "dispatch_rows")
+    n, k, shape = plan.num_rows, plan.k, x.shape
+    if shape[0] != n:
+        raise DGLError("dispatch_rows: the plan is of {} rows, got {}".format(n, shape[0]))
+    x = _lib.rows_on_device(x, x.dtype)
+    out = torch.empty((n * k,) + tuple(shape[1:]), dtype=x.dtype, device=x.device)
     _lib.check(_lib.lib().mdgl_dispatch_rows(
-        x.data_ptr(), plan.slot.data_ptr(), out.data_ptr(), n, k, d, _lib.ROW_CODES[X.dtype],
-        _lib.stream()), "dispatch_rows")
-    return out, lambda t: _lib.give_back(t, X.is_torch, X.device)
+        x.data_ptr(), plan.slot.data_ptr(), out.data_ptr(), n, k, math.prod(shape[1:]),
+        _lib.ROW_CODES[x.dtype], _lib.stream()), "dispatch_rows")
+    return out
 
 
 def _sum_rows(x, weights, plan):
     """(N, ...) sums of the plan's entries of the contiguous GPU rows `x`."""
-    n, k, d = plan.num_rows, plan.k, int(math.prod(x.shape[1:]))
+    n, k, d = plan.num_rows, plan.k, math.prod(x.shape[1:])
     out = torch.empty((n,) + tuple(x.shape[1:]), dtype=x.dtype, device=x.device)
     _lib.check(_lib.lib().mdgl_combine_rows(
         x.data_ptr(), plan.slot.data_ptr(), _lib.ptr(weights), out.data_ptr(), n, k, d,
@@ -232,38 +233,39 @@ def combine_rows(value, weights, plan):
     """
     if _autograd.needs_grad(value, weights):
         return _autograd.CombineRows.apply(value, weights, plan)
-    out, back = _combine_rows(value, weights, plan)
-    return back(out)
+    return _lib.hand_back(_combine_rows(value, weights, plan),
+                          _lib.caller_device(value, weights))
 
 
 def _combine_operands(value, weights, plan):
-    X, W = _lib.rows(value), _lib.rows(weights)
-    if X.ndim < 1:
+    x, w = _lib.rows(value), _lib.rows(weights)
+    if x.ndim < 1:
         raise DGLError("combine_rows wants rows, got a value without axes")
-    _check_plan(plan, "combine_rows", X.shape[0], plan.num_rows * plan.k if isinstance(
-        plan, RoutePlan) else None)
-    if W.shape != (plan.num_rows, plan.k) and not (plan.k == 1 and W.shape == (plan.num_rows,)):
-        raise DGLError("weights must have shape {}, got {}".format((plan.num_rows, plan.k),
-                                                                   W.shape))
-    return X, W, _lib.rows_on_device(X, X.dtype), \
-        _lib.rows_on_device(W, _lib.state_dtype(X.dtype))
+    _lib.device()
+    _check_plan(plan, "combine_rows")
+    n, k = plan.num_rows, plan.k
+    if x.shape[0] != n * k:
+        raise DGLError("combine_rows: the plan is of {} entries, got {} rows".format(
+            n * k, x.shape[0]))
+    if tuple(w.shape) != (n, k) and not (k == 1 and tuple(w.shape) == (n,)):
+        raise DGLError("weights must have shape {}, got {}".format((n, k), tuple(w.shape)))
+    return _lib.rows_on_device(x, x.dtype), _lib.rows_on_device(w, _lib.state_dtype(x.dtype))
 
 
 def _combine_rows(value, weights, plan):
-    X, W, x, w = _combine_operands(value, weights, plan)
-    as_torch, where = _lib.wants_torch(X, W), _lib.out_device(X, W)
-    return _sum_rows(x, w, plan), lambda t: _lib.give_back(t, as_torch, where)
+    x, w = _combine_operands(value, weights, plan)
+    return _sum_rows(x, w, plan)
 
 
 def _combine_rows_grad(value, weights, plan, grad, need):
     """(dvalue, dweights) on the GPU, those that `need` wants."""
-    X, W, x, w = _combine_operands(value, weights, plan)
-    n, k, d = plan.num_rows, plan.k, int(math.prod(X.shape[1:]))
-    g = grad.to(device=x.device, dtype=X.dtype).contiguous()
+    x, w = _combine_operands(value, weights, plan)
+    n, k, d = plan.num_rows, plan.k, math.prod(x.shape[1:])
+    g = _lib.rows_on_device(grad, x.dtype)
     dx = torch.empty_like(x) if need[0] else None
     # without columns the kernel writes nothing
     dw = (torch.empty_like if d else torch.zeros_like)(w) if need[1] else None
     _lib.check(_lib.lib().mdgl_combine_rows_grad(
         x.data_ptr(), plan.slot.data_ptr(), w.data_ptr(), g.data_ptr(), _lib.ptr(dx), _lib.ptr(dw),
-        n, k, d, _lib.ROW_CODES[X.dtype], _lib.stream()), "combine_rows_grad")
+        n, k, d, _lib.ROW_CODES[x.dtype], _lib.stream()), "combine_rows_grad")
     return dx, dw

@@ -116,32 +116,33 @@ def segment_scan(seglen, gate, value, initial=None, return_state=False):
     if _autograd.needs_grad(gate, value, initial):
         h, last = _autograd.SegmentScan.apply(seglen, gate, value, initial, bool(return_state))
         return (h, last) if return_state else h
-    h, last, _, _, back = _scan(seglen, gate, value, initial, return_state, False)
-    return (back(h), back(last)) if return_state else back(h)
+    h, last, _, _ = _scan(seglen, gate, value, initial, return_state, False)
+    where = _lib.caller_device(value, gate, initial)
+    h = _lib.hand_back(h, where)
+    return (h, _lib.hand_back(last, where)) if return_state else h
 
 
 def _scan(seglen, gate, value, initial, want_state, want_marks):
-    """(h, last, marks, plan, back): GPU tensors and the function that gives a
-    result back in the caller's container."""
-    G, V = _lib.rows(gate), _lib.rows(value)
-    I = None if initial is None else _lib.rows(initial)  # noqa: E741
-    if V.ndim < 1 or G.shape != V.shape:
+    """(h, last, marks, plan), the first three on the GPU."""
+    g, v = _lib.rows(gate), _lib.rows(value)
+    i = None if initial is None else _lib.rows(initial)
+    shape = v.shape
+    if v.ndim < 1 or g.shape != shape:
         raise DGLError("segment_scan wants a gate for every value, got shapes {} and {}".format(
-            G.shape, V.shape))
-    n, d = V.shape[0], int(math.prod(V.shape[1:]))
+            tuple(g.shape), tuple(shape)))
+    n, d = shape[0], math.prod(shape[1:])
     plan = _plan_for(seglen, n)
-    if I is not None and I.shape != (plan.num_segments,) + V.shape[1:]:
-        raise DGLError("initial states of shape {} wanted, got {}".format(
-            (plan.num_segments,) + V.shape[1:], I.shape))
-    vt, gt = _types(V.dtype, G.dtype)
+    states = (plan.num_segments,) + tuple(shape[1:])
+    if i is not None and tuple(i.shape) != states:
+        raise DGLError("initial states of shape {} wanted, got {}".format(states, tuple(i.shape)))
+    vt, gt = _types(v.dtype, g.dtype)
     st = _lib.state_dtype(vt)
     dev = _lib.device()
-    g, v = _lib.rows_on_device(G, gt), _lib.rows_on_device(V, vt)
-    i = None if I is None else _lib.rows_on_device(I, st)
-    h = torch.empty(V.shape, dtype=vt, device=dev)
-    last = marks = None
-    if want_state:
-        last = torch.empty((plan.num_segments,) + V.shape[1:], dtype=st, device=dev)
+    g, v = _lib.rows_on_device(g, gt), _lib.rows_on_device(v, vt)
+    i = None if i is None else _lib.rows_on_device(i, st)
+    h = torch.empty_like(v)
+    last = torch.empty(states, dtype=st, device=dev) if want_state else None
+    marks = None
     if want_marks:
         marks = torch.empty((n + MARK_ROWS - 1) // MARK_ROWS, d, dtype=st, device=dev)
     L = _lib.lib()
@@ -151,15 +152,9 @@ def _scan(seglen, gate, value, initial, want_state, want_marks):
     _lib.check(L.mdgl_segment_scan(
         g.data_ptr(), v.data_ptr(), _lib.ptr(i), plan.offsets.data_ptr(), plan.ids.data_ptr(),
         plan.starts.data_ptr(), plan.ends.data_ptr(), h.data_ptr(), _lib.ptr(last),
-        _lib.ptr(marks), plan.num_segments, n, d, plan.has_empty, _lib.ptr(ws),
-        nbytes, code, _lib.ROW_CODES[gt], _lib.stream()), "segment_scan")
-    as_torch = _lib.wants_torch(G, V, I)
-    where = _lib.out_device(V, G, I)
-
-    def back(t):
-        return _lib.give_back(t, as_torch, where)
-
-    return h, last, marks, plan, back
+        _lib.ptr(marks), plan.num_segments, n, d, plan.has_empty, _lib.ptr(ws), nbytes, code,
+        _lib.ROW_CODES[gt], _lib.stream()), "segment_scan")
+    return h, last, marks, plan
 
 
 def _plan_for(seglen, n) -> SegmentPlan:
@@ -176,22 +171,17 @@ def _plan_for(seglen, n) -> SegmentPlan:
 def _scan_grad(plan, gate, value, initial, marks, grad, grad_last, need):
     """Gradients (GPU tensors or None) of gate, value and initial; `need` says
     which are wanted."""
-    G, V = _lib.rows(gate), _lib.rows(value)
-    vt, gt = _types(V.dtype, G.dtype)
+    g, v = _lib.rows(gate), _lib.rows(value)
+    vt, gt = _types(v.dtype, g.dtype)
     st = _lib.state_dtype(vt)
     dev = _lib.device()
-    shape = V.shape
-    n, d = shape[0], int(math.prod(shape[1:]))
-    g, v = _lib.rows_on_device(G, gt), _lib.rows_on_device(V, vt)
+    shape = tuple(v.shape)
+    n, d = shape[0], math.prod(shape[1:])
+    g, v = _lib.rows_on_device(g, gt), _lib.rows_on_device(v, vt)
     i = None if initial is None else _lib.rows_on_device(_lib.rows(initial), st)
-
-    def incoming(t, dtype):
-        return None if t is None else t.to(device=dev, dtype=dtype).contiguous()
-
-    gh = incoming(grad, vt)
-    if gh is None:
-        gh = torch.zeros(shape, dtype=vt, device=dev)
-    gl = incoming(grad_last, st)
+    gh = torch.zeros(shape, dtype=vt, device=dev) if grad is None else \
+        _lib.rows_on_device(grad, vt)
+    gl = None if grad_last is None else _lib.rows_on_device(grad_last, st)
     dg = torch.empty(shape, dtype=gt, device=dev) if need[0] else None
     dv = torch.empty(shape, dtype=vt, device=dev) if need[1] else None
     di = None
@@ -228,35 +218,35 @@ def segment_scan_step(gate, value, state, out=None):
     """
     if _autograd.needs_grad(gate, value, state):
         raise DGLError("segment_scan_step has no gradient; segment_scan has")
-    G, V, S = _lib.rows(gate), _lib.rows(value), _lib.rows(state)
-    if G.shape != V.shape or S.shape != V.shape:
+    g, v, s = _lib.rows(gate), _lib.rows(value), _lib.rows(state)
+    if g.shape != v.shape or s.shape != v.shape:
         raise DGLError("segment_scan_step wants a gate, a value and a state of one shape, got "
-                       "{}, {} and {}".format(G.shape, V.shape, S.shape))
-    vt, gt = _types(V.dtype, G.dtype)
+                       "{}, {} and {}".format(*(tuple(t.shape) for t in (g, v, s))))
+    vt, gt = _types(v.dtype, g.dtype)
     st = _lib.state_dtype(vt)
+    _lib.device()
+    where = _lib.caller_device(value, gate, state, out)
     if out is not None:
         if not isinstance(out, torch.Tensor) or not out.is_cuda or out.dtype != st \
-                or tuple(out.shape) != S.shape or not out.is_contiguous() \
+                or out.shape != s.shape or not out.is_contiguous() \
                 or out.get_device() != _lib.current_device():
             raise DGLError("out must be a contiguous {} tensor of shape {} on the current "
-                           "GPU".format(st, S.shape))
+                           "GPU".format(st, tuple(s.shape)))
         if out.requires_grad and torch.is_grad_enabled():
             raise DGLError("out must not require grad")
-    dev = _lib.device()
-    g, v, s = _lib.rows_on_device(G, gt), _lib.rows_on_device(V, vt), _lib.rows_on_device(S, st)
-    h = torch.empty(V.shape, dtype=vt, device=dev)
-    new = torch.empty(S.shape, dtype=st, device=dev) if out is None else out
-    if out is not None and v.numel():
+    g, v, s = _lib.rows_on_device(g, gt), _lib.rows_on_device(v, vt), _lib.rows_on_device(s, st)
+    h = torch.empty_like(v)
+    if out is None:
+        new = torch.empty_like(s)
+    else:
+        new = out
         for t in (g, v, s):
             if _overlap(new, t) and not (t is s and t.data_ptr() == new.data_ptr()):
                 raise DGLError("out overlaps an operand it is not")
     _lib.check(_lib.lib().mdgl_segment_scan_step(
         g.data_ptr(), v.data_ptr(), s.data_ptr(), h.data_ptr(), new.data_ptr(), v.numel(),
         _lib.ROW_CODES[vt], _lib.ROW_CODES[gt], _lib.stream()), "segment_scan_step")
-    as_torch = _lib.wants_torch(G, V, S) or out is not None
-    where = _lib.out_device(V, G, S)
-    return (_lib.give_back(h, as_torch, where),
-            new if out is not None else _lib.give_back(new, as_torch, where))
+    return _lib.hand_back(h, where), new if out is not None else _lib.hand_back(new, where)
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
