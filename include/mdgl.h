@@ -667,8 +667,10 @@ int64_t mdgl_layer_norm_grad_workspace_bytes(int64_t n, int64_t d, int dtype);
  * (num_experts / num_groups neighbours each; num_groups at most 64), by the largest
  * key of a group or the sum of its two largest. weights = scale * score, divided by
  * the sum of the row's k scores with `renormalize`. A logit of -inf masks its
- * expert: it is chosen only when nothing else is left, with a weight of 0. A row
- * with a NaN or +inf has NaN among its weights, and ids in range. */
+ * expert: it is chosen only when nothing else is left, with a weight of 0. A NaN
+ * ranks with the masked and makes the weights it enters NaN: its own, and all of a
+ * row whose softmax is formed (without `renormalize`, or with a bias). So does a
+ * +inf with softmax. ids stay in range. The bias must be finite. */
 #define MDGL_SCORE_SOFTMAX 0
 #define MDGL_SCORE_SIGMOID 1
 #define MDGL_GROUP_MAX 0

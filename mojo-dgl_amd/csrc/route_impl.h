@@ -155,11 +155,10 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
 #pragma unroll
     for (int i = 0; i < R; ++i) c.top = v[i] > c.top ? v[i] : c.top;
     c.top = lanes_max<G>(c.top);
-    if (c.top > lowest<float>()) {
 #pragma unroll
-      for (int i = 0; i < R; ++i) c.sum += expf(v[i] - c.top);  // 0 where none is
-      c.sum = group_sum(c.sum, G);
-    }
+    for (int i = 0; i < R; ++i)  // 0 where no expert is, and in a row of masks
+      c.sum += v[i] == lowest<float>() ? 0.0f : expf(v[i] - c.top);
+    c.sum = group_sum(c.sum, G);
   }
   uint32_t key[R];
   float most = 1.0f;  // no score is larger
@@ -196,9 +195,10 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
 
   if (p.groups > 1) {
     const int size = p.e / p.groups, span = route_span(p.e, p.groups, per);
+    // (a sum that overflows stays above a masked group's, and its row is near)
     auto grade = [&](uint32_t a, uint32_t b) {
       const float f = unordered(a);
-      return p.top2 && b > KEY_LOWEST ? f + unordered(b) : f;
+      return p.top2 && b > KEY_LOWEST ? fmaxf(f + unordered(b), -__FLT_MAX__) : f;
     };
     auto two = [](uint32_t& a, uint32_t& b, uint32_t k) {  // a >= b the larger two
       const uint32_t lo = k < a ? k : a;
@@ -331,12 +331,10 @@ __device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T
 #pragma unroll
     for (int i = 0; i < R; ++i) c.top = key[i] > c.top ? key[i] : c.top;
     c.top = lanes_max<G>(c.top);
-    if (c.top > lowest<K>()) {
 #pragma unroll
-      for (int i = 0; i < R; ++i)
-        if (!(gone >> i & 1)) c.sum += exp_of(key[i] - c.top);
-      c.sum = group_sum(c.sum, G);
-    }
+    for (int i = 0; i < R; ++i)
+      c.sum += gone >> i & 1 || key[i] == lowest<K>() ? K(0) : exp_of(key[i] - c.top);
+    c.sum = group_sum(c.sum, G);
   }
   K most = K(1);  // no score is larger
   if (p.bias) {
@@ -432,12 +430,13 @@ template <int G, class A>
 __device__ __forceinline__ A route_weight(A x, bool live, bool sigmoid, bool renorm, A top, A sum) {
   if (!renorm) {
     if (sigmoid) return sigmoid_of(x);
-    return top > lowest<A>() ? exp_of(x - top) / sum : A(0);
+    return top > lowest<A>() ? exp_of(x - top) / sum : sum;  // masks, NaN: 0 or NaN
   }
   const A most = lanes_max<G>(live && x == x ? x : lowest<A>());
   // scores that would underflow are in the ratio of exp(x) in any case
   A v = sigmoid && most > A(-60) ? sigmoid_of(x) : exp_of(x - most);
   if (most == lowest<A>() && x == x) v = A(0);
+  if (!sigmoid && sum != sum) v = sum;  // the row's softmax is NaN
   const A total = group_sum(live ? v : A(0), G);
   return total == A(0) ? A(0) : v / total;
 }
@@ -524,7 +523,7 @@ __global__ void __launch_bounds__(BLOCK) route_grad_kernel(RouteArgs<T> p) {
     }
     top = lanes_max<G>(top);
     for (int i = lane; i < p.e; i += G) {
-      const A v = top > lowest<A>() ? exp_of(buf[i] - top) : A(0);
+      const A v = buf[i] == lowest<A>() ? A(0) : exp_of(buf[i] - top);
       buf[i] = v;
       sum += v;
     }

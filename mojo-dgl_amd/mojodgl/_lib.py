@@ -464,8 +464,8 @@ def rows(a) -> torch.Tensor:
     if isinstance(a, torch.Tensor):
         return a if a.dtype in ROW_CODES else feature(a).data
     a = np.asanyarray(a)
-    a = np.ascontiguousarray(a) if a.dtype == np.float16 else feature(a).data
-    return torch.from_numpy(a)
+    data = np.ascontiguousarray(a) if a.dtype == np.float16 else feature(a).data
+    return torch.from_numpy(data.reshape(a.shape))  # both make a scalar 1-D
 
 
 def rows_on_device(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

@@ -708,10 +708,9 @@ class TopkRoute(torch.autograd.Function):
 
         w, ids = _topk_route(logits, k, score, bias, num_groups, topk_groups, group_score,
                              renormalize, scale)
-        # a copy of the ids the caller cannot write to
-        ctx.ids, ctx.how = ids.clone(), (score, renormalize, scale)
-        ctx.save_for_backward(logits)
-        w, ids = (_lib.hand_back(t, logits.device) for t in (w, ids))
+        ctx.how = score, renormalize, scale
+        w, ids = _lib.hand_back(w, logits.device), _lib.hand_back(ids, logits.device)
+        ctx.save_for_backward(logits, ids)
         ctx.mark_non_differentiable(ids)
         return w, ids
 
@@ -720,8 +719,8 @@ class TopkRoute(torch.autograd.Function):
     def backward(ctx, grad, _):
         from .route import _topk_route_grad
 
-        (logits,) = ctx.saved_tensors
-        return (_back(_topk_route_grad(logits, ctx.ids, grad, *ctx.how), logits),) + (None,) * 8
+        logits, ids = ctx.saved_tensors
+        return (_back(_topk_route_grad(logits, ids, grad, *ctx.how), logits),) + (None,) * 8
 
 
 class DispatchRows(torch.autograd.Function):

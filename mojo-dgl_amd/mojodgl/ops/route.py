@@ -35,8 +35,8 @@ def topk_route(logits, k, score="softmax", bias=None, num_groups=1, topk_groups=
     logits : (N, E) array or tensor, E at most 2048; -inf masks an expert
     k : experts a row, at most 32
     score : 'softmax' over the row's experts, or 'sigmoid' of each
-    bias : (E,) added to the scores for the choice only (to balance the experts'
-        load); without it the logits' order decides
+    bias : (E,) finite, added to the scores for the choice only (to balance the
+        experts' load); without it the logits' order decides
     num_groups : the experts fall into this many groups of neighbours (at most 64)
     topk_groups : only experts of this many best groups are chosen (None: all)
     group_score : a group's rank: its 'max' score, or its best two's sum ('top2'),
@@ -49,7 +49,7 @@ def topk_route(logits, k, score="softmax", bias=None, num_groups=1, topk_groups=
     ``(weights, ids)``, both (N, k), best first, the lowest index among equals;
     ids are int64. Scores that differ by less than float32 shows are compared in
     float64. An expert masked by -inf is chosen only when nothing else is left and
-    weighs 0. With torch logits that require grad the weights take part in
+    weighs 0; a NaN ranks with the masked and makes the weights it enters NaN. With torch logits that require grad the weights take part in
     autograd; `bias` gets no gradient.
     """
     if _autograd.needs_grad(logits):
@@ -100,6 +100,7 @@ def _topk_route_grad(logits, ids, grad, score, renormalize, scale):
     xt = x.dtype
     x = _lib.rows_on_device(x, xt)
     g = _lib.rows_on_device(grad, _lib.state_dtype(xt))
+    ids = _lib.i64_device(ids) if ids.is_cuda else ids.to(x.device)
     dx = torch.empty_like(x)
     _lib.check(_lib.lib().mdgl_topk_route_grad(
         x.data_ptr(), ids.data_ptr(), g.data_ptr(), dx.data_ptr(), n, e, ids.shape[1],
