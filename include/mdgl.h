@@ -640,7 +640,7 @@ int mdgl_segment_scan_grad(const void* gate, const void* value, const void* init
 int mdgl_segment_scan_step(const void* gate, const void* value, const void* state, void* dst,
                            void* next, int64_t count, int dtype, int gate_dtype, void* stream);
 
-/* Layer norm over the d columns of each of n rows:
+/* Layer norm over the d columns (fewer than 2**26) of each of n rows:
  *   dst = (value - mean) * rstd * weight + bias,
  *   rstd = 1 / sqrt(mean((value - mean)^2) + eps)
  * weight / bias: d values in the rows' dtype, or MDGL_FLOAT32 with rows of 16

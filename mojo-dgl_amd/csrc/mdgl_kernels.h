@@ -331,6 +331,9 @@ struct ScanParams {
   hipStream_t stream;
 };
 constexpr int64_t SCAN_TICKET_BYTES = 256;  // the ticket, in front of what chunks publish
+constexpr int SCAN_GROUP = 4;  // chunks a group
+// Words a column that `chunks` chunks publish: their maps, the groups' maps and states.
+inline int64_t scan_words(int64_t chunks) { return chunks * 2 + chunks / SCAN_GROUP * 3; }
 hipError_t launch_scan_reset(uint32_t* ticket, uint32_t* words, int64_t n, hipStream_t s);
 int64_t scan_workspace_bytes(int64_t n, int64_t d, int dtype);
 hipError_t launch_scan(const ScanParams& q, bool back, int dtype);

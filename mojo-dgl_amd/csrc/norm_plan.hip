@@ -18,7 +18,9 @@ NormGeometry norm_geometry(int64_t n, int64_t d, int size) {
   // workgroups of the gradient, each of which leaves a row of sums
   int64_t parts;
   if (shape == COUNT) {
-    parts = n < 64 ? n : 64;
+    // d times parts work-items in a launch
+    const int64_t most = d < (int64_t(1) << 25) ? 64 : 32;
+    parts = n < most ? n : most;
   } else {
     const int g = shapes[shape].threads, block = g > 256 ? g : 256;
     const int64_t want = (n + block / g - 1) / (block / g), most = 256 * (1024 / block);

@@ -17,11 +17,9 @@
 // scan_pass_kernel reads each row once. A workgroup holds its chunk's rows in
 // registers, 16 rows of two columns a thread, composes their maps (in the thread,
 // then over the threads of a column in LDS), publishes the chunk's map, and looks
-// back along the chunks in front of it, composing maps until it meets one whose
-// final state is already there. With that state it goes over its registers again
-// and writes. A chunk that holds a segment's border knows its final state at once,
-// so short segments wait for nobody; the one other launch resets what chunks
-// publish, and a single chunk needs neither.
+// back along the chunks in front of it for the state it starts from. With that state
+// it goes over its registers again and writes. The one other launch resets what
+// chunks publish; a single chunk needs neither.
 //
 // The gradient's walk runs the other way. It has h again from gate and value, in
 // float whatever the rows' type (a float gate's gradient would otherwise carry the
@@ -58,7 +56,7 @@ struct ScanArgs {
   A* dinitial;
   int64_t n, d, lanes, chunks;
   uint32_t* ticket;
-  A* words;       // [chunks][3][d]: A, B, and the state behind the chunk
+  A* words;       // [chunks][2][d]: A, B; then those of groups, and groups' states
   int64_t tiles;  // of `wide` lanes of columns
   int wide;       // a power of two, 1 to 64
 };
@@ -81,8 +79,23 @@ template <> struct WordOf<double> { using type = unsigned long long; };
 template <class A>
 __device__ __forceinline__ void publish(A* p, A v) {
   using W = typename WordOf<A>::type;
-  if (__builtin_bit_cast(W, v) == ~W(0)) v = A(__builtin_nan(""));
+  if (__builtin_bit_cast(W, v) >= W(~W(0) - 1)) v = A(__builtin_nan(""));
   __hip_atomic_store(reinterpret_cast<W*>(p), __builtin_bit_cast(W, v), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The A of a chunk that holds a segment's border: its B replaces the state. (No other
+// A has this pattern: publish() rids values of it too.)
+template <class A>
+__device__ __forceinline__ bool scan_is_cut(A a) {
+  using W = typename WordOf<A>::type;
+  return __builtin_bit_cast(W, a) == W(~W(0) - 1);
+}
+
+template <class A>
+__device__ __forceinline__ void publish_cut(A* p) {
+  using W = typename WordOf<A>::type;
+  __hip_atomic_store(reinterpret_cast<W*>(p), W(~W(0) - 1), __ATOMIC_RELAXED,
                      __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -95,57 +108,129 @@ __device__ __forceinline__ bool observe(const A* p, A* v) {
   return w != ~W(0);
 }
 
-// The state in front of chunk `c` of the walk's order (BACK: from the last chunk
-// to the first). LOOK chunks are read at a time, which hides all but the first
-// one's latency. The wait ends: chunks are handed out by ticket in this order, so
-// the workgroups of all chunks in front have started, and each publishes its map
-// without waiting for anything; the first chunk holds a segment's border and
-// publishes its final state.
-constexpr int SCAN_LOOK = 2;
+// The published maps [i, end) at `words` (two words a column an item) in order,
+// SCAN_LOOK read at a time, which hides all but the first one's latency; waits for
+// each. TAKE is given them one by one.
+constexpr int SCAN_LOOK = 4;
 
-template <class A, int V, bool BACK>
-__device__ __forceinline__ void look_back(const A* words, int64_t d, int64_t col, int64_t c,
-                                          int64_t chunks, A (&x)[V]) {
-  A ma[V], mb[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) { ma[k] = A(1); mb[k] = A(0); }
-  int64_t j = c - 1;
-  while (j >= 0) {
-    A a[SCAN_LOOK][V], b[SCAN_LOOK][V], s[SCAN_LOOK][V];
-    bool map[SCAN_LOOK], state[SCAN_LOOK];
+template <class A, int V, class Take>
+__device__ __forceinline__ void scan_maps(const A* words, int64_t d, int64_t col, int64_t i,
+                                          int64_t end, Take take) {
+  while (i < end) {
+    A a[SCAN_LOOK][V], b[SCAN_LOOK][V];
+    bool there[SCAN_LOOK];
 #pragma unroll
     for (int q = 0; q < SCAN_LOOK; ++q) {
-      const int64_t at = j - q > 0 ? j - q : 0;
-      const A* w = words + (BACK ? chunks - 1 - at : at) * 3 * d + col;
-      map[q] = state[q] = true;
+      const A* w = words + (i + q < end ? i + q : end - 1) * 2 * d + col;
+      there[q] = true;
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        map[q] &= observe(w + k, &a[q][k]);
-        map[q] &= observe(w + d + k, &b[q][k]);
-        state[q] &= observe(w + 2 * d + k, &s[q][k]);
+        there[q] &= observe(w + k, &a[q][k]);
+        there[q] &= observe(w + d + k, &b[q][k]);
       }
     }
-    bool stuck = false, found = false;
+    int taken = 0;
 #pragma unroll
     for (int q = 0; q < SCAN_LOOK; ++q) {
-      const bool here = !stuck && !found && j >= 0;
-      const bool last = here && __all(state[q]);
-      const bool next = here && !last && __all(map[q]);
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const A from = last ? s[q][k] : b[q][k];
-        mb[k] = last || next ? scan_apply(ma[k], mb[k], from) : mb[k];
-        ma[k] = next ? ma[k] * a[q][k] : ma[k];
-      }
-      found |= last;
-      stuck |= here && !last && !next;
-      j -= next;
+      const bool step = taken == q && i + q < end && __all(there[q]);
+      take(a[q], b[q], step);
+      taken += step;
     }
-    if (found) break;
-    if (stuck) __builtin_amdgcn_s_sleep(1);
+    i += taken;
+    if (!taken) __builtin_amdgcn_s_sleep(1);
   }
+}
+
+template <class A, int V>
+__device__ __forceinline__ void scan_walk_maps(const A* words, int64_t d, int64_t col, int64_t i,
+                                               int64_t end, A (&x)[V]) {
+  scan_maps<A, V>(words, d, col, i, end, [&](A (&a)[V], A (&b)[V], bool step) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) x[k] = mb[k];
+    for (int k = 0; k < V; ++k) {
+      const A to = scan_is_cut(a[k]) ? b[k] : scan_apply(a[k], b[k], x[k]);
+      x[k] = step ? to : x[k];
+    }
+  });
+}
+
+// The state in front of chunk `c` in the order of the walk, into x; (fa, fb, cut) is
+// the chunk's own map, already published. Only the lanes that are `mine` publish.
+//
+// SCAN_GROUP chunks form a group. Its last chunk composes the group's map, and the
+// state behind a group is that map applied to the state in front of it; a chunk's
+// state is its group's, taken through the chunks of the group in front of it. So a
+// look back goes group by group, back to the nearest state that is there and forward
+// again through the maps, and what it finds does not depend on how far it had to go:
+// results are the same bits each time.
+//
+// Every wait ends: chunks are handed out by ticket in this order, so the workgroups
+// of all chunks in front have started. Each publishes its map without waiting for
+// anything, and the last of a group the group's map after waiting for such maps only.
+template <class A, int V>
+__device__ __forceinline__ void look_back(A* words, int64_t chunks, int64_t d, int64_t col,
+                                          int64_t c, const A (&fa)[V], const A (&fb)[V], bool cut,
+                                          bool mine, A (&x)[V]) {
+  const int64_t groups = chunks / SCAN_GROUP, g = c / SCAN_GROUP;
+  A* maps = words + chunks * 2 * d;       // [groups][2][d]
+  A* states = maps + groups * 2 * d;      // [groups][d]: behind each group
+  const bool closing = c % SCAN_GROUP == SCAN_GROUP - 1;
+  A ma[V], mb[V];
+  bool gone = cut;
+  if (closing) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) { ma[k] = A(1); mb[k] = A(0); }
+    scan_maps<A, V>(words, d, col, g * SCAN_GROUP, c, [&](A (&a)[V], A (&b)[V], bool step) {
+      const bool border = scan_is_cut(a[0]);
+      gone |= step && border;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const A to = border ? b[k] : scan_apply(a[k], b[k], mb[k]);
+        mb[k] = step ? to : mb[k];
+        ma[k] = step ? ma[k] * a[k] : ma[k];
+      }
+    });
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      mb[k] = cut ? fb[k] : scan_apply(fa[k], fb[k], mb[k]);
+      ma[k] = ma[k] * fa[k];
+      if (!mine) continue;
+      A* w = maps + g * 2 * d + col + k;
+      if (gone) publish_cut(w);
+      else publish(w, ma[k]);
+      publish(w + d, mb[k]);
+      if (gone) publish(states + g * d + col + k, mb[k]);
+    }
+  }
+  // the nearest group in front whose state is there; none: zeros
+#pragma unroll
+  for (int k = 0; k < V; ++k) x[k] = A(0);
+  int64_t j = g - 1;
+  for (bool found = false; j >= 0 && !found;) {
+    A s[SCAN_LOOK][V];
+    bool there[SCAN_LOOK];
+#pragma unroll
+    for (int q = 0; q < SCAN_LOOK; ++q) {
+      const A* w = states + (j - q > 0 ? j - q : 0) * d + col;
+      there[q] = true;
+#pragma unroll
+      for (int k = 0; k < V; ++k) there[q] &= observe(w + k, &s[q][k]);
+    }
+#pragma unroll
+    for (int q = 0; q < SCAN_LOOK; ++q) {
+      const bool last = !found && j >= 0 && __all(there[q]);
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[k] = last ? s[q][k] : x[k];
+      found |= last;
+      j -= !found && j >= 0;
+    }
+  }
+  scan_walk_maps<A, V>(maps, d, col, j + 1, g, x);
+  if (closing && !gone && mine) {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      publish(states + g * d + col + k, scan_apply(ma[k], mb[k], x[k]));
+  }
+  scan_walk_maps<A, V>(words, d, col, g * SCAN_GROUP, c, x);
 }
 
 // A chunk's rows, SCAN_BLOCK a thread: threads of `wide` lanes of columns form a
@@ -153,12 +238,14 @@ __device__ __forceinline__ void look_back(const A* words, int64_t d, int64_t col
 // over the strips in LDS.
 //
 // Bound by memory; 32,768 rows of 2,048 bfloat16 values with float gates, in four
-// sequences: forward 122 us (570 MB, 4.7 TB/s), gradient 181 us (955 MB,
-// 5.3 TB/s), where a copy of 1 GiB runs at 5.1 TB/s. Two columns a lane: four took
-// 138 and 195 us, as registers then leave room for half the wavefronts. Rows that
-// are not used yet stay as they came, two 16-bit values to a register: 311 us ->
-// 260 us for the gradient. 512 threads: 256 make the chain of chunks twice as long
-// (100,000 rows of 1,024 float16 values in one sequence: 190 us against 139 us).
+// sequences: forward 127 us (570 MB, 4.5 TB/s), gradient 190 us (955 MB,
+// 5.0 TB/s), where a copy of 1 GiB runs at 5.1 TB/s; 100,000 rows of 1,024 float16
+// values in one sequence, whose 782 chunks are one chain: 139 us (614 MB, 4.4 TB/s).
+// Two columns a lane: four took 10% longer, as registers then leave room for half
+// the wavefronts. Rows that are not used yet stay as they came, two 16-bit values to
+// a register: the gradient's 260 us became 195 us. 512 threads: 256 make the chain
+// twice as long (the one sequence 190 us). Groups of 4 chunks: 8 take 146 us for it,
+// 16 163 us, and no groups, with the state handed from chunk to chunk, 217 us.
 constexpr int PASS_BLOCK = 512;
 
 template <class T, class G, int V, bool BACK>
@@ -265,27 +352,28 @@ __global__ void __launch_bounds__(PASS_BLOCK) scan_pass_kernel(ScanArgs<T, G> p)
       for (int k = 0; k < V; ++k) carry[me][k] = A(0);
   } else if (me / WAVE == (BACK ? 0 : PASS_BLOCK / WAVE - 1)) {
     const bool mine = pos == strips - 1;  // narrow rows: several strips a wavefront
-    A* w = p.words + chunk * 3 * p.d + col;
     if (mine) {
+      A* w = p.words + order * 2 * p.d + col;
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        if (cut) {
-          publish(w + 2 * p.d + k, fb[k]);
-        } else {
-          publish(w + k, fa[k]);
-          publish(w + p.d + k, fb[k]);
-        }
+        if (cut) publish_cut(w + k);
+        else publish(w + k, fa[k]);
+        publish(w + p.d + k, fb[k]);
       }
     }
-    A s[V];
-    look_back<A, V, BACK>(p.words, p.d, col, order, p.chunks, s);
-    if (mine) {
+    // every strip of this wavefront looks back with the last one's map
+    const int last = BACK ? threadIdx.x % p.wide : WAVE - p.wide + threadIdx.x % p.wide;
+    A la[V], lb[V], s[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        if (!cut) publish(w + 2 * p.d + k, scan_apply(fa[k], fb[k], s[k]));
-        carry[me % p.wide][k] = s[k];
-      }
+    for (int k = 0; k < V; ++k) {
+      la[k] = __shfl(fa[k], last);
+      lb[k] = __shfl(fb[k], last);
     }
+    look_back<A, V>(p.words, p.chunks, p.d, col, order, la, lb, __shfl((int)cut, last) != 0, mine,
+                    s);
+    if (mine)
+#pragma unroll
+      for (int k = 0; k < V; ++k) carry[me % p.wide][k] = s[k];
   }
   __syncthreads();
   if (!any) return;
@@ -420,7 +508,7 @@ hipError_t run_scan_pass(ScanArgs<T, G> p, void* workspace, bool back, hipStream
   if (p.chunks > 1) {
     p.ticket = (uint32_t*)workspace;
     p.words = (A*)((char*)workspace + SCAN_TICKET_BYTES);
-    const int64_t words = p.chunks * 3 * p.d * (int64_t)(sizeof(A) / 4);
+    const int64_t words = scan_words(p.chunks) * p.d * (int64_t)(sizeof(A) / 4);
     const hipError_t e = launch_scan_reset(p.ticket, (uint32_t*)p.words, words, s);
     if (e != hipSuccess) return e;
   }

@@ -58,9 +58,9 @@ hipError_t launch_segment_marks(const int32_t* offsets, int64_t num_seg, int64_t
 }
 
 int64_t scan_workspace_bytes(int64_t n, int64_t d, int dtype) {
-  // chunks of 128 rows at least, three words a column; one chunk needs none
+  // chunks of 128 rows at least; one chunk needs none
   const int64_t chunks = (n + 127) / 128;
-  return chunks > 1 ? SCAN_TICKET_BYTES + chunks * 3 * d * (dtype == DT_F64 ? 8 : 4) : 0;
+  return chunks > 1 ? SCAN_TICKET_BYTES + scan_words(chunks) * d * (dtype == DT_F64 ? 8 : 4) : 0;
 }
 
 hipError_t launch_scan(const ScanParams& q, bool back, int dtype) {

@@ -490,6 +490,16 @@ def hand_back(t: torch.Tensor, where):
     return t.cpu().numpy() if where is None else t if t.device == where else t.to(where)
 
 
+def used_here(made_on: int, *tensors) -> None:
+    """Tell the allocator that a plan's tensors, made on the stream `made_on`, are
+    read on the current one: their memory is not given out before that is done, even
+    if the plan is dropped meanwhile."""
+    if stream() != made_on:
+        current = torch.cuda.current_stream()
+        for t in tensors:
+            t.record_stream(current)
+
+
 def state_dtype(dtype: torch.dtype) -> torch.dtype:
     """What the row operators keep sums and states of `dtype` values in."""
     return torch.float64 if dtype == torch.float64 else torch.float32

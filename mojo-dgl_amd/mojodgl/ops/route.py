@@ -131,7 +131,7 @@ class RoutePlan:
         self.num_rows = flat.shape[0]
         self.k = flat.shape[1] if flat.ndim == 2 else 1
         self.num_experts = num_experts
-        self.device_index = _lib.current_device()
+        self.device_index, self._stream = _lib.current_device(), _lib.stream()
         m = flat.numel()
         dev = flat.device
         nbytes = L.mdgl_route_plan_workspace_bytes(m, num_experts)
@@ -169,6 +169,7 @@ def _check_plan(plan, what):
     if plan.device_index != _lib.current_device():
         raise DGLError("the plan lies on GPU {}, the current one is {}".format(
             plan.device_index, _lib.current_device()))
+    _lib.used_here(plan._stream, plan.slot)
 
 
 def dispatch_rows(value, plan):

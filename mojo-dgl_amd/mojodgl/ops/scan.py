@@ -42,7 +42,7 @@ class SegmentPlan:
         self.num_rows, self.num_segments = num_rows, seg.num
         self.has_empty = bool(seg.num) and seg.shortest == 0
         self.offsets = seg.device()
-        self.device_index = _lib.current_device()
+        self.device_index, self._stream = _lib.current_device(), _lib.stream()
         words = (num_rows + 63) // 64
         self.ids = torch.empty(num_rows, dtype=torch.int32, device=dev)
         self.starts = torch.empty(words, dtype=torch.int64, device=dev)
@@ -165,6 +165,7 @@ def _plan_for(seglen, n) -> SegmentPlan:
     if seglen.device_index != _lib.current_device():
         raise DGLError("the plan lies on GPU {}, the current one is {}".format(
             seglen.device_index, _lib.current_device()))
+    _lib.used_here(seglen._stream, seglen.offsets, seglen.ids, seglen.starts, seglen.ends)
     return seglen
 
 

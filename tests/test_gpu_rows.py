@@ -515,6 +515,49 @@ def test_results_are_the_same_each_time():
         assert same(run(), first)
 
 
+def test_scan_results_do_not_depend_on_timing():
+    """Chains of hundreds of chunks beside other work on the GPU, which changes how far
+    each chunk has to look back: the same bits."""
+    g = gen(20)
+    n, d = 120_000, 200
+    a = 0.99 + 0.01 * torch.rand(n, d, generator=g, device="cuda")
+    v, dh = rand(g, n, d), rand(g, n, d)
+    plan = ops.segment_plan([n - 50_000, 50_000])
+
+    def run():
+        A, V = a.detach().requires_grad_(), v.detach().requires_grad_()
+        h = ops.segment_scan(plan, A, V)
+        return [h.detach()] + list(torch.autograd.grad(h, (A, V), dh))
+
+    first = bits(run())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for i in range(12):
+        with torch.cuda.stream(side):
+            for _ in range(i):
+                ops.layer_norm(v[: 10_000 * (i + 1)])
+        assert same(run(), first)
+    torch.cuda.synchronize()
+
+
+def test_a_plan_dropped_while_another_stream_reads_it():
+    g = gen(21)
+    x = rand(g, 4000, 64)
+    want = ops.segment_scan([1500, 2500], torch.sigmoid(x), x)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    plan = ops.segment_plan([1500, 2500])
+    with torch.cuda.stream(side):
+        z = x
+        for _ in range(50):
+            z = z * 1.0
+        got = ops.segment_scan(plan, torch.sigmoid(z), z)
+    del plan
+    junk = [torch.full((4000,), -1, dtype=torch.int32, device="cuda") for _ in range(8)]
+    side.synchronize()
+    assert torch.equal(got, want) and len(junk) == 8
+
+
 def test_other_streams():
     """Each call runs on the current stream, behind what its inputs wait for there; a
     plan made on one stream serves another."""

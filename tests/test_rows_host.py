@@ -142,6 +142,7 @@ def test_abi_layer_norm(lib):
                  (P, P, P, P, P, None, 4, 4, 1e-5, F32, F32),
                  (P, P, P, P, None, None, -4, 4, 1e-5, F32, F32),
                  (P, P, P, P, None, None, 4, 2 ** 30, 1e-5, F32, F32),
+                 (P, P, P, P, None, None, 4, 2 ** 26, 1e-5, F16, F32),
                  (P, P, P, P, None, None, 4, 4, 1e-5, F32, F64),
                  (P, P, P, P, None, None, 4, 4, 1e-5, BF16, F16),
                  (P, P, P, P, None, None, 4, 4, 1e-5, 7, 7),
