@@ -16,6 +16,12 @@
 // for a workgroup's registers go through norm_wide_kernel and norm_cols_kernel,
 // which read them again instead.
 //
+// Bound by memory: 32,768 bfloat16 rows of 4,096 take 99 us forward (537 MB, 5.4 TB/s)
+// and 172 + 5 us backward (805 MB and 17 MB of partial sums, 4.8 TB/s), a million float32
+// rows of 47 75 us (376 MB, 5.0 TB/s) and 115 + 9 us (564 MB, 4.9 TB/s), where a copy of
+// 1 GiB runs at 5.1 TB/s. A workgroup a row from 256 vectors on: a wavefront a row would
+// hold 512 vectors in 256 registers and leave one wavefront a SIMD in the gradient.
+//
 // A row whose width is no whole number of vectors ends with a vector that shares
 // columns with the one before it: they count once in every sum, and both write
 // the same values.

@@ -141,27 +141,16 @@ __device__ __forceinline__ void scan_maps(const A* words, int64_t d, int64_t col
   }
 }
 
-template <class A, int V>
-__device__ __forceinline__ void scan_walk_maps(const A* words, int64_t d, int64_t col, int64_t i,
-                                               int64_t end, A (&x)[V]) {
-  scan_maps<A, V>(words, d, col, i, end, [&](A (&a)[V], A (&b)[V], bool step) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const A to = scan_is_cut(a[k]) ? b[k] : scan_apply(a[k], b[k], x[k]);
-      x[k] = step ? to : x[k];
-    }
-  });
-}
-
 // The state in front of chunk `c` in the order of the walk, into x; (fa, fb, cut) is
 // the chunk's own map, already published. Only the lanes that are `mine` publish.
 //
-// SCAN_GROUP chunks form a group. Its last chunk composes the group's map, and the
-// state behind a group is that map applied to the state in front of it; a chunk's
-// state is its group's, taken through the chunks of the group in front of it. So a
-// look back goes group by group, back to the nearest state that is there and forward
-// again through the maps, and what it finds does not depend on how far it had to go:
-// results are the same bits each time.
+// SCAN_GROUP chunks form a group. A chunk composes the maps of its group's chunks in
+// front of it, and applies that to the state in front of the group, unless a border
+// lies between; the group's last chunk composes the group's map and, with the same
+// state, the state behind it. The state in front of a group is looked for group by
+// group, back to the nearest that is there and forward again through the groups' maps.
+// What is found does not depend on how far that was: each state is one map applied
+// to one other, always the same two. Results are the same bits each time.
 //
 // Every wait ends: chunks are handed out by ticket in this order, so the workgroups
 // of all chunks in front have started. Each publishes its map without waiting for
@@ -175,62 +164,73 @@ __device__ __forceinline__ void look_back(A* words, int64_t chunks, int64_t d, i
   A* states = maps + groups * 2 * d;      // [groups][d]: behind each group
   const bool closing = c % SCAN_GROUP == SCAN_GROUP - 1;
   A ma[V], mb[V];
-  bool gone = cut;
-  if (closing) {
+  bool border = false;
 #pragma unroll
-    for (int k = 0; k < V; ++k) { ma[k] = A(1); mb[k] = A(0); }
-    scan_maps<A, V>(words, d, col, g * SCAN_GROUP, c, [&](A (&a)[V], A (&b)[V], bool step) {
-      const bool border = scan_is_cut(a[0]);
-      gone |= step && border;
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const A to = border ? b[k] : scan_apply(a[k], b[k], mb[k]);
-        mb[k] = step ? to : mb[k];
-        ma[k] = step ? ma[k] * a[k] : ma[k];
-      }
-    });
+  for (int k = 0; k < V; ++k) { ma[k] = A(1); mb[k] = A(0); }
+  scan_maps<A, V>(words, d, col, g * SCAN_GROUP, c, [&](A (&a)[V], A (&b)[V], bool step) {
+    const bool here = scan_is_cut(a[0]);
+    border |= step && here;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      mb[k] = cut ? fb[k] : scan_apply(fa[k], fb[k], mb[k]);
-      ma[k] = ma[k] * fa[k];
+      const A to = here ? b[k] : scan_apply(a[k], b[k], mb[k]);
+      mb[k] = step ? to : mb[k];
+      ma[k] = step ? ma[k] * a[k] : ma[k];
+    }
+  });
+  A ga[V], gb[V];
+  if (closing) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      gb[k] = cut ? fb[k] : scan_apply(fa[k], fb[k], mb[k]);
+      ga[k] = ma[k] * fa[k];
       if (!mine) continue;
       A* w = maps + g * 2 * d + col + k;
-      if (gone) publish_cut(w);
-      else publish(w, ma[k]);
-      publish(w + d, mb[k]);
-      if (gone) publish(states + g * d + col + k, mb[k]);
+      if (cut || border) publish_cut(w);
+      else publish(w, ga[k]);
+      publish(w + d, gb[k]);
+      if (cut || border) publish(states + g * d + col + k, gb[k]);
     }
   }
-  // the nearest group in front whose state is there; none: zeros
 #pragma unroll
-  for (int k = 0; k < V; ++k) x[k] = A(0);
+  for (int k = 0; k < V; ++k) x[k] = mb[k];
+  if (border) return;
+  // the nearest group in front whose state is there; none: zeros
+  A s[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) s[k] = A(0);
   int64_t j = g - 1;
   for (bool found = false; j >= 0 && !found;) {
-    A s[SCAN_LOOK][V];
+    A t[SCAN_LOOK][V];
     bool there[SCAN_LOOK];
 #pragma unroll
     for (int q = 0; q < SCAN_LOOK; ++q) {
       const A* w = states + (j - q > 0 ? j - q : 0) * d + col;
       there[q] = true;
 #pragma unroll
-      for (int k = 0; k < V; ++k) there[q] &= observe(w + k, &s[q][k]);
+      for (int k = 0; k < V; ++k) there[q] &= observe(w + k, &t[q][k]);
     }
 #pragma unroll
     for (int q = 0; q < SCAN_LOOK; ++q) {
       const bool last = !found && j >= 0 && __all(there[q]);
 #pragma unroll
-      for (int k = 0; k < V; ++k) x[k] = last ? s[q][k] : x[k];
+      for (int k = 0; k < V; ++k) s[k] = last ? t[q][k] : s[k];
       found |= last;
       j -= !found && j >= 0;
     }
   }
-  scan_walk_maps<A, V>(maps, d, col, j + 1, g, x);
-  if (closing && !gone && mine) {
+  scan_maps<A, V>(maps, d, col, j + 1, g, [&](A (&a)[V], A (&b)[V], bool step) {
 #pragma unroll
-    for (int k = 0; k < V; ++k)
-      publish(states + g * d + col + k, scan_apply(ma[k], mb[k], x[k]));
+    for (int k = 0; k < V; ++k) {
+      const A to = scan_is_cut(a[k]) ? b[k] : scan_apply(a[k], b[k], s[k]);
+      s[k] = step ? to : s[k];
+    }
+  });
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    x[k] = scan_apply(ma[k], mb[k], s[k]);
+    if (closing && !cut && mine)
+      publish(states + g * d + col + k, scan_apply(ga[k], gb[k], s[k]));
   }
-  scan_walk_maps<A, V>(words, d, col, g * SCAN_GROUP, c, x);
 }
 
 // A chunk's rows, SCAN_BLOCK a thread: threads of `wide` lanes of columns form a
@@ -238,9 +238,9 @@ __device__ __forceinline__ void look_back(A* words, int64_t chunks, int64_t d, i
 // over the strips in LDS.
 //
 // Bound by memory; 32,768 rows of 2,048 bfloat16 values with float gates, in four
-// sequences: forward 127 us (570 MB, 4.5 TB/s), gradient 190 us (955 MB,
-// 5.0 TB/s), where a copy of 1 GiB runs at 5.1 TB/s; 100,000 rows of 1,024 float16
-// values in one sequence, whose 782 chunks are one chain: 139 us (614 MB, 4.4 TB/s).
+// sequences: forward 125 us (570 MB, 4.6 TB/s), gradient 187 us (955 MB,
+// 5.1 TB/s), where a copy of 1 GiB runs at 5.1 TB/s; 100,000 rows of 1,024 float16
+// values in one sequence, whose 782 chunks are one chain: 145 us (614 MB, 4.2 TB/s).
 // Two columns a lane: four took 10% longer, as registers then leave room for half
 // the wavefronts. Rows that are not used yet stay as they came, two 16-bit values to
 // a register: the gradient's 260 us became 195 us. 512 threads: 256 make the chain

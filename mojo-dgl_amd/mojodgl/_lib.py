@@ -470,8 +470,8 @@ def rows(a) -> torch.Tensor:
 
 def rows_on_device(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """The operand as a contiguous tensor of `dtype` on the current GPU."""
-    if t.dtype is dtype and t.is_cuda and t.get_device() == current_device() \
-            and t.is_contiguous():
+    if t.dtype is dtype and t.is_cuda and t.is_contiguous() \
+            and t.get_device() == (_get_device or current_device)():
         return t
     return t.detach().to(device=device(), dtype=dtype).contiguous()
 

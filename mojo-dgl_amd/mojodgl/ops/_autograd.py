@@ -74,8 +74,11 @@ __all__ = ["needs_grad", "GSpMM", "GSDDMM", "EdgeSoftmax", "SegmentReduce", "Seg
 
 
 def needs_grad(*xs) -> bool:
-    return torch.is_grad_enabled() and any(
-        isinstance(x, torch.Tensor) and x.requires_grad for x in xs)
+    if torch.is_grad_enabled():
+        for x in xs:
+            if isinstance(x, torch.Tensor) and x.requires_grad:
+                return True
+    return False
 
 
 def _gpu(t):
@@ -590,6 +593,8 @@ def _back(g, like):
     """A gradient in the operand's dtype and on its device (None for numpy)."""
     if g is None or not isinstance(like, torch.Tensor):
         return None
+    if g.dtype is like.dtype and g.device == like.device:
+        return g
     return g.to(device=like.device, dtype=like.dtype)
 
 

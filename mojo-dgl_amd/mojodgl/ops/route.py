@@ -100,7 +100,8 @@ def _topk_route_grad(logits, ids, grad, score, renormalize, scale):
     xt = x.dtype
     x = _lib.rows_on_device(x, xt)
     g = _lib.rows_on_device(grad, _lib.state_dtype(xt))
-    ids = _lib.i64_device(ids) if ids.is_cuda else ids.to(x.device)
+    if ids.device != x.device:
+        ids = ids.to(x.device)
     dx = torch.empty_like(x)
     _lib.check(_lib.lib().mdgl_topk_route_grad(
         x.data_ptr(), ids.data_ptr(), g.data_ptr(), dx.data_ptr(), n, e, ids.shape[1],
