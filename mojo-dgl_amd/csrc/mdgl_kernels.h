@@ -380,6 +380,7 @@ struct NormParams {
 };
 // shape: the instance (threads a row, vectors a thread); parts: the gradient's
 // workgroups, whose sums of dw and db are added afterwards.
+constexpr int NORM_WIDE_SHAPE = 99;  // rows read again instead of held
 struct NormGeometry {
   int shape;
   int64_t parts;

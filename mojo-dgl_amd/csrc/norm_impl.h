@@ -8,7 +8,7 @@
 // Both passes read and write each row once: a group of G threads holds a row in
 // registers, K vectors of 16 bytes a thread, so the variance is summed around the
 // mean (no difference of large squares) without a second read. G is 8 to 64 lanes
-// of a wavefront for rows of up to 128 vectors, a workgroup of 256 or 512 for
+// of a wavefront for rows of up to 128 vectors, a workgroup of 256 to 1,024 for
 // wider ones; a group goes on to further rows with the next one's loads in
 // flight. The gradient sums its rows' dw and db in registers, adds the groups of
 // a workgroup in a fixed order through LDS, leaves one row of sums a workgroup, and
@@ -174,8 +174,9 @@ template <class T, class W, int V, int G, int K>
 __global__ void __launch_bounds__(norm_block<G>()) norm_grad_kernel(NormArgs<T, W> p) {
   using A = acc_t<T>;
   constexpr int GROUPS = norm_block<G>() / G;
-  // four vectors a thread leave no registers for w and the next row's loads
-  constexpr bool HOLD = K < 4;
+  // four vectors a thread leave no registers for w, and with 1,024 threads (128
+  // registers each) none for the next row's loads either
+  constexpr bool HOLD = K < 4, AHEAD = G < 1024;
   __shared__ A lds[G > WAVE ? 4 * (G / WAVE) : 1];
   __shared__ A sums[GROUPS > 1 ? 2 * G * K * V : 1];
   int turn = 0;
@@ -200,46 +201,61 @@ __global__ void __launch_bounds__(norm_block<G>()) norm_grad_kernel(NormArgs<T, 
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   const A inv = A(1) / (A)p.d;
   int64_t row = (int64_t)blockIdx.x * GROUPS + group;
-  T xr[K][V], gr[K][V];
-  A mean = A(0), r = A(0);
+  // rows stay as they came from memory, 16-bit values two to a register, and xh and g
+  // are formed again for dx: the registers saved leave room for the next row's loads
+  Held<T, V> xn[K], gn[K];
+  A mean_n = A(0), r_n = A(0);
   auto fetch = [&](int64_t at) {
     if (at >= p.n) return;
-    mean = p.mean[at];
-    r = p.rstd[at];
+    mean_n = p.mean[at];
+    r_n = p.rstd[at];
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       if (!live[j]) continue;
-      load_any<false>(p.x + at * p.d + col[j], xr[j]);
-      load_any<false>(p.dy + at * p.d + col[j], gr[j]);
+      xn[j].load(p.x + at * p.d + col[j]);
+      gn[j].load(p.dy + at * p.d + col[j]);
     }
   };
-  if (HOLD) fetch(row);
+  fetch(row);
   while (row < p.n) {
-    if (!HOLD) fetch(row);
-    A x[K][V], g[K][V];
-    const A r0 = r;
-    A s = A(0), q = A(0);
+    Held<T, V> x[K], g[K];
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      if (!HOLD) {
+      x[j] = xn[j];
+      g[j] = gn[j];
+    }
+    const A mean = mean_n, r = r_n;
+    const int64_t next = row + step;
+    if (AHEAD) fetch(next);
+    A s = A(0), q = A(0);
+    // xh and g of vector j
+    auto form = [&](int j, A (&xh)[V], A (&dy)[V], A (&gw)[V]) {
+      if constexpr (!HOLD) {
 #pragma unroll
         for (int k = 0; k < V; ++k) w[0][k] = A(1);
-        if (live[j] && p.w) load_acc<W, A, V>(p.w + col[j], w[0]);
+        if (p.w) load_acc<W, A, V>(p.w + col[j], w[0]);
       }
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const A dy = live[j] ? (A)gr[j][k] : A(0);
-        x[j][k] = live[j] ? ((A)xr[j][k] - mean) * r : A(0);
-        dw[j][k] = fma_of(dy, x[j][k], dw[j][k]);
-        db[j][k] += dy;
-        g[j][k] = dy * w[HOLD ? j : 0][k];
-        const A c = k >= skip[j] ? g[j][k] : A(0);
+        dy[k] = g[j].at(k);
+        xh[k] = (x[j].at(k) - mean) * r;
+        gw[k] = dy[k] * w[HOLD ? j : 0][k];
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      if (!live[j]) continue;
+      A xh[V], dy[V], gw[V];
+      form(j, xh, dy, gw);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        dw[j][k] = fma_of(dy[k], xh[k], dw[j][k]);
+        db[j][k] += dy[k];
+        const A c = k >= skip[j] ? gw[k] : A(0);
         s += c;
-        q = fma_of(c, x[j][k], q);
+        q = fma_of(c, xh[k], q);
       }
     }
-    const int64_t next = row + step;
-    if (HOLD) fetch(next);
     if (p.dx) {
       norm_sum2<G>(s, q, lds, turn);
       s *= inv;
@@ -247,11 +263,14 @@ __global__ void __launch_bounds__(norm_block<G>()) norm_grad_kernel(NormArgs<T, 
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         if (!live[j]) continue;
+        A xh[V], dy[V], gw[V];
+        form(j, xh, dy, gw);
 #pragma unroll
-        for (int k = 0; k < V; ++k) g[j][k] = r0 * (g[j][k] - s - x[j][k] * q);
-        store_acc<T, A, V>(p.dx + row * p.d + col[j], g[j]);
+        for (int k = 0; k < V; ++k) gw[k] = r * (gw[k] - s - xh[k] * q);
+        store_acc<T, A, V>(p.dx + row * p.d + col[j], gw);
       }
     }
+    if (!AHEAD) fetch(next);
     row = next;
   }
   if (!p.part_w && !p.part_b) return;
@@ -427,6 +446,11 @@ hipError_t run_norm_width(const NormParams& q) {
     case 7: e = run_norm<T, W, V, 256, 2>(p, back, parts, s); break;
     case 8: e = run_norm<T, W, V, 512, 2>(p, back, parts, s); break;
     case 9: e = run_norm<T, W, V, 512, 4>(p, back, parts, s); break;
+    case 10:
+      if constexpr (V <= 4) {
+        e = run_norm<T, W, V, 1024, 4>(p, back, parts, s);
+        break;
+      }
     default: {
       const int64_t grid = q.n < 1024 ? q.n : 1024;
       if (!back) {

@@ -11,8 +11,10 @@ NormGeometry norm_geometry(int64_t n, int64_t d, int size) {
   const int64_t nv = (d + V - 1) / V;
   const struct { int64_t vecs; int threads; } shapes[] = {
       {8, 8}, {8, 8}, {16, 16}, {32, 32}, {64, 64}, {128, 64},
-      {256, 256}, {512, 256}, {1024, 512}, {2048, 512}};
-  constexpr int COUNT = sizeof shapes / sizeof shapes[0];
+      {256, 256}, {512, 256}, {1024, 512}, {2048, 512},
+      {4096, 1024}};
+  // 16-bit rows of more than 2,048 vectors have more sums than 1,024 threads' registers
+  const int COUNT = (int)(sizeof shapes / sizeof shapes[0]) - (size == 2 ? 1 : 0);
   int shape = d < V ? 0 : 1;
   if (shape) while (shape < COUNT && shapes[shape].vecs < nv) ++shape;
   // workgroups of the gradient, each of which leaves a row of sums
@@ -26,7 +28,7 @@ NormGeometry norm_geometry(int64_t n, int64_t d, int size) {
     const int64_t want = (n + block / g - 1) / (block / g), most = 256 * (1024 / block);
     parts = want < most ? want : most;
   }
-  return {shape, parts < 1 ? 1 : parts};
+  return {shape == COUNT ? NORM_WIDE_SHAPE : shape, parts < 1 ? 1 : parts};
 }
 
 int64_t norm_workspace_bytes(int64_t n, int64_t d, int dtype) {
