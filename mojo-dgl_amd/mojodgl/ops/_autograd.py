@@ -689,8 +689,7 @@ class LayerNorm(torch.autograd.Function):
     def forward(ctx, value, weight, bias, eps):
         from .norm import _layer_norm
 
-        y, mean, rstd = _layer_norm(value, weight, bias, eps, True)
-        ctx.stats = mean, rstd
+        y, ctx.stats = _layer_norm(value, weight, bias, eps, True)
         _save_some(ctx, value, weight, bias)
         return _lib.hand_back(y, _lib.caller_device(value, weight, bias))
 
@@ -700,7 +699,7 @@ class LayerNorm(torch.autograd.Function):
         from .norm import _layer_norm_grad
 
         value, weight, bias = _saved_some(ctx)
-        dx, dw, db = _layer_norm_grad(value, weight, bias, *ctx.stats, grad,
+        dx, dw, db = _layer_norm_grad(value, weight, bias, ctx.stats, grad,
                                       ctx.needs_input_grad[:3])
         return _back(dx, value), _back(dw, weight), _back(db, bias), None
 

@@ -36,7 +36,7 @@ def layer_norm(value, weight=None, bias=None, eps=1e-5):
     """
     if _autograd.needs_grad(value, weight, bias):
         return _autograd.LayerNorm.apply(value, weight, bias, eps)
-    y = _layer_norm(value, weight, bias, eps, False)[0]
+    y, _ = _layer_norm(value, weight, bias, eps, False)
     return _lib.hand_back(y, _lib.caller_device(value, weight, bias))
 
 
@@ -62,7 +62,7 @@ def _operands(value, weight, bias):
 
 
 def _layer_norm(value, weight, bias, eps, want_stats):
-    """(y, mean, rstd) on the GPU."""
+    """(y, stats) on the GPU; stats: the rows' means, then their 1 / deviations."""
     x, w, b, vt, wt, d = _operands(value, weight, bias)
     eps = float(eps)
     if not eps >= 0.0:
@@ -73,16 +73,22 @@ def _layer_norm(value, weight, bias, eps, want_stats):
     b = None if b is None else _lib.rows_on_device(b, wt)
     n = x.numel() // d if d else 0
     y = torch.empty_like(x)
-    mean = rstd = None
+    stats = mean = rstd = None
     if want_stats:
-        mean, rstd = torch.empty(2, n, dtype=_lib.state_dtype(vt), device=x.device).unbind(0)
+        stats = torch.empty(2 * n, dtype=_lib.state_dtype(vt), device=x.device)
+        mean, rstd = _stats_ptrs(stats)
     _lib.check(_lib.lib().mdgl_layer_norm(
-        x.data_ptr(), _lib.ptr(w), _lib.ptr(b), y.data_ptr(), _lib.ptr(mean), _lib.ptr(rstd), n, d,
-        eps, _lib.ROW_CODES[vt], _lib.ROW_CODES[wt], _lib.stream()), "layer_norm")
-    return y, mean, rstd
+        x.data_ptr(), _lib.ptr(w), _lib.ptr(b), y.data_ptr(), mean, rstd, n, d, eps,
+        _lib.ROW_CODES[vt], _lib.ROW_CODES[wt], _lib.stream()), "layer_norm")
+    return y, stats
 
 
-def _layer_norm_grad(value, weight, bias, mean, rstd, grad, need):
+def _stats_ptrs(stats):
+    base = stats.data_ptr()
+    return base, base + stats.numel() // 2 * stats.element_size()
+
+
+def _layer_norm_grad(value, weight, bias, stats, grad, need):
     """(dvalue, dweight, dbias) on the GPU, those that `need` wants."""
     x, w, _, vt, wt, d = _operands(value, weight, bias)
     x = _lib.rows_on_device(x, vt)
@@ -102,7 +108,6 @@ def _layer_norm_grad(value, weight, bias, mean, rstd, grad, need):
         nbytes = L.mdgl_layer_norm_grad_workspace_bytes(n, d, code)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
     _lib.check(L.mdgl_layer_norm_grad(
-        x.data_ptr(), _lib.ptr(w), mean.data_ptr(), rstd.data_ptr(), g.data_ptr(), _lib.ptr(dx),
-        _lib.ptr(dw), _lib.ptr(db), n, d, _lib.ptr(ws), nbytes, code, _lib.ROW_CODES[wt],
+        x.data_ptr(), _lib.ptr(w), *_stats_ptrs(stats), g.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), n, d, _lib.ptr(ws), nbytes, code, _lib.ROW_CODES[wt],
         _lib.stream()), "layer_norm_grad")
     return dx, dw, db
