@@ -426,6 +426,28 @@ def test_scan_types_meet():
     assert d.dtype == F16
 
 
+def test_scan_of_cpu_tensors():
+    """Results and gradients come back to where the operands are."""
+    lens = [40, 0, 90]
+    args = scan_inputs(16, lens, 12, F32, F32)
+    a, v, init, dh, dl = args
+
+    def run(*t):
+        a, v, init, dh, dl = t
+        A, V, I = (x.detach().requires_grad_() for x in (a, v, init))  # noqa: E741
+        h, last = ops.segment_scan(lens, A, V, I, return_state=True)
+        return [h.detach(), last.detach()] + \
+            list(torch.autograd.grad((h, last), (A, V, I), (dh, dl)))
+
+    for got, want in zip(run(*(t.cpu() for t in args)), run(*args)):
+        assert got.device.type == "cpu" and torch.equal(got, want.cpu())
+    # gates on the GPU, values on the CPU: results where the values are
+    A, V = a.detach().requires_grad_(), v.cpu().requires_grad_()
+    h = ops.segment_scan(lens, A, V)
+    da, dv = torch.autograd.grad(h, (A, V), dh.cpu())
+    assert h.device.type == dv.device.type == "cpu" and da.device.type == "cuda"
+
+
 def test_scan_strides_alignment_and_broadcasts():
     g = gen(7)
     lens = [50, 0, 83]
