@@ -665,7 +665,8 @@ int64_t mdgl_layer_norm_grad_workspace_bytes(int64_t n, int64_t d, int dtype);
  * the logits; keys: score + bias (state, num_experts; null: the order of the
  * logits). With topk_groups < num_groups the experts of the best groups only
  * (num_experts / num_groups neighbours each; num_groups at most 64), by the largest
- * key of a group or the sum of its two largest. weights = scale * score, divided by
+ * key of a group or the sum of its two largest scores + bias (scores without a bias,
+ * too; a masked expert adds nothing). weights = scale * score, divided by
  * the sum of the row's k scores with `renormalize`. A logit of -inf masks its
  * expert: it is chosen only when nothing else is left, with a weight of 0. A NaN
  * ranks with the masked and makes the weights it enters NaN: its own, and all of a

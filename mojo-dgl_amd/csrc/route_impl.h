@@ -4,7 +4,8 @@
 //   s = softmax(x) or sigmoid(x) over a row's E logits x
 //   key = s + bias, or x itself without a bias (both scores grow with x)
 //   groups of E / groups neighbouring experts: the topk_groups best by their
-//   largest key, or by the sum of their two largest, stay
+//   largest key, or by the sum of their two best experts' s + bias, stay (a sum of
+//   scores, with or without a bias: one of logits has another order)
 //   ids = the k largest keys in falling order, the lowest index among equals
 //   w = scale * s[ids], divided by their sum when renormalised
 //
@@ -60,6 +61,16 @@ template <class K> __device__ __forceinline__ K lowest() { return -K(__builtin_h
 
 template <class K>
 __device__ __forceinline__ K sigmoid_of(K x) { return K(1) / (K(1) + exp_of(-x)); }
+
+// A score in float by the hardware's exponential and reciprocal; of softmax, as a
+// multiple of the score of `top`, the row's largest logit.
+constexpr float LOG2E = 1.44269504088896340736f;
+__device__ __forceinline__ float sigmoid_near(float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * x));
+}
+__device__ __forceinline__ float softmax_near(float x, float top) {
+  return x == top ? 1.0f : __builtin_amdgcn_exp2f(LOG2E * (x - top));  // both may be +inf
+}
 
 // Maximum / minimum over G lanes, in all of them. No value is NaN.
 template <int G, class K>
@@ -135,7 +146,6 @@ __device__ __forceinline__ uint32_t lanes_umax(uint32_t v) {
 template <class T, int G, int R>
 __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& p, const T* x,
                                                             int count) {
-  constexpr float LOG2E = 1.44269504088896340736f;
   const int lane = threadIdx.x % G;
   const int per = (p.e + G - 1) / G, base = lane * per;
   const int have = base >= p.e ? 0 : (p.e - base < per ? p.e - base : per);
@@ -158,11 +168,15 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
   c.near = false;
   c.id = 0;
   c.key = lowest<float>();
-  if (!p.sigmoid && (p.bias || !p.renorm)) {
-    // the row's softmax statistics; a NaN goes into the sum
+  // without a bias, the marks of groups by two experts need scores that no key has
+  const bool marks = p.groups > 1 && p.top2 && !p.bias, sums = !p.sigmoid && (p.bias || !p.renorm);
+  if (sums || marks) {
 #pragma unroll
     for (int i = 0; i < R; ++i) c.top = v[i] > c.top ? v[i] : c.top;
     c.top = lanes_max<G>(c.top);
+  }
+  if (sums) {
+    // the sum of softmax; a NaN goes into it
 #pragma unroll
     for (int i = 0; i < R; ++i)  // 0 where no expert is, and in a row of masks
       c.sum += v[i] == lowest<float>() ? 0.0f : expf(v[i] - c.top);
@@ -186,9 +200,8 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float y = v[i + q];
-        const float s = p.sigmoid
-                            ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * y))
-                            : __builtin_amdgcn_exp2f(LOG2E * (y - c.top)) * part;
+        const float s = p.sigmoid ? sigmoid_near(y)
+                                  : __builtin_amdgcn_exp2f(LOG2E * (y - c.top)) * part;
         const uint32_t k = ordered(s + b[q]);  // no -0: s is not negative
         key[i + q] = i + q >= have ? 0u : y > lowest<float>() ? k : KEY_LOWEST;
       }
@@ -203,8 +216,14 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
 
   if (p.groups > 1) {
     const int size = p.e / p.groups, span = route_span(p.e, p.groups, per);
+    auto score = [&](uint32_t k) {
+      const float y = unordered(k);
+      return p.sigmoid ? sigmoid_near(y) : softmax_near(y, c.top);
+    };
+    // a group's mark, from its two largest keys: -inf where all are masked
     // (a sum that overflows stays above a masked group's, and its row is near)
     auto grade = [&](uint32_t a, uint32_t b) {
+      if (marks && a > KEY_LOWEST) return b > KEY_LOWEST ? score(a) + score(b) : score(a);
       const float f = unordered(a);
       return p.top2 && b > KEY_LOWEST ? fmaxf(f + unordered(b), -__FLT_MAX__) : f;
     };
@@ -217,9 +236,10 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
       const uint32_t oa = __shfl_xor(a, off), ob = __shfl_xor(b, off);
       join_two(a, b, oa, ob);
     };
-    // lane j: the mark of group j, and how large the keys summed in it are
+    // lane j: the mark of group j, and how large what is summed in it is
     float mark = lowest<float>(), size_of = 0.0f;
     auto large = [&](uint32_t a, uint32_t b) {
+      if (marks) return a > KEY_LOWEST ? grade(a, b) : 0.0f;
       const float f = a > KEY_LOWEST ? abs_of(unordered(a)) : 0.0f;
       return p.top2 && b > KEY_LOWEST ? f + abs_of(unordered(b)) : f;
     };
@@ -259,8 +279,16 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
     const float lost_top = lanes_max<G>(real && !stays ? mark : lowest<float>());
     // marks are sums of up to two keys, of scores up to `most`
     const float big = lanes_max<G>(real ? size_of : 0.0f);
-    const float wrong = (p.bias ? (p.sigmoid ? 64.0f : 512.0f) * most : 0.0f) + 8.0f * big;
-    c.near = kept_low - lost_top <= wrong * 0x1p-24f && lost_top > lowest<float>();
+    float wrong = (p.bias ? (p.sigmoid ? 64.0f : 512.0f) * most : 0.0f) + 8.0f * big;
+    // without a bias, of two scores: each is wrong by at most 16 + 2 |x| half steps of
+    // itself (sigmoid; softmax: 16 + 3 (top - x)), as its argument rounds, and the
+    // larger the score the larger that is: four times its value at the row's top
+    if (marks) {
+      const float s = p.sigmoid ? sigmoid_near(c.top) * (16.0f + 2.0f * fmaxf(-c.top, 0.0f)) : 16.0f;
+      wrong = 4.0f * s + 8.0f * big;
+    }
+    // (below 2^-126 the hardware's exponential is 0)
+    c.near = kept_low - lost_top <= wrong * 0x1p-24f + 0x1p-100f && lost_top > lowest<float>();
     const uint64_t all = __ballot(stays) >> (threadIdx.x % WAVE / G * G);
     if (span) {
       const int mine = lane / span;
@@ -334,11 +362,14 @@ __device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T
   c.near = false;
   c.id = 0;
   c.key = lowest<K>();
-  if (!p.sigmoid && (p.bias || !p.renorm)) {
-    // the row's softmax statistics; a NaN goes into the sum
+  const bool marks = p.groups > 1 && p.top2 && !p.bias, sums = !p.sigmoid && (p.bias || !p.renorm);
+  if (sums || marks) {
 #pragma unroll
     for (int i = 0; i < R; ++i) c.top = key[i] > c.top ? key[i] : c.top;
     c.top = lanes_max<G>(c.top);
+  }
+  if (sums) {
+    // the sum of softmax; a NaN goes into it
 #pragma unroll
     for (int i = 0; i < R; ++i)
       c.sum += gone >> i & 1 || key[i] == lowest<K>() ? K(0) : exp_of(key[i] - c.top);
@@ -361,7 +392,13 @@ __device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T
   if (p.groups > 1) {
     const int size = p.e / p.groups;
     K mark = lowest<K>();  // lane j: the mark of group j
-    auto grade = [&](K a, K b) { return p.top2 && b > lowest<K>() ? a + b : a; };
+    auto score = [&](K y) {
+      return p.sigmoid ? sigmoid_of(y) : y == c.top ? K(1) : exp_of(y - c.top);
+    };
+    auto grade = [&](K a, K b) {
+      if (marks && a > lowest<K>()) return b > lowest<K>() ? score(a) + score(b) : score(a);
+      return p.top2 && b > lowest<K>() ? a + b : a;
+    };
     const int span = route_span(p.e, p.groups, per);
     const bool whole = span != 0;
     int mine = lane / (whole ? span : 1);  // the group of all of the lane's experts
@@ -485,7 +522,7 @@ __global__ void __launch_bounds__(BLOCK) route_kernel(RouteArgs<T> p) {
                         !(lane < p.k && x1 == logit && b1 == bias);
       again = near;
     }
-    // without a bias only sums of two logits can round
+    // without a bias only marks that are sums of scores can round
     again = again || (c.near && (p.bias || p.top2));
     for (uint64_t flags = __ballot(again); flags;) {
       const int g = __builtin_ctzll(flags) / G;  // the wavefront's g-th row

@@ -39,8 +39,8 @@ def topk_route(logits, k, score="softmax", bias=None, num_groups=1, topk_groups=
         experts' load); without it the logits' order decides
     num_groups : the experts fall into this many groups of neighbours (at most 64)
     topk_groups : only experts of this many best groups are chosen (None: all)
-    group_score : a group's rank: its 'max' score, or its best two's sum ('top2'),
-        with the bias
+    group_score : a group's rank: its 'max' score, or the sum of its best two
+        scores ('top2'), with the bias
     renormalize : divide a row's weights by their sum
     scale : factor of the weights
 
