@@ -97,6 +97,15 @@ __device__ __forceinline__ void join_two(K& a, K& b, K c, K d) {
   b = b > lo ? b : lo;
 }
 
+// How far a score of the float pass can be off, in half steps (2^-24) of itself. The
+// argument of the exponential is rounded, up to three times: sigmoid's error grows
+// with -x, softmax's with the distance to the row's largest logit. Beside that a few
+// steps of the exponential, the reciprocal, and softmax's sum over a lane's experts,
+// up to 32 of them, and over the lanes. Scores below 2^-126 are 0: callers add 2^-100.
+__device__ __forceinline__ float route_off(float x, float top, bool sigmoid) {
+  return sigmoid ? 16.0f + 2.0f * fmaxf(-x, 0.0f) : 64.0f + 3.0f * (top - x);
+}
+
 template <class K>
 struct Choice {
   int id;    // lane j: the j-th choice
@@ -280,13 +289,11 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
     // marks are sums of up to two keys, of scores up to `most`
     const float big = lanes_max<G>(real ? size_of : 0.0f);
     float wrong = (p.bias ? (p.sigmoid ? 64.0f : 512.0f) * most : 0.0f) + 8.0f * big;
-    // without a bias, of two scores: each is wrong by at most 16 + 2 |x| half steps of
-    // itself (sigmoid; softmax: 16 + 3 (top - x)), as its argument rounds, and the
-    // larger the score the larger that is: four times its value at the row's top
-    if (marks) {
-      const float s = p.sigmoid ? sigmoid_near(c.top) * (16.0f + 2.0f * fmaxf(-c.top, 0.0f)) : 16.0f;
-      wrong = 4.0f * s + 8.0f * big;
-    }
+    // without a bias, of two scores; the larger a score the more it can be off, so
+    // four times what it can be off at the row's top (softmax: its score there is 1)
+    if (marks)
+      wrong = 4.0f * (p.sigmoid ? sigmoid_near(c.top) : 1.0f) *
+                  route_off(c.top, c.top, p.sigmoid) + 8.0f * big;
     // (below 2^-126 the hardware's exponential is 0)
     c.near = kept_low - lost_top <= wrong * 0x1p-24f + 0x1p-100f && lost_top > lowest<float>();
     const uint64_t all = __ballot(stays) >> (threadIdx.x % WAVE / G * G);
@@ -514,11 +521,12 @@ __global__ void __launch_bounds__(BLOCK) route_kernel(RouteArgs<T> p) {
     if (p.bias) {
       const A bias = kept ? p.bias[id] : A(0);
       const A s = abs_of(c.key - bias);  // the score, near enough
+      const A off = s * route_off(logit, c.top, p.sigmoid);
       const A key1 = __shfl_up(c.key, 1, G), x1 = __shfl_up(logit, 1, G);
-      const A b1 = __shfl_up(bias, 1, G), s1 = __shfl_up(s, 1, G);
-      const A wrong = A(p.sigmoid ? 16 : 128) * (s + s1) + A(2) * (abs_of(c.key) + abs_of(key1));
+      const A b1 = __shfl_up(bias, 1, G), off1 = __shfl_up(off, 1, G);
+      const A wrong = off + off1 + A(2) * (abs_of(c.key) + abs_of(key1));
       const bool near = lane > 0 && kept && c.key > lowest<A>() &&
-                        key1 - c.key <= wrong * A(0x1p-24) &&
+                        key1 - c.key <= wrong * A(0x1p-24) + A(0x1p-100) &&
                         !(lane < p.k && x1 == logit && b1 == bias);
       again = near;
     }
