@@ -20,9 +20,12 @@
 // therefore makes one choice more than asked for, and a row two of whose
 // neighbouring keys (or whose last kept and first dropped group) lie closer than
 // the float keys can be wrong is chosen again in double, by a whole wavefront.
-// Chosen keys of equal logits and biases need no second look: they are equal however
-// they are formed. (The last chosen and the first that is not do: a third may lie
-// as close.)
+// Keys of equal logits and biases need no second look: they are equal however they
+// are formed. Behind the first that is not chosen lie others, perhaps with larger
+// scores, and errors, under lower biases: where it lies closer to the last chosen than
+// the largest error of the row, the row is chosen again (sigmoid: few scores are much
+// smaller than the largest), or each of them is compared first (softmax; 65,536 rows of
+// 256 with a bias: 43 us, 46 without that, and with it 53 instead of 50 for sigmoid).
 //
 // 65,536 rows of 256 float32 logits in 8 groups, 8 of 4 groups chosen, with a bias:
 // 54 us, and 18 us for the gradient, where reading and writing take 14 and 14. The
@@ -112,6 +115,7 @@ struct Choice {
   K key;     // and its key
   K top, sum;  // softmax: the row's largest logit, the sum of exp(x - top)
   bool near;   // the choice of groups hangs on the last bits
+  K limit;     // how far any of the row's scores can be off (float pass), in 2^-24
 };
 
 // The group of the lane's experts where every lane's lie in one, by its first
@@ -175,6 +179,7 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
   c.top = lowest<float>();
   c.sum = 0.0f;
   c.near = false;
+  c.limit = 0.0f;
   c.id = 0;
   c.key = lowest<float>();
   // without a bias, the marks of groups by two experts need scores that no key has
@@ -192,10 +197,12 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
     c.sum = group_sum(c.sum, G);
   }
   uint32_t key[R];
-  float most = 1.0f;  // no score is larger
+  // the larger a score the more it can be off: no more than the row's largest
+  if (marks)  // formed from multiples of softmax's largest
+    c.limit = (p.sigmoid ? sigmoid_near(c.top) : 1.0f) * route_off(c.top, c.top, p.sigmoid);
   if (p.bias) {
     const float part = c.sum > 0.0f ? 1.0f / c.sum : 0.0f;
-    if (!p.sigmoid) most = part;
+    uint32_t most = 0u;  // the largest score's bits; scores are not negative
 #pragma unroll
     for (int i = 0; i < R; i += 4) {
       float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -212,9 +219,15 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
         const float s = p.sigmoid ? sigmoid_near(y)
                                   : __builtin_amdgcn_exp2f(LOG2E * (y - c.top)) * part;
         const uint32_t k = ordered(s + b[q]);  // no -0: s is not negative
+        const uint32_t bits = __builtin_bit_cast(uint32_t, s);
+        most = bits > most ? bits : most;
         key[i + q] = i + q >= have ? 0u : y > lowest<float>() ? k : KEY_LOWEST;
       }
     }
+    // (1 beside a NaN; the logit of a sigmoid lies above its logarithm)
+    const float big = fminf(__builtin_bit_cast(float, lanes_umax<G>(most)), 1.0f);
+    const float at = p.sigmoid ? 0.6931472f * __builtin_amdgcn_logf(big + 0x1p-100f) : c.top;
+    c.limit = big * route_off(at, c.top, p.sigmoid);
   } else {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -286,15 +299,9 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
     const bool stays = real && before < p.topk_groups;
     const float kept_low = -lanes_max<G>(stays ? -mark : lowest<float>());
     const float lost_top = lanes_max<G>(real && !stays ? mark : lowest<float>());
-    // marks are sums of up to two keys, of scores up to `most`
+    // both marks are sums of up to two scores or keys, which round, too
     const float big = lanes_max<G>(real ? size_of : 0.0f);
-    float wrong = (p.bias ? (p.sigmoid ? 64.0f : 512.0f) * most : 0.0f) + 8.0f * big;
-    // without a bias, of two scores; the larger a score the more it can be off, so
-    // four times what it can be off at the row's top (softmax: its score there is 1)
-    if (marks)
-      wrong = 4.0f * (p.sigmoid ? sigmoid_near(c.top) : 1.0f) *
-                  route_off(c.top, c.top, p.sigmoid) + 8.0f * big;
-    // (below 2^-126 the hardware's exponential is 0)
+    const float wrong = 4.0f * c.limit + 8.0f * big;
     c.near = kept_low - lost_top <= wrong * 0x1p-24f + 0x1p-100f && lost_top > lowest<float>();
     const uint64_t all = __ballot(stays) >> (threadIdx.x % WAVE / G * G);
     if (span) {
@@ -340,6 +347,46 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
   return c;
 }
 
+// Softmax: whether an expert that was not chosen may belong in front of the last that
+// was, `id` (with its key, logit and bias, and how far its score can be off): the row's
+// keys once more, each with its own error. (Experts of dropped groups may answer, too.)
+template <class T, int G, int R>
+__device__ __forceinline__ bool route_rival(const RouteArgs<T>& p, const T* x, float top, float sum,
+                                            int id, float key, float logit, float bias,
+                                            float off) {
+  const int lane = threadIdx.x % G;
+  const int per = (p.e + G - 1) / G, base = lane * per;
+  const float part = sum > 0.0f ? 1.0f / sum : 0.0f;
+  const int have = base >= p.e ? 0 : (p.e - base < per ? p.e - base : per);
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < R; i += 4) {
+    T raw[4];
+    float b[4];
+    if (i + 4 <= have) {
+      load_any<false>(x + base + i, raw);
+      load_any<false>(p.bias + base + i, b);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        raw[q] = i + q < have ? x[base + i + q] : (T)lowest<float>();
+        b[q] = i + q < have ? p.bias[base + i + q] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float y = (float)raw[q];
+      const float s = __builtin_amdgcn_exp2f(LOG2E * (y - top)) * part;
+      const float k = s + b[q];
+      const int e = base + i + q;
+      const bool behind = y > lowest<float>() && (k < key || (k == key && e > id));
+      const float wrong = off + s * route_off(y, top, false) + 2.0f * (abs_of(k) + abs_of(key));
+      found |= behind && key - k <= wrong * 0x1p-24f + 0x1p-100f && !(y == logit && b[q] == bias);
+    }
+  }
+  return (__ballot(found) >> (threadIdx.x % WAVE / G * G) & (~uint64_t(0) >> (WAVE - G))) != 0;
+}
+
 // The first `count` choices of a row (count <= G), keys formed in K.
 template <class K, class T, int G, int R>
 __device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T* x, int count) {
@@ -367,6 +414,7 @@ __device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T
   c.top = lowest<K>();
   c.sum = K(0);
   c.near = false;
+  c.limit = K(0);
   c.id = 0;
   c.key = lowest<K>();
   const bool marks = p.groups > 1 && p.top2 && !p.bias, sums = !p.sigmoid && (p.bias || !p.renorm);
@@ -382,10 +430,8 @@ __device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T
       c.sum += gone >> i & 1 || key[i] == lowest<K>() ? K(0) : exp_of(key[i] - c.top);
     c.sum = group_sum(c.sum, G);
   }
-  K most = K(1);  // no score is larger
   if (p.bias) {
     const K part = c.sum > K(0) ? K(1) / c.sum : K(0);
-    if (!p.sigmoid) most = part;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (gone >> i & 1 || key[i] == lowest<K>()) continue;
@@ -524,11 +570,20 @@ __global__ void __launch_bounds__(BLOCK) route_kernel(RouteArgs<T> p) {
       const A off = s * route_off(logit, c.top, p.sigmoid);
       const A key1 = __shfl_up(c.key, 1, G), x1 = __shfl_up(logit, 1, G);
       const A b1 = __shfl_up(bias, 1, G), off1 = __shfl_up(off, 1, G);
-      const A wrong = off + off1 + A(2) * (abs_of(c.key) + abs_of(key1));
+      // the last lane's is the first that is not chosen: any other of these may be the
+      // one that belongs in front of it, whatever its score
+      const A wrong = (lane < p.k ? off : c.limit) + off1 + A(2) * (abs_of(c.key) + abs_of(key1));
       const bool near = lane > 0 && kept && c.key > lowest<A>() &&
                         key1 - c.key <= wrong * A(0x1p-24) + A(0x1p-100) &&
                         !(lane < p.k && x1 == logit && b1 == bias);
-      again = near;
+      again = near && (p.sigmoid || lane < p.k);
+      if (!p.sigmoid && __ballot(near && lane == p.k)) {
+        const int last = p.k - 1;
+        const bool rival = route_rival<T, G, R>(
+            p, x, top, sum, __shfl(id, last, G), __shfl(c.key, last, G), __shfl(logit, last, G),
+            __shfl(bias, last, G), __shfl(off, last, G));
+        again = again || (near && rival);
+      }
     }
     // without a bias only marks that are sums of scores can round
     again = again || (c.near && (p.bias || p.top2));

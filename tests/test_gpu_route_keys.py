@@ -66,6 +66,36 @@ def test_softmax_far_below_the_largest(depth):
             check(logits, bias, k, "softmax")
 
 
+def test_an_expert_of_larger_error_than_the_first_dropped():
+    """The first chosen and the first dropped key come from small scores with small
+    errors; behind them lies a large score, lowered by its bias, whose error reaches
+    the chosen one."""
+    x = torch.tensor([[-11.1723, -11.8963, 3.0226]], device="cuda")
+    bias = torch.tensor([0.00998594, 0.00999318, -0.94358444], device="cuda")
+    check(x, bias, 1, "sigmoid")
+    g = gen(3)
+    n = 20000
+    half = 2.0 ** -24
+    offset = [torch.tensor(t, device="cuda").double() for t in (0.00998, 0.009985, -0.94)]
+    for score in ("sigmoid", "softmax"):
+        back = torch.logit if score == "sigmoid" else torch.log
+        for lag in (0.5, 1.0, 2.0, 4.0):
+            # keys of 0.01: two of scores of 1e-5, one of a score of 0.95
+            large = back(0.95 + uniform(g, -1e-6, 1e-6, n, 1)).float()
+            s = torch.sigmoid(large.double()) if score == "sigmoid" else large.double().exp()
+            first = s + offset[2] + uniform(g, -lag * half, lag * half, n, 1)
+            second = (first + s + offset[2]) / 2
+            small = [first - offset[0], second - offset[1]]
+            cols = [back(t).float() for t in small] + [large]
+            bias = offset[:]
+            if score == "softmax":  # a fourth that makes the scores sum to 1
+                cols.append((1.0 - s - small[0] - small[1]).log().float())
+                bias.append(torch.tensor(-5.0, device="cuda"))
+            x, bias = torch.cat(cols, 1), torch.stack([t.float() for t in bias])
+            for k in (1, 2):
+                check(x, bias, k, score)
+
+
 @pytest.mark.parametrize("score", ["sigmoid", "softmax"])
 def test_groups_of_nearly_equal_keys(score):
     """Groups whose marks meet far below one half, and sums of biases past float32's
