@@ -243,11 +243,12 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
       return p.sigmoid ? sigmoid_near(y) : softmax_near(y, c.top);
     };
     // a group's mark, from its two largest keys: -inf where all are masked
-    // (a sum that overflows stays above a masked group's, and its row is near)
+    // (a sum that overflows stays finite, above a masked group's, and its row is near)
     auto grade = [&](uint32_t a, uint32_t b) {
       if (marks && a > KEY_LOWEST) return b > KEY_LOWEST ? score(a) + score(b) : score(a);
       const float f = unordered(a);
-      return p.top2 && b > KEY_LOWEST ? fmaxf(f + unordered(b), -__FLT_MAX__) : f;
+      if (!p.top2 || b <= KEY_LOWEST) return f;
+      return fminf(fmaxf(f + unordered(b), -__FLT_MAX__), __FLT_MAX__);
     };
     auto two = [](uint32_t& a, uint32_t& b, uint32_t k) {  // a >= b the larger two
       const uint32_t lo = k < a ? k : a;
@@ -450,7 +451,8 @@ __device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T
     };
     auto grade = [&](K a, K b) {
       if (marks && a > lowest<K>()) return b > lowest<K>() ? score(a) + score(b) : score(a);
-      return p.top2 && b > lowest<K>() ? a + b : a;
+      // (a sum of biases that overflows stays above a masked group's)
+      return p.top2 && b > lowest<K>() ? fmax(a + b, -__DBL_MAX__) : a;
     };
     const int span = route_span(p.e, p.groups, per);
     const bool whole = span != 0;

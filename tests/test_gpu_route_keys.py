@@ -132,3 +132,23 @@ def test_groups_of_nearly_equal_keys(score):
                     else torch.softmax(x[r].double(), 0)
                 want = sorted(inside, key=lambda i: (-(s[i].item() + key[i][0]), i))[:2]
                 assert ids[r].tolist() == want
+
+
+@pytest.mark.parametrize("dtype", [F32, F64])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_sums_of_the_lowest_biases_stay_above_masked_groups(dtype, score):
+    low = torch.finfo(dtype).min
+    inf = float("inf")
+    x = torch.tensor([[-inf, -inf, 0.1, 0.2, 0.3, -inf], [0.5, 0.4, -inf, -inf, -inf, 0.3],
+                      [-inf, -inf, -inf, -inf, 0.0, 1.0]], device="cuda", dtype=dtype)
+    bias = torch.full((6,), 0.75 * low, device="cuda", dtype=dtype)
+    for top, want in ((1, [[4], [5], [4]]), (2, [[2, 3], [0, 1], [4, 5]])):
+        # a group of one bias ranks above a group of two, both above the masked
+        ids = ops.topk_route(x, len(want[0]), score=score, bias=bias, num_groups=3,
+                             topk_groups=top, group_score="top2")[1]
+        got = ids.tolist()
+        if top == 1:
+            assert got == want
+        else:
+            live = [sorted(i for i in r if x[n, i] > -inf) for n, r in enumerate(got)]
+            assert all(len(r) == 2 for r in live), got
