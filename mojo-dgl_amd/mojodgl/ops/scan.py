@@ -210,7 +210,8 @@ def segment_scan_step(gate, value, state, out=None):
     gate, value : (S, ...) one row a sequence, types as in `segment_scan`
     state : (S, ...) the sequences' states, float32 (float64 for float64 values)
     out : tensor of the new states (a contiguous GPU tensor like the result's);
-        it may be ``state`` itself, which is then updated in place
+        it may be ``state`` itself, which is then updated in place (autograd counts
+        it as torch's in-place operations)
 
     Returns
     -------
@@ -247,6 +248,9 @@ def segment_scan_step(gate, value, state, out=None):
     _lib.check(_lib.lib().mdgl_segment_scan_step(
         g.data_ptr(), v.data_ptr(), s.data_ptr(), h.data_ptr(), new.data_ptr(), v.numel(),
         _lib.ROW_CODES[vt], _lib.ROW_CODES[gt], _lib.stream()), "segment_scan_step")
+    if out is not None:
+        # a backward pass that saved what was written over now raises
+        torch.autograd.graph.increment_version(out)
     return _lib.hand_back(h, where), new if out is not None else _lib.hand_back(new, where)
 
 
