@@ -616,7 +616,8 @@ int mdgl_segment_marks(const int32_t* offsets, int64_t num_seg, int64_t n, int32
  * (has_empty: whether there are any). marks (state, [ceil(n / 16)][d], nullable)
  * is what mdgl_segment_scan_grad needs of the forward pass. ids, starts, ends:
  * mdgl_segment_marks. Products of neighbouring rows' gates within a segment are
- * formed: they must not overflow the state's type (gates in [-1, 1] never do). */
+ * formed: they must not overflow the state's type (gates in [-1, 1] never do), and
+ * where one underflows to 0 an infinite state in front of it gives NaN. */
 int mdgl_segment_scan(const void* gate, const void* value, const void* initial,
                       const int32_t* offsets, const int32_t* ids, const uint64_t* starts,
                       const uint64_t* ends, void* dst, void* last, void* marks, int64_t num_seg,

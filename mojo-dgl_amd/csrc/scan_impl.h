@@ -13,6 +13,9 @@
 // chunks of equal size whatever the lengths: bit r of `starts` / `ends` says that
 // row r is the first / last of its segment, and a walk replaces its state there
 // (nothing is multiplied by zero, so an infinity or a NaN stays in its segment).
+// Within it an infinite state times a product of gates that underflowed to 0 is a NaN.
+// Telling that product from one with a gate of 0, where a NaN is right, took 5 to 10 %
+// of every scan's time, and 30 % of a long one with gates of 0.
 //
 // scan_pass_kernel reads each row once. A workgroup holds its chunk's rows in
 // registers, 16 rows of two columns a thread, composes their maps (in the thread,

@@ -99,9 +99,10 @@ def segment_scan(seglen, gate, value, initial=None, return_state=False):
     ``h`` in the type of ``value``, and with ``return_state`` the states,
     (len(seglen), ...) in float32 (float64 for float64 values), which the next
     call takes as ``initial``. With torch tensors that require grad the results
-    take part in autograd. Products of the gates of a segment's
-    neighbouring rows are formed: they must not overflow (gates in [-1, 1] never
-    do).
+    take part in autograd. Products of the gates of a segment's neighbouring rows
+    are formed: they must not overflow (gates in [-1, 1] never do), and where one is
+    too small for the type an infinite state in front of it gives NaN, as behind a
+    gate of 0.
 
     Examples
     --------

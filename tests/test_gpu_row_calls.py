@@ -1,5 +1,7 @@
-"""Calls of the row operators beside others: what autograd saved and is written over."""
+"""Calls of the row operators beside others: what autograd saved and is written over,
+states that are infinite."""
 
+import numpy as np
 import pytest
 import torch
 
@@ -29,3 +31,55 @@ def test_a_step_into_a_saved_state_is_seen_by_the_backward_pass():
     with torch.inference_mode():  # tensors without versions
         mine = torch.rand(2, 4, device="cuda")
         ops.segment_scan_step(mine, mine, mine.clone(), out=torch.empty_like(mine))
+
+
+def walk(lens, a, v, init, dh, dl):
+    """The recurrence and its gradients row by row in float64."""
+    h, da, dv, di = np.empty_like(v), np.empty_like(v), np.empty_like(v), np.empty_like(init)
+    at = 0
+    with np.errstate(invalid="ignore"):
+        for s, m in enumerate(lens):
+            before, cur = [], init[s]
+            for t in range(at, at + m):
+                before.append(cur)
+                h[t] = cur = a[t] * cur + v[t]
+            back = dl[s]
+            for t in range(at + m - 1, at - 1, -1):
+                dv[t] = dh[t] + back
+                da[t] = dv[t] * before[t - at]
+                back = a[t] * dv[t]
+            di[s] = back
+            at += m
+    return h, da, dv, di
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,d", [([700, 0, 60], 20), ([9000, 1200], 3), ([3000], 140),
+                                    ([15, 129, 17, 1300], 64)])
+def test_infinite_states_stay_to_be_seen(lens, d, dtype):
+    """Results are finite exactly where the recurrence's are, whatever lies between an
+    infinite state and them: gates whose product is too small for the type (which makes
+    it a NaN at the latest), or a gate of 0."""
+    g = torch.Generator(device="cuda").manual_seed(d)
+    n, s = sum(lens), len(lens)
+    st = torch.float64 if dtype == torch.float64 else torch.float32
+
+    def rand(*shape, dtype=dtype):
+        return torch.randn(*shape, generator=g, device="cuda", dtype=torch.float64).to(dtype)
+
+    a = rand(n, d)
+    a = torch.where(a < 0, -1.0, 1.0).to(dtype) * (0.02 + 0.1 * rand(n, d).abs())
+    v, dh = rand(n, d), rand(n, d)
+    init, dl = rand(s, d, dtype=st), rand(s, d, dtype=st)
+    inf = float("inf")
+    a[n // 2, 2] = a[n // 3, 0] = 0.0
+    init[0, 0], init[-1, 1], dl[0, 1], dl[-1, 2] = inf, -inf, -inf, inf
+    v[n // 4, d - 1], dh[n // 3, d - 1] = inf, -inf
+    if d > 3:
+        v[1, 5], v[n - 2, 5], dh[n - 1, 6], init[0, 7], a[n // 2, 7] = inf, -inf, inf, inf, -0.0
+    A, V, I = (t.clone().requires_grad_() for t in (a, v, init))  # noqa: E741
+    h, last = ops.segment_scan(lens, A, V, I, return_state=True)
+    got = [h.detach()] + list(torch.autograd.grad((h, last), (A, V, I), (dh, dl)))
+    want = walk(lens, *(t.double().cpu().numpy() for t in (a, v, init, dh, dl)))
+    for name, x, w in zip(("h", "dgate", "dvalue", "dinitial"), got, want):
+        assert (np.isfinite(x.double().cpu().numpy()) == np.isfinite(w)).all(), name
