@@ -49,7 +49,8 @@ these follow the calculus of the forward ops and run on the same kernels:
   ``mdgl_combine_rows_grad``.
 
 The backward passes run on the library's kernels, outside torch's graph, so
-they are differentiable once: a second derivative through them raises.
+they are differentiable once: a second derivative through them raises. So does
+an operand with a tangent (`torch.autograd.forward_ad`).
 
 Gradients come back in the operand's shape: an operand broadcast along its
 trailing feature axes gets its gradient summed over them (a segmented sum,
@@ -63,6 +64,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -74,6 +76,13 @@ __all__ = ["needs_grad", "GSpMM", "GSDDMM", "EdgeSoftmax", "SegmentReduce", "Seg
 
 
 def needs_grad(*xs) -> bool:
+    """Whether a call of these operands takes part in autograd. Tangents (forward
+    mode), which the kernels do not carry, are refused rather than dropped."""
+    if forward_ad._current_level >= 0:
+        for x in xs:
+            if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+                raise DGLError("forward-mode derivatives are not supported: an operand has a "
+                               "tangent")
     if torch.is_grad_enabled():
         for x in xs:
             if isinstance(x, torch.Tensor) and x.requires_grad:
