@@ -297,8 +297,12 @@ __global__ void __launch_bounds__(norm_block<G>()) norm_grad_kernel(NormArgs<T, 
   }
 #pragma unroll
   for (int j = 0; j < K; ++j) {
-    if (!live[j]) continue;
-    const int64_t at = (int64_t)blockIdx.x * p.d + col[j];
+    // formed again: held until here they put two of 1,024 threads' registers in memory
+    // (double)
+    int64_t c;
+    int shared;
+    if (!norm_cols<V>(t + j * G, p.d, &c, &shared)) continue;
+    const int64_t at = (int64_t)blockIdx.x * p.d + c;
     if (p.part_w) store_acc<A, A, V>(p.part_w + at, dw[j]);
     if (p.part_b) store_acc<A, A, V>(p.part_b + at, db[j]);
   }
