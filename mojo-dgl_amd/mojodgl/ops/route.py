@@ -7,7 +7,8 @@ row, and puts the rows in that order.
     y = combine_rows(segment_mm(dispatch_rows(x, plan), w, plan.seglen), weights, plan)
 
 Rows keep float32, float64, bfloat16 or float16; weights and sums are float32
-(float64 for float64 rows).
+(float64 for float64 rows). segment_mm takes 16-bit rows as float32 and returns
+float32: `.to(x.dtype)` behind it keeps such a layer's rows in their type.
 """
 
 from __future__ import annotations

@@ -1,5 +1,5 @@
 """Calls of the row operators beside others: what autograd saved and is written over,
-states that are infinite."""
+states that are infinite, 16-bit layers."""
 
 import numpy as np
 import pytest
@@ -83,3 +83,72 @@ def test_infinite_states_stay_to_be_seen(lens, d, dtype):
     want = walk(lens, *(t.double().cpu().numpy() for t in (a, v, init, dh, dl)))
     for name, x, w in zip(("h", "dgate", "dvalue", "dinitial"), got, want):
         assert (np.isfinite(x.double().cpu().numpy()) == np.isfinite(w)).all(), name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,d,experts,k", [(37, 24, 5, 2), (150, 72, 16, 4), (3, 130, 8, 1)])
+def test_a_layer_of_16_bit_rows(dtype, n, d, experts, k):
+    """Routing, the experts' products cast back to the rows' type, and the way there and
+    back: h is the half step of the rows' type, taken once for each rounding to it;
+    sums of up to N terms in float32 take N + 64 of its half steps."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    h, u = torch.finfo(dtype).eps / 2, 2.0 ** -24
+
+    def rand(*shape, dtype=dtype):
+        return torch.randn(*shape, generator=g, device="cuda", dtype=torch.float64).to(dtype)
+
+    x, w, dy = rand(n, d), (rand(experts, d, d).double() * d ** -0.5).to(dtype), rand(n, d)
+    logits = rand(n, experts, dtype=torch.float32)
+    X, W, L = (t.clone().requires_grad_() for t in (x, w, logits))
+    weights, ids = ops.topk_route(L, k)
+    plan = ops.route_plan(ids, experts)
+    ys = ops.segment_mm(ops.dispatch_rows(X, plan), W, plan.seglen)
+    assert ys.dtype == torch.float32
+    y = ops.combine_rows(ys.to(X.dtype), weights, plan)
+    assert y.dtype == dtype
+    dx, dw, dl = torch.autograd.grad(y, (X, W, L), dy)
+    assert (dx.dtype, dw.dtype, dl.dtype) == (dtype, dtype, torch.float32)
+
+    x, w, dy = x.double(), w.double(), dy.double()
+    p = torch.softmax(logits.double().gather(1, ids), 1)     # (n, k)
+    e_p = 60 * u * p
+    we = w[ids]                                              # (n, k, d, d)
+    rows = (x[:, None, None, :] @ we)[:, :, 0]               # (n, k, d)
+    size = (x.abs()[:, None, None, :] @ we.abs())[:, :, 0]
+    e_rows = h * rows.abs() + (1 + h) * (d + 64) * u * size
+    want = (p[:, :, None] * rows).sum(1)
+    bound = (p[:, :, None] * e_rows + (e_p + k * u * p)[:, :, None] * (rows.abs() + e_rows)).sum(1)
+
+    def check(got, want, bound, last, name):
+        off = (got.double() - want).abs()
+        limit = bound * (1 + last) + last * want.abs() + torch.finfo(got.dtype).tiny
+        assert bool((off <= limit).all()), (name, float((off / limit).max()))
+
+    check(y.detach(), want, bound, h, "y")
+    back = p[:, :, None] * dy[:, None, :]                    # gradient of the rows
+    e_back = h * back.abs() + (1 + h) * (e_p + 2 * u * p)[:, :, None] * dy.abs()[:, None, :]
+    through = (back[:, :, None, :] @ we.transpose(2, 3).contiguous())[:, :, 0]
+    wide = ((back.abs() + e_back)[:, :, None, :] @ we.abs().transpose(2, 3).contiguous())[:, :, 0]
+    e_through = (e_back[:, :, None, :] @ we.abs().transpose(2, 3).contiguous())[:, :, 0] \
+        + (d + 64) * u * wide
+    e_through = h * through.abs() + (1 + h) * e_through      # the product's gradient in x's type
+    check(dx, through.sum(1), e_through.sum(1) + k * u * (through.abs() + e_through).sum(1), h,
+          "dx")
+    outer = torch.zeros_like(w)
+    e_outer = torch.zeros_like(w)
+    for e in range(experts):
+        at = (ids == e).nonzero()
+        a, b, eb = x[at[:, 0]], back[at[:, 0], at[:, 1]], e_back[at[:, 0], at[:, 1]]
+        outer[e] = a.t().contiguous() @ b
+        e_outer[e] = a.t().abs().contiguous() @ (eb + (n + 64) * u * (b.abs() + eb))
+    check(dw, outer, e_outer, h, "dw")
+    dots = (rows * dy[:, None, :]).sum(2)
+    e_dots = ((e_rows + (d + 64) * u * (rows.abs() + e_rows)) * dy.abs()[:, None, :]).sum(2)
+    inner = (p * dots).sum(1, keepdim=True)
+    dlog = torch.zeros(n, experts, dtype=torch.float64, device="cuda").scatter(
+        1, ids, p * (dots - inner))
+    e_inner = (p * e_dots + (e_p + (k + 8) * u * p) * (dots.abs() + e_dots)).sum(1, keepdim=True)
+    size = dots.abs() + e_dots + inner.abs() + e_inner
+    e_log = torch.zeros_like(dlog).scatter(
+        1, ids, p * (e_dots + e_inner) + (e_p + 4 * u * p) * size)
+    check(dl, dlog, e_log, u, "dlogits")
