@@ -183,7 +183,8 @@ __device__ __forceinline__ Choice<float> route_choose_float(const RouteArgs<T>& 
   c.id = 0;
   c.key = lowest<float>();
   // without a bias, the marks of groups by two experts need scores that no key has
-  const bool marks = p.groups > 1 && p.top2 && !p.bias, sums = !p.sigmoid && (p.bias || !p.renorm);
+  const bool marks = p.groups > 1 && p.top2 && !p.bias;
+  const bool sums = !p.sigmoid && (p.bias || !p.renorm);
   if (sums || marks) {
 #pragma unroll
     for (int i = 0; i < R; ++i) c.top = v[i] > c.top ? v[i] : c.top;
@@ -418,7 +419,8 @@ __device__ __forceinline__ Choice<K> route_choose(const RouteArgs<T>& p, const T
   c.limit = K(0);
   c.id = 0;
   c.key = lowest<K>();
-  const bool marks = p.groups > 1 && p.top2 && !p.bias, sums = !p.sigmoid && (p.bias || !p.renorm);
+  const bool marks = p.groups > 1 && p.top2 && !p.bias;
+  const bool sums = !p.sigmoid && (p.bias || !p.renorm);
   if (sums || marks) {
 #pragma unroll
     for (int i = 0; i < R; ++i) c.top = key[i] > c.top ? key[i] : c.top;
@@ -608,7 +610,7 @@ __global__ void __launch_bounds__(BLOCK) route_kernel(RouteArgs<T> p) {
 }
 
 // dlogits of a row, formed in LDS: zeros (or, where every score counts, the
-// softmax's share) with the choices' terms added, then written as vectors.
+// softmax's share) with the choices' terms added, then written, a value a lane.
 template <class T, int G>
 __global__ void __launch_bounds__(BLOCK) route_grad_kernel(RouteArgs<T> p) {
   using A = acc_t<T>;

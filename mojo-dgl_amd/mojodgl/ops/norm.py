@@ -108,6 +108,7 @@ def _layer_norm_grad(value, weight, bias, stats, grad, need):
         nbytes = L.mdgl_layer_norm_grad_workspace_bytes(n, d, code)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
     _lib.check(L.mdgl_layer_norm_grad(
-        x.data_ptr(), _lib.ptr(w), *_stats_ptrs(stats), g.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), n, d, _lib.ptr(ws), nbytes, code, _lib.ROW_CODES[wt],
-        _lib.stream()), "layer_norm_grad")
+        x.data_ptr(), _lib.ptr(w), *_stats_ptrs(stats), g.data_ptr(), _lib.ptr(dx), _lib.ptr(dw),
+        _lib.ptr(db), n, d, _lib.ptr(ws), nbytes, code, _lib.ROW_CODES[wt], _lib.stream()),
+        "layer_norm_grad")
     return dx, dw, db

@@ -50,8 +50,9 @@ def topk_route(logits, k, score="softmax", bias=None, num_groups=1, topk_groups=
     ``(weights, ids)``, both (N, k), best first, the lowest index among equals;
     ids are int64. Scores that differ by less than float32 shows are compared in
     float64. An expert masked by -inf is chosen only when nothing else is left and
-    weighs 0; a NaN ranks with the masked and makes the weights it enters NaN. With torch logits that require grad the weights take part in
-    autograd; `bias` gets no gradient.
+    weighs 0; a NaN ranks with the masked and makes the weights it enters NaN. With
+    torch logits that require grad the weights take part in autograd; `bias` gets no
+    gradient.
     """
     if _autograd.needs_grad(logits):
         return _autograd.TopkRoute.apply(logits, k, score, bias, num_groups, topk_groups,
