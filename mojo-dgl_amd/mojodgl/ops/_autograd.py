@@ -60,6 +60,7 @@ Only torch tensors take part (numpy operands have no autograd).
 
 from __future__ import annotations
 
+import functools
 import math
 
 import numpy as np
@@ -667,6 +668,30 @@ def _saved_some(ctx):
     return tuple(h if t is None else t for t, h in zip(ctx.saved_tensors, ctx.host))
 
 
+def _made_here(ctx, where):
+    """Keep what the backward pass needs to run on this GPU, where the forward pass has
+    its plan and statistics: autograd runs it on the results' device `where`."""
+    ctx.gpu, ctx.queue = _lib.current_device(), None
+    if where is not None and where.type == "cuda" and where.index != ctx.gpu:
+        ctx.queue = torch.cuda.current_stream()
+
+
+def _where_made(backward):
+    """`backward` on the GPU of the forward pass, and on its stream where autograd does
+    not see to that."""
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        if ctx.queue is not None:
+            with torch.cuda.stream(ctx.queue):
+                return backward(ctx, *grads)
+        if ctx.gpu != _lib.current_device():
+            with torch.cuda.device(ctx.gpu):
+                return backward(ctx, *grads)
+        return backward(ctx, *grads)
+
+    return run
+
+
 class SegmentScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, seglen, gate, value, initial, return_state):
@@ -678,10 +703,12 @@ class SegmentScan(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         _save_some(ctx, gate, value, initial)
         where = _lib.caller_device(value, gate, initial)
+        _made_here(ctx, where)
         return _lib.hand_back(h, where), _lib.hand_back(last, where) if return_state else None
 
     @staticmethod
     @once_differentiable
+    @_where_made
     def backward(ctx, grad, grad_last):
         from .scan import _scan_grad
 
@@ -700,10 +727,13 @@ class LayerNorm(torch.autograd.Function):
 
         y, ctx.stats = _layer_norm(value, weight, bias, eps, True)
         _save_some(ctx, value, weight, bias)
-        return _lib.hand_back(y, _lib.caller_device(value, weight, bias))
+        where = _lib.caller_device(value, weight, bias)
+        _made_here(ctx, where)
+        return _lib.hand_back(y, where)
 
     @staticmethod
     @once_differentiable
+    @_where_made
     def backward(ctx, grad):
         from .norm import _layer_norm_grad
 
@@ -722,6 +752,7 @@ class TopkRoute(torch.autograd.Function):
         w, ids = _topk_route(logits, k, score, bias, num_groups, topk_groups, group_score,
                              renormalize, scale)
         ctx.how = score, renormalize, scale
+        _made_here(ctx, logits.device)
         w, ids = _lib.hand_back(w, logits.device), _lib.hand_back(ids, logits.device)
         ctx.save_for_backward(logits, ids)
         ctx.mark_non_differentiable(ids)
@@ -729,6 +760,7 @@ class TopkRoute(torch.autograd.Function):
 
     @staticmethod
     @once_differentiable
+    @_where_made
     def backward(ctx, grad, _):
         from .route import _topk_route_grad
 
@@ -743,10 +775,13 @@ class DispatchRows(torch.autograd.Function):
 
         ctx.plan = plan
         ctx.like = torch.empty(0, dtype=value.dtype, device=value.device)
-        return _lib.hand_back(_dispatch_rows(value, plan), value.device)
+        xs = _dispatch_rows(value, plan)
+        _made_here(ctx, value.device)
+        return _lib.hand_back(xs, value.device)
 
     @staticmethod
     @once_differentiable
+    @_where_made
     def backward(ctx, grad):
         from .route import _sum_rows
 
@@ -760,11 +795,13 @@ class CombineRows(torch.autograd.Function):
 
         ctx.plan = plan
         _save_some(ctx, value, weights)
-        return _lib.hand_back(_combine_rows(value, weights, plan),
-                              _lib.caller_device(value, weights))
+        y, where = _combine_rows(value, weights, plan), _lib.caller_device(value, weights)
+        _made_here(ctx, where)
+        return _lib.hand_back(y, where)
 
     @staticmethod
     @once_differentiable
+    @_where_made
     def backward(ctx, grad):
         from .route import _combine_rows_grad
 

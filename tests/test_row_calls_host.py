@@ -1,11 +1,16 @@
-"""Calls that are refused before any GPU work."""
+"""Calls of the row operators without a GPU: refusals before any GPU work, and where a
+backward pass runs."""
+
+import contextlib
+from types import SimpleNamespace
 
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 import mojodgl.ops as ops
-from mojodgl import DGLError
+from mojodgl import DGLError, _lib
+from mojodgl.ops import _autograd
 
 
 def test_tangents_are_refused():
@@ -27,3 +32,39 @@ def test_tangents_are_refused():
                 call()
     with pytest.raises(DGLError, match="tangent"):
         torch.func.jvp(ops.layer_norm, (torch.ones(4, 3),), (torch.ones(4, 3),))
+
+
+def test_a_backward_pass_runs_where_its_forward_pass_ran(monkeypatch):
+    """Autograd runs it on the results' GPU, which is the operands' and need not be the one
+    that was current: the plan and the statistics lie there, and the kernels belong on
+    that GPU's stream."""
+    entered = []
+
+    def note(kind):
+        @contextlib.contextmanager
+        def enter(what):
+            entered.append((kind, what))
+            yield
+            entered.append((kind, None))
+        return enter
+
+    monkeypatch.setattr(torch.cuda, "device", note("device"))
+    monkeypatch.setattr(torch.cuda, "stream", note("stream"))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: "queue 0")
+    now = SimpleNamespace(gpu=0)
+    monkeypatch.setattr(_lib, "current_device", lambda: now.gpu)
+    run = _autograd._where_made(lambda ctx, a, b: entered.append((a, b)) or "grads")
+    for where, later, want in ((torch.device("cuda", 0), 0, []),
+                               (torch.device("cpu"), 0, []), (None, 0, []),
+                               (torch.device("cpu"), 1, [("device", 0)]),
+                               (torch.device("cuda", 1), 1, [("stream", "queue 0")])):
+        ctx, now.gpu = SimpleNamespace(), 0
+        _autograd._made_here(ctx, where)
+        now.gpu = later
+        assert run(ctx, 1, 2) == "grads"
+        assert entered == want + [(1, 2)] + [(kind, None) for kind, _ in want]
+        entered.clear()
+    for name in ("SegmentScan", "LayerNorm", "TopkRoute", "DispatchRows", "CombineRows"):
+        # once_differentiable around it, around the pass itself
+        backward = getattr(_autograd, name).backward
+        assert backward.__wrapped__.__code__ is run.__code__, name
