@@ -699,9 +699,9 @@ class SegmentScan(torch.autograd.Function):
 
         # the states in front of every 16th row serve the gates' gradient
         h, last, marks, plan = _scan(seglen, gate, value, initial, return_state, True)
-        ctx.plan, ctx.marks = plan, marks
+        ctx.plan = plan
         ctx.set_materialize_grads(False)
-        _save_some(ctx, gate, value, initial)
+        _save_some(ctx, gate, value, initial, marks)
         where = _lib.caller_device(value, gate, initial)
         _made_here(ctx, where)
         return _lib.hand_back(h, where), _lib.hand_back(last, where) if return_state else None
@@ -712,10 +712,10 @@ class SegmentScan(torch.autograd.Function):
     def backward(ctx, grad, grad_last):
         from .scan import _scan_grad
 
-        gate, value, initial = _saved_some(ctx)
+        gate, value, initial, marks = _saved_some(ctx)
         if grad is None and grad_last is None:
             return None, None, None, None, None
-        dg, dv, di = _scan_grad(ctx.plan, gate, value, initial, ctx.marks, grad, grad_last,
+        dg, dv, di = _scan_grad(ctx.plan, gate, value, initial, marks, grad, grad_last,
                                 ctx.needs_input_grad[1:4])
         return None, _back(dg, gate), _back(dv, value), _back(di, initial), None
 
@@ -725,8 +725,8 @@ class LayerNorm(torch.autograd.Function):
     def forward(ctx, value, weight, bias, eps):
         from .norm import _layer_norm
 
-        y, ctx.stats = _layer_norm(value, weight, bias, eps, True)
-        _save_some(ctx, value, weight, bias)
+        y, stats = _layer_norm(value, weight, bias, eps, True)
+        _save_some(ctx, value, weight, bias, stats)
         where = _lib.caller_device(value, weight, bias)
         _made_here(ctx, where)
         return _lib.hand_back(y, where)
@@ -737,8 +737,8 @@ class LayerNorm(torch.autograd.Function):
     def backward(ctx, grad):
         from .norm import _layer_norm_grad
 
-        value, weight, bias = _saved_some(ctx)
-        dx, dw, db = _layer_norm_grad(value, weight, bias, ctx.stats, grad,
+        value, weight, bias, stats = _saved_some(ctx)
+        dx, dw, db = _layer_norm_grad(value, weight, bias, stats, grad,
                                       ctx.needs_input_grad[:3])
         return _back(dx, value), _back(dw, weight), _back(db, bias), None
 

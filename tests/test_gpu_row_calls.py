@@ -1,5 +1,5 @@
 """Calls of the row operators beside others: what autograd saved and is written over,
-states that are infinite, 16-bit layers."""
+states that are infinite, 16-bit layers, memory after a backward pass."""
 
 import numpy as np
 import pytest
@@ -152,3 +152,25 @@ def test_a_layer_of_16_bit_rows(dtype, n, d, experts, k):
     e_log = torch.zeros_like(dlog).scatter(
         1, ids, p * (e_dots + e_inner) + (e_p + 4 * u * p) * size)
     check(dl, dlog, e_log, u, "dlogits")
+
+
+def test_a_backward_pass_lets_go_of_what_was_kept_for_it():
+    """The scan's marks and layer norm's statistics go with the saved operands, while
+    the results (a loss that is looked at later) live on."""
+    n, d = 4096, 512
+    x = torch.rand(n, d, device="cuda", requires_grad=True)
+    y = torch.rand(n, d, device="cuda")
+    plan = ops.segment_plan([n])
+    for call, kept in ((lambda: ops.segment_scan(plan, x, y).sum(), n * d // 16 * 4),
+                       (lambda: ops.layer_norm(x).sum(), 2 * n * 4)):
+        for _ in range(2):
+            loss = call()
+            torch.autograd.grad(loss, x)
+            del loss
+        before = torch.cuda.memory_allocated()
+        loss = call()
+        held = torch.cuda.memory_allocated() - before
+        torch.autograd.grad(loss, x)
+        assert held >= kept and torch.cuda.memory_allocated() - before <= 1024
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(loss, x)
