@@ -87,8 +87,9 @@ def _topk_route(logits, k, score, bias, num_groups, topk_groups, group_score, re
     b = None if b is None else _lib.rows_on_device(b, st)
     k, num_groups = int(k), int(num_groups)
     topk_groups = num_groups if topk_groups is None else int(topk_groups)
-    w = torch.empty(n, max(k, 0), dtype=st, device=dev)
-    ids = torch.empty(n, max(k, 0), dtype=torch.int64, device=dev)
+    cols = min(max(k, 0), e)  # other k are refused below
+    w = torch.empty(n, cols, dtype=st, device=dev)
+    ids = torch.empty(n, cols, dtype=torch.int64, device=dev)
     _lib.check(_lib.lib().mdgl_topk_route(
         x.data_ptr(), _lib.ptr(b), w.data_ptr(), ids.data_ptr(), n, e, k, _SCORES[score],
         num_groups, topk_groups, _GROUP_SCORES[group_score], bool(renormalize), scale,
@@ -138,13 +139,16 @@ class RoutePlan:
         m = flat.numel()
         dev = flat.device
         nbytes = L.mdgl_route_plan_workspace_bytes(m, num_experts)
+        if nbytes < 0:  # refused before anything of that size is allocated
+            _lib.check(L.mdgl_route_plan(None, m, num_experts, None, None, None, None, 0,
+                                         _lib.stream()), "route_plan")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
-        self.seglen = torch.empty(max(num_experts, 0), dtype=torch.int64, device=dev)
+        self.seglen = torch.empty(num_experts, dtype=torch.int64, device=dev)
         self.order = torch.empty(m, dtype=torch.int32, device=dev)
         self.slot = torch.empty(self.num_rows, self.k, dtype=torch.int32, device=dev)
         _lib.check(L.mdgl_route_plan(
             flat.data_ptr(), m, num_experts, self.seglen.data_ptr(), self.order.data_ptr(),
-            self.slot.data_ptr(), _lib.ptr(ws), max(nbytes, 0), _lib.stream()), "route_plan")
+            self.slot.data_ptr(), _lib.ptr(ws), nbytes, _lib.stream()), "route_plan")
 
 
 def route_plan(ids, num_experts) -> RoutePlan:

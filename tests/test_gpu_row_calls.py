@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import mojodgl.ops as ops
+from mojodgl import DGLError
 
 pytestmark = pytest.mark.gpu
 
@@ -174,3 +175,14 @@ def test_a_backward_pass_lets_go_of_what_was_kept_for_it():
         assert held >= kept and torch.cuda.memory_allocated() - before <= 1024
         with pytest.raises(RuntimeError, match="second time"):
             torch.autograd.grad(loss, x)
+
+
+def test_sizes_out_of_range_are_refused_before_they_are_allocated():
+    x = torch.zeros(8, 16, device="cuda")
+    for k in (17, 2 ** 40, 0, -3):
+        with pytest.raises(DGLError, match="experts a row"):
+            ops.topk_route(x, k)
+    ids = torch.zeros(8, 2, dtype=torch.int64, device="cuda")
+    for experts in (2 ** 45, 2049, 0, -1):
+        with pytest.raises(DGLError, match="2048 experts"):
+            ops.route_plan(ids, experts)
