@@ -1617,7 +1617,7 @@ int mdgl_segment_scan(const void* gate, const void* value, const void* initial,
   MDGL_RANGE();
   int rc = scan_sizes("segment_scan", num_seg, n, d, dtype, gate_dtype);
   if (rc) return rc;
-  if (d == 0 || (n == 0 && !(has_empty && last))) return MDGL_OK;
+  if (d == 0 || (n == 0 && !(has_empty && last && num_seg > 0))) return MDGL_OK;
   if (n > 0 && (!gate || !value || !ids || !starts || !ends || !dst))
     return fail(MDGL_EINVAL, "segment_scan: null buffer");
   if (has_empty && last && !offsets) return fail(MDGL_EINVAL, "segment_scan: null buffer");
@@ -1654,7 +1654,7 @@ int mdgl_segment_scan_grad(const void* gate, const void* value, const void* init
   MDGL_RANGE();
   int rc = scan_sizes("segment_scan_grad", num_seg, n, d, dtype, gate_dtype);
   if (rc) return rc;
-  if (d == 0 || (n == 0 && !(has_empty && dinitial))) return MDGL_OK;
+  if (d == 0 || (n == 0 && !(has_empty && dinitial && num_seg > 0))) return MDGL_OK;
   if (n > 0 && (!gate || !grad || !ids || !starts || !ends || (dgate && (!value || !marks))))
     return fail(MDGL_EINVAL, "segment_scan_grad: null buffer");
   if (has_empty && dinitial && !offsets)

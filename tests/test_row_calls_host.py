@@ -68,3 +68,12 @@ def test_a_backward_pass_runs_where_its_forward_pass_ran(monkeypatch):
         # once_differentiable around it, around the pass itself
         backward = getattr(_autograd, name).backward
         assert backward.__wrapped__.__code__ is run.__code__, name
+
+
+def test_no_segments_at_all_is_nothing_to_do():
+    """`has_empty` without a segment launches nothing."""
+    lib, p = _lib.lib(), 4096  # an aligned address that is not read
+    assert lib.mdgl_segment_scan(p, p, None, p, p, p, p, p, p, None, 0, 0, 16, 1, None, 0, 0, 0,
+                                 None) == 0
+    assert lib.mdgl_segment_scan_grad(p, p, None, p, p, None, p, p, p, p, p, p, p, 0, 0, 16, 1,
+                                      None, 0, 0, 0, None) == 0
