@@ -28,8 +28,8 @@
 // 256 with a bias: 43 us, 46 without that, and with it 53 instead of 50 for sigmoid).
 //
 // 65,536 rows of 256 float32 logits in 8 groups, 8 of 4 groups chosen, with a bias:
-// 54 us, and 18 us for the gradient, where reading and writing take 14 and 14. The
-// choice is bound by its instructions: 1,460 of the vector unit's a wavefront of four
+// 56 us, and 18 us for the gradient, where reading and writing take 14 and 14. The
+// choice is bound by its instructions: 1,520 of the vector unit's a wavefront of four
 // rows, half of them the nine rounds (98 us with compares and selects on floats
 // instead of integer maxima, a second search in double of whole wavefronts, exact
 // exponentials for the keys). 16 lanes a row: with 64 a round's two reductions over

@@ -20,7 +20,8 @@
 // scan_pass_kernel reads each row once. A workgroup holds its chunk's rows in
 // registers, 16 rows of two columns a thread, composes their maps (in the thread,
 // then over the threads of a column in LDS), publishes the chunk's map, and looks
-// back along the chunks in front of it for the state it starts from. With that state
+// back along the chunks in front of it for the state it starts from (a scan by
+// decoupled look-back; by groups of chunks, look_back() says why). With that state
 // it goes over its registers again and writes. The one other launch resets what
 // chunks publish; a single chunk needs neither.
 //
@@ -249,6 +250,9 @@ __device__ __forceinline__ void look_back(A* words, int64_t chunks, int64_t d, i
 // a register: the gradient's 260 us became 195 us. 512 threads: 256 make the chain
 // twice as long (the one sequence 190 us). Groups of 4 chunks: 8 take 146 us for it,
 // 16 163 us, and no groups, with the state handed from chunk to chunk, 217 us.
+// The gradient of 16-bit rows keeps to 128 registers, two workgroups on a compute
+// unit; that of float rows takes 148, so there one waits alone (150,001 float rows of
+// 100 in 5,000 segments: 96 us, 310 MB, 3.2 TB/s).
 constexpr int PASS_BLOCK = 512;
 
 template <class T, class G, int V, bool BACK>
