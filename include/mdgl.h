@@ -637,7 +637,7 @@ int mdgl_segment_scan_grad(const void* gate, const void* value, const void* init
                            void* stream);
 
 /* One row of every sequence: next = gate * state + value (state), dst = next in
- * the values' dtype, for `count` values. `next` may be `state`. */
+ * the values' dtype, for `count` values (fewer than 2**32). `next` may be `state`. */
 int mdgl_segment_scan_step(const void* gate, const void* value, const void* state, void* dst,
                            void* next, int64_t count, int dtype, int gate_dtype, void* stream);
 

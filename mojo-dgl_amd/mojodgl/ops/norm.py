@@ -25,7 +25,8 @@ def layer_norm(value, weight=None, bias=None, eps=1e-5):
     value : (..., D) array or tensor; float32, float64, float16 and bfloat16
         keep their type, with the sums in float32 (float64 for float64)
     weight, bias : (D,) arrays or tensors, or None for 1 and 0; in the type of
-        ``value`` or, beside 16-bit values, in float32
+        ``value`` or, beside 16-bit values, in float32 (float64 ones make the rows
+        float64, too)
     eps : added to the variance, >= 0
 
     Returns

@@ -96,8 +96,9 @@ def segment_scan(seglen, gate, value, initial=None, return_state=False):
 
     Returns
     -------
-    ``h`` in the type of ``value``, and with ``return_state`` the states,
-    (len(seglen), ...) in float32 (float64 for float64 values), which the next
+    ``h`` in the type of ``value`` (float64 beside a float64 gate), and with
+    ``return_state`` the states, (len(seglen), ...) in float32 (float64 for float64
+    ``h``), which the next
     call takes as ``initial``. With torch tensors that require grad the results
     take part in autograd. Products of the gates of a segment's neighbouring rows
     are formed: they must not overflow (gates in [-1, 1] never do), and where one is
@@ -216,8 +217,8 @@ def segment_scan_step(gate, value, state, out=None):
 
     Returns
     -------
-    ``(h, new_state)``: h in the type of ``value``. It has no gradient
-    (`segment_scan` has).
+    ``(h, new_state)``: h in the type of ``value`` (float64 beside a float64 gate).
+    It has no gradient (`segment_scan` has). One call takes fewer than 2**32 values.
     """
     if _autograd.needs_grad(gate, value, state):
         raise DGLError("segment_scan_step has no gradient; segment_scan has")

@@ -24,9 +24,15 @@ def uniform(g, low, high, *shape):
     return low + (high - low) * torch.rand(*shape, generator=g, device="cuda", dtype=F64)
 
 
+def softmax(x):
+    """In numpy: torch's own of float64 rows of more than 1,024 is off by 1e-6."""
+    p = np.exp(x - x.max(1, keepdims=True))
+    return torch.from_numpy(p / p.sum(1, keepdims=True)).cuda()
+
+
 def check(x, bias, k, score, **kw):
-    f = torch.sigmoid if score == "sigmoid" else lambda t: torch.softmax(t, 1)
-    key = f(x.double()) + bias.double()
+    s = torch.sigmoid(x.double()) if score == "sigmoid" else softmax(x.double().cpu().numpy())
+    key = s + bias.double()
     want = np.argsort(-key.cpu().numpy(), axis=1, kind="stable")[:, :k]
     ids = ops.topk_route(x, k, score=score, bias=bias, **kw)[1].cpu().numpy()
     assert (ids == want).all(), "{} of {} rows".format(int((ids != want).any(1).sum()), len(x))
@@ -152,3 +158,34 @@ def test_sums_of_the_lowest_biases_stay_above_masked_groups(dtype, score):
         else:
             live = [sorted(i for i in r if x[n, i] > -inf) for n, r in enumerate(got)]
             assert all(len(r) == 2 for r in live), got
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("e,k", [(60, 2), (200, 9), (256, 20), (512, 5), (1000, 3), (2048, 2)])
+def test_the_rival_lies_anywhere(e, k, score):
+    """The same with the three among others, at any place: k - 1 experts in front of them
+    by their biases, the rest far behind."""
+    g = gen(e)
+    n = 4000
+    half = 2.0 ** -24
+    back = torch.logit if score == "sigmoid" else torch.log
+    fill = 1e-9
+    offset = [torch.tensor(t, device="cuda").double() for t in (0.00998, 0.009985, -0.94)]
+    large = back(0.95 + uniform(g, -1e-6, 1e-6, n, 1)).float()
+    s = torch.sigmoid(large.double()) if score == "sigmoid" else large.double().exp()
+    for lag in (0.5, 2.0):
+        first = s + offset[2] + uniform(g, -lag * half, lag * half, n, 1)
+        second = (first + s + offset[2]) / 2
+        small = [first - offset[0], second - offset[1]]
+        x = back(torch.full((n, e), fill, dtype=F64, device="cuda"))
+        bias = torch.full((e,), -0.5, dtype=F64, device="cuda")
+        place = torch.randperm(e, generator=g, device="cuda")
+        for i, col in enumerate([back(t) for t in small] + [large.double()]):
+            x[:, place[i]] = col[:, 0]
+            bias[place[i]] = offset[i]
+        for i in range(k - 1):
+            bias[place[3 + i]] = 0.5 + 0.01 * i
+        if score == "softmax":  # one that makes the scores sum to 1
+            x[:, place[k + 2]] = (1.0 - s - small[0] - small[1] - fill * (e - 4))[:, 0].log()
+            bias[place[k + 2]] = -5.0
+        check(x.float(), bias.float(), k, score)
