@@ -47,6 +47,8 @@ extern "C" {
  * routing) also take, with sums, statistics and states in float32: */
 #define MDGL_BFLOAT16 2
 #define MDGL_FLOAT16 3
+/* e4m3 values, one byte each (mdgl_dispatch_rows; 8-bit results have it by name) */
+#define MDGL_FLOAT8 4
 
 /* flags of mdgl_gspmm / mdgl_segment_reduce */
 #define MDGL_REPLACE_INF 1 /* +-inf results become 0 (heterograph.py:232-239) */
@@ -659,6 +661,50 @@ int mdgl_layer_norm_grad(const void* value, const void* weight, const void* mean
                          int64_t d, void* workspace, int64_t workspace_bytes, int dtype,
                          int weight_dtype, void* stream);
 int64_t mdgl_layer_norm_grad_workspace_bytes(int64_t n, int64_t d, int dtype);
+
+/* Root-mean-square norm over the d columns (fewer than 2**26) of each of n rows, with
+ * the residual's addition in front:
+ *   total = value + residual,  dst = total * rstd * weight,
+ *   rstd = 1 / sqrt(mean(total^2) + eps)
+ * dst is formed from the sum before its rounding. residual (null: none, total is then
+ * value and not written) and total have residual_dtype: the rows' dtype, or
+ * MDGL_FLOAT32 with rows of 16 bits; so has weight (null: 1) weight_dtype. rstd
+ * (state, n, nullable) is what the gradient takes. With dst_scale dst holds e4m3
+ * bytes, and dst_scale (float, [n][ceil(d / 128)]) the scales of their blocks of 128
+ * columns as mdgl_quantize_rows forms them of the unrounded results; not for
+ * MDGL_FLOAT64. No output may overlap an operand. */
+int mdgl_rms_norm(const void* value, const void* residual, const void* weight, void* dst,
+                  float* dst_scale, void* total, void* rstd, int64_t n, int64_t d, double eps,
+                  int dtype, int weight_dtype, int residual_dtype, void* stream);
+
+/* Gradients of mdgl_rms_norm from those of dst (grad) and of total (grad_total,
+ * residual_dtype, nullable). The rows that were normalised come in residual_dtype:
+ * with a residual in the state's type as the forward's total, and residual null; with
+ * a 16-bit residual, whose total is rounded, as value (`total`) and residual; without
+ * one as value, residual_dtype = dtype. dvalue (rows' dtype), dresidual
+ * (residual_dtype) and dweight (weight_dtype), each nullable; the workspace is needed
+ * for the last (summed over the rows in a fixed order). Nothing is written when n is 0. */
+int mdgl_rms_norm_grad(const void* total, const void* residual, const void* weight,
+                       const void* rstd, const void* grad, const void* grad_total, void* dvalue,
+                       void* dresidual, void* dweight, int64_t n, int64_t d, void* workspace,
+                       int64_t workspace_bytes, int dtype, int weight_dtype, int residual_dtype,
+                       void* stream);
+int64_t mdgl_rms_norm_grad_workspace_bytes(int64_t n, int64_t d, int dtype);
+
+/* n rows of d columns (not MDGL_FLOAT64) as e4m3 bytes with a scale for each block of
+ * 128 columns, [n][ceil(d / 128)]:
+ *   scale = max(max |value| / 448, 2^-126),  dst = value / scale to nearest even.
+ * A NaN stays one and does not enter the scale; an infinity makes its block's scale
+ * infinite. */
+int mdgl_quantize_rows(const void* value, void* dst, float* scale, int64_t n, int64_t d, int dtype,
+                       void* stream);
+
+/* r matrices of [d1][d2] values ([d2][d1] with `transposed`) as e4m3 bytes, always
+ * [d2][d1], with a scale for each block of 128 by 128,
+ * [r][ceil(d1 / 128)][ceil(d2 / 128)]: the weights of mdgl_scaled_mm. Fewer than
+ * 2**24 blocks a matrix. */
+int mdgl_quantize_blocks(const void* value, void* dst, float* scale, int64_t r, int64_t d1,
+                         int64_t d2, int transposed, int dtype, void* stream);
 
 /* Routing rows to experts. For each of n rows of num_experts logits (at most
  * 2048), the k (at most 32) experts of the largest keys, falling, the lowest index

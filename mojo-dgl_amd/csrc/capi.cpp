@@ -1783,6 +1783,125 @@ int mdgl_layer_norm_grad(const void* value, const void* weight, const void* mean
 
 namespace {
 
+int rms_common(const char* what, int64_t n, int64_t d, int dtype, int weight_dtype,
+               int residual_dtype) {
+  if (int rc = norm_common(what, n, d, dtype, weight_dtype)) return rc;
+  if (residual_dtype != dtype && !(residual_dtype == MDGL_FLOAT32 && half_dtype(dtype)))
+    return fail(MDGL_EINVAL, "%s: a residual of dtype %d with rows of %d", what, residual_dtype,
+                dtype);
+  return MDGL_OK;
+}
+
+int quant_dtype(const char* what, int dtype) {
+  if (dtype == MDGL_FLOAT64 || !row_dtype_ok(dtype))
+    return fail(MDGL_EINVAL, "%s: no 8-bit values of dtype %d", what, dtype);
+  return MDGL_OK;
+}
+
+}  // namespace
+
+int mdgl_rms_norm(const void* value, const void* residual, const void* weight, void* dst,
+                  float* dst_scale, void* total, void* rstd, int64_t n, int64_t d, double eps,
+                  int dtype, int weight_dtype, int residual_dtype, void* stream) {
+  MDGL_RANGE();
+  if (int rc = rms_common("rms_norm", n, d, dtype, weight_dtype, residual_dtype)) return rc;
+  if (dst_scale)
+    if (int rc = quant_dtype("rms_norm", dtype)) return rc;
+  if (!(eps >= 0)) return fail(MDGL_EINVAL, "rms_norm: eps must be >= 0");
+  if (n == 0 || d == 0) return MDGL_OK;
+  if (!value || !dst || (residual && !total))
+    return fail(MDGL_EINVAL, "rms_norm: null buffer");
+  RmsParams q{};
+  q.x = value;
+  q.residual = residual;
+  q.w = weight;
+  q.y = dst;
+  q.scale = dst_scale;
+  q.total = residual ? total : nullptr;
+  q.rstd = rstd;
+  q.n = n;
+  q.d = d;
+  q.eps = eps;
+  q.weight_f32 = weight_dtype == MDGL_FLOAT32;
+  q.residual_f32 = residual_dtype == MDGL_FLOAT32;
+  q.stream = (hipStream_t)stream;
+  return hip_status(launch_rms(q, dtype), "rms_norm");
+}
+
+int64_t mdgl_rms_norm_grad_workspace_bytes(int64_t n, int64_t d, int dtype) {
+  if (n < 0 || d < 0 || !row_dtype_ok(dtype)) return -1;
+  // one sum a column and workgroup, where layer norm's gradient has two
+  return n == 0 || d == 0 ? 0 : norm_workspace_bytes(n, d, dtype) / 2;
+}
+
+int mdgl_rms_norm_grad(const void* total, const void* residual, const void* weight,
+                       const void* rstd, const void* grad, const void* grad_total, void* dvalue,
+                       void* dresidual, void* dweight, int64_t n, int64_t d, void* workspace,
+                       int64_t workspace_bytes, int dtype, int weight_dtype, int residual_dtype,
+                       void* stream) {
+  MDGL_RANGE();
+  if (int rc = rms_common("rms_norm_grad", n, d, dtype, weight_dtype, residual_dtype)) return rc;
+  if (n == 0 || d == 0) return MDGL_OK;
+  if (!dvalue && !dresidual && !dweight) return MDGL_OK;
+  if (residual && !half_dtype(residual_dtype))
+    return fail(MDGL_EINVAL, "rms_norm_grad: a residual of dtype %d is in the total",
+                residual_dtype);
+  if (!total || !rstd || !grad) return fail(MDGL_EINVAL, "rms_norm_grad: null buffer");
+  const int64_t need = dweight ? norm_workspace_bytes(n, d, dtype) / 2 : 0;
+  if (need > 0 && workspace && !aligned(workspace, WS_ALIGN))
+    return fail(MDGL_EINVAL, "workspace must be %lld-byte aligned", (long long)WS_ALIGN);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(MDGL_EWORKSPACE, "rms_norm_grad: workspace of %lld bytes needed, %lld given",
+                (long long)need, (long long)workspace_bytes);
+  RmsParams q{};
+  q.total = const_cast<void*>(total);
+  q.residual = residual;
+  q.w = weight;
+  q.rstd = const_cast<void*>(rstd);
+  q.dy = grad;
+  q.dtotal = grad_total;
+  q.dx = dvalue;
+  q.dresidual = dresidual;
+  q.dw = dweight;
+  q.n = n;
+  q.d = d;
+  q.weight_f32 = weight_dtype == MDGL_FLOAT32;
+  q.residual_f32 = residual_dtype == MDGL_FLOAT32;
+  q.workspace = workspace;
+  q.stream = (hipStream_t)stream;
+  return hip_status(launch_rms(q, dtype), "rms_norm_grad");
+}
+
+int mdgl_quantize_rows(const void* value, void* dst, float* scale, int64_t n, int64_t d, int dtype,
+                       void* stream) {
+  MDGL_RANGE();
+  if (int rc = quant_dtype("quantize_rows", dtype)) return rc;
+  if (n < 0 || d < 0) return fail(MDGL_EINVAL, "quantize_rows: negative size");
+  if (!row_widths_fit(d, dtype_bytes(dtype)))
+    return fail(MDGL_EINVAL, "quantize_rows: rows of 2 GiB or more");
+  if (n == 0 || d == 0) return MDGL_OK;
+  if (!value || !dst || !scale) return fail(MDGL_EINVAL, "quantize_rows: null buffer");
+  return hip_status(launch_quantize_rows(value, dst, scale, n, d, dtype, (hipStream_t)stream),
+                    "quantize_rows");
+}
+
+int mdgl_quantize_blocks(const void* value, void* dst, float* scale, int64_t r, int64_t d1,
+                         int64_t d2, int transposed, int dtype, void* stream) {
+  MDGL_RANGE();
+  if (int rc = quant_dtype("quantize_blocks", dtype)) return rc;
+  if (r < 0 || d1 < 0 || d2 < 0) return fail(MDGL_EINVAL, "quantize_blocks: negative size");
+  if (!row_widths_fit(d1, dtype_bytes(dtype)) || !row_widths_fit(d2, dtype_bytes(dtype)) ||
+      ((d1 + 127) / 128) * ((d2 + 127) / 128) >= (int64_t(1) << 24))
+    return fail(MDGL_EINVAL, "quantize_blocks: 2**24 or more blocks a matrix");
+  if (r == 0 || d1 == 0 || d2 == 0) return MDGL_OK;
+  if (!value || !dst || !scale) return fail(MDGL_EINVAL, "quantize_blocks: null buffer");
+  return hip_status(launch_quantize_blocks(value, dst, scale, r, d1, d2, transposed != 0, dtype,
+                                           (hipStream_t)stream),
+                    "quantize_blocks");
+}
+
+namespace {
+
 int route_common(const char* what, int64_t n, int64_t e, int64_t k, int score, int dtype) {
   if (!row_dtype_ok(dtype)) return fail(MDGL_EINVAL, "%s: bad dtype %d", what, dtype);
   if (n < 0) return fail(MDGL_EINVAL, "%s: negative size", what);

@@ -394,6 +394,42 @@ hipError_t launch_norm_f64(const NormParams& q);
 hipError_t launch_norm_bf16(const NormParams& q);
 hipError_t launch_norm_f16(const NormParams& q);
 
+// Root-mean-square norm (rms_impl.h), laid out by norm_geometry; the gradients when
+// `dy` is given. With `scale` y is in 8 bits. `total`: the sum forward (may be null),
+// the normalised rows backward.
+struct RmsParams {
+  const void* x;
+  const void* residual;
+  const void* w;
+  void* y;
+  void* scale;
+  void* total;
+  void* rstd;
+  const void* dy;
+  const void* dtotal;
+  void* dx;
+  void* dresidual;
+  void* dw;
+  int64_t n, d;
+  double eps;
+  int weight_f32, residual_f32;
+  void* workspace;
+  hipStream_t stream;
+};
+hipError_t launch_rms(const RmsParams& q, int dtype);
+hipError_t launch_rms_f32(const RmsParams& q);
+hipError_t launch_rms_f64(const RmsParams& q);
+hipError_t launch_rms_bf16(const RmsParams& q);
+hipError_t launch_rms_f16(const RmsParams& q);
+
+// Values in 8 bits (quant.h, quant.hip): rows of d columns with a scale a block of 128,
+// or r matrices [d1][d2] (transposed: [d2][d1]) as [d2][d1] with a scale a block of 128
+// by 128.
+hipError_t launch_quantize_rows(const void* src, void* dst, float* scale, int64_t n, int64_t d,
+                                int dtype, hipStream_t s);
+hipError_t launch_quantize_blocks(const void* src, void* dst, float* scale, int64_t r, int64_t d1,
+                                  int64_t d2, bool transposed, int dtype, hipStream_t s);
+
 // Routing to experts (route_impl.h); the weights' gradient when `dlogits` is given.
 constexpr int ROUTE_MAX_EXPERTS = 2048;
 constexpr int ROUTE_MAX_K = 32;

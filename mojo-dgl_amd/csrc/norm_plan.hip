@@ -1,4 +1,4 @@
-// How layer norm lays its rows on threads, and the dispatch by type.
+// How the norms lay their rows on threads, and the dispatch by type.
 #include "mdgl_half.h"
 #include "mdgl_kernels.h"
 
@@ -42,6 +42,15 @@ hipError_t launch_norm(const NormParams& q, int dtype) {
     case DT_F64: return launch_norm_f64(q);
     case DT_BF16: return launch_norm_bf16(q);
     default: return launch_norm_f16(q);
+  }
+}
+
+hipError_t launch_rms(const RmsParams& q, int dtype) {
+  switch (dtype) {
+    case DT_F32: return launch_rms_f32(q);
+    case DT_F64: return launch_rms_f64(q);
+    case DT_BF16: return launch_rms_bf16(q);
+    default: return launch_rms_f16(q);
   }
 }
 

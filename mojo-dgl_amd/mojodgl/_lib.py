@@ -51,6 +51,7 @@ TARGETS = {"u": SRC_CODE, "v": DST_CODE, "e": EDGE_CODE}
 
 FLOAT32, FLOAT64 = 0, 1
 BFLOAT16, FLOAT16 = 2, 3  # row operators only (layer norm, the segment scan, routing)
+FLOAT8 = 4  # dispatch_rows only
 REPLACE_INF = 1
 RHS_CSR_ORDER = 2
 LHS_LINE_ROWS = 8  # mdgl_gspmm: lhs rows copied to start on 128-byte lines
@@ -151,6 +152,13 @@ _SIGNATURES = {
     "mdgl_layer_norm_grad": ([_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _C, _C, _P],
                              _C),
     "mdgl_layer_norm_grad_workspace_bytes": ([_I64, _I64, _C], _I64),
+    "mdgl_rms_norm": ([_P, _P, _P, _P, _P, _P, _P, _I64, _I64, ctypes.c_double, _C, _C, _C, _P],
+                      _C),
+    "mdgl_rms_norm_grad": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _C, _C, _C,
+                            _P], _C),
+    "mdgl_rms_norm_grad_workspace_bytes": ([_I64, _I64, _C], _I64),
+    "mdgl_quantize_rows": ([_P, _P, _P, _I64, _I64, _C, _P], _C),
+    "mdgl_quantize_blocks": ([_P, _P, _P, _I64, _I64, _I64, _C, _C, _P], _C),
     "mdgl_topk_route": ([_P, _P, _P, _P, _I64, _I64, _I64, _C, _I64, _I64, _C, _C,
                          ctypes.c_double, _C, _P], _C),
     "mdgl_topk_route_grad": ([_P, _P, _P, _P, _I64, _I64, _I64, _C, _C, ctypes.c_double, _C, _P],

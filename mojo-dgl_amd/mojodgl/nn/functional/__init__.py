@@ -1,4 +1,4 @@
-"""`nn.functional.edge_softmax` is `ops.edge_softmax` itself, and `layer_norm`
-`ops.layer_norm`."""
+"""`nn.functional.edge_softmax` is `ops.edge_softmax` itself, `layer_norm` and
+`rms_norm` are those of `ops`."""
 
-from ...ops import edge_softmax, layer_norm  # noqa: F401
+from ...ops import edge_softmax, layer_norm, rms_norm  # noqa: F401

@@ -42,7 +42,8 @@ these follow the calculus of the forward ops and run on the same kernels:
   ``mdgl_segment_reduce_arg``), softmax as edge_softmax;
 * segment_scan: the reverse recurrence (``mdgl_segment_scan_grad``);
 * layer_norm: dx and the sums of the weights' gradients in one pass
-  (``mdgl_layer_norm_grad``);
+  (``mdgl_layer_norm_grad``); rms_norm: the same from its sum of value and
+  residual, whose own gradient is added (``mdgl_rms_norm_grad``);
 * topk_route: the chosen experts' weights back to the logits
   (``mdgl_topk_route_grad``); dispatch_rows: the sum of a row's copies
   (``mdgl_combine_rows`` without weights); combine_rows:
@@ -72,7 +73,7 @@ from .. import _lib
 from ..base import DGLError
 
 __all__ = ["needs_grad", "GSpMM", "GSDDMM", "EdgeSoftmax", "SegmentReduce", "SegmentSoftmax",
-           "SegmentMM", "GatherMM", "SegmentScan", "LayerNorm",
+           "SegmentMM", "GatherMM", "SegmentScan", "LayerNorm", "RmsNorm",
            "TopkRoute", "DispatchRows", "CombineRows"]
 
 
@@ -741,6 +742,43 @@ class LayerNorm(torch.autograd.Function):
         dx, dw, db = _layer_norm_grad(value, weight, bias, stats, grad,
                                       ctx.needs_input_grad[:3])
         return _back(dx, value), _back(dw, weight), _back(db, bias), None
+
+
+class RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, value, weight, residual, eps):
+        from .norm import _rms_norm, _rms_operands
+
+        y, total, rstd = _rms_norm(value, weight, residual, eps, False, True)
+        ctx.types = _rms_operands(value, weight, residual)[3:6]
+        ctx.set_materialize_grads(False)
+        where = _lib.caller_device(value, weight, residual)
+        y = _lib.hand_back(y, where)
+        total = None if total is None else _lib.hand_back(total, where)
+        ctx.like = tuple(x if x is None or not isinstance(x, torch.Tensor)
+                         else torch.empty(0, dtype=x.dtype, device=x.device)
+                         for x in (value, residual))
+        # of the rows and the residual their sum will do unless it is rounded to 16 bits
+        if residual is None or ctx.types[2].itemsize == 2:
+            _save_some(ctx, value, residual, weight, rstd)
+        else:
+            _save_some(ctx, total, None, weight, rstd)
+        _made_here(ctx, where)
+        return y, total
+
+    @staticmethod
+    @once_differentiable
+    @_where_made
+    def backward(ctx, grad, grad_total):
+        from .norm import _rms_norm_grad
+
+        if grad is None and grad_total is None:
+            return None, None, None, None
+        total, added, weight, rstd = _saved_some(ctx)
+        dx, dw, dr = _rms_norm_grad(total, added, weight, rstd, grad, grad_total, *ctx.types,
+                                    ctx.needs_input_grad[:3])
+        value, residual = ctx.like
+        return _back(dx, value), _back(dw, weight), _back(dr, residual), None
 
 
 class TopkRoute(torch.autograd.Function):
