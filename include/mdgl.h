@@ -706,6 +706,40 @@ int mdgl_quantize_rows(const void* value, void* dst, float* scale, int64_t n, in
 int mdgl_quantize_blocks(const void* value, void* dst, float* scale, int64_t r, int64_t d1,
                          int64_t d2, int transposed, int dtype, void* stream);
 
+/* Products of n rows of d1 columns with the r matrices of [d1][d2] of their groups
+ * (MDGL_BFLOAT16 or MDGL_FLOAT16, sums in float):
+ *   dst[i] = a[i] @ b[g(i)]
+ * for consecutive groups of seglen[g] rows (device; cut where they do not fit the n
+ * rows, negative ones are 0); rows behind the last group are written as zeros. With
+ * `transposed` b holds [d2][d1] each: with the same b, a gradient of dst and d1 and d2
+ * exchanged that is the gradient of a. Fewer than 2**31 rows and 2**20 columns, at
+ * most 65535 groups. Without any group or d1 dst is zeros. */
+int mdgl_expert_mm(const void* a, const void* b, void* dst, const int64_t* seglen, int64_t n,
+                   int64_t d1, int64_t r, int64_t d2, int transposed, void* workspace,
+                   int64_t workspace_bytes, int dtype, void* stream);
+int64_t mdgl_expert_mm_workspace_bytes(int64_t n, int64_t d1, int64_t r, int64_t d2, int dtype);
+
+/* Gradient of mdgl_expert_mm in b, from that of dst (grad): db[g] = sum over the rows
+ * of group g, in a fixed order, of a[i]^T grad[i]; [d1][d2] each (exchange a and grad,
+ * and d1 and d2, for [d2][d1]). Zeros for groups without rows. */
+int mdgl_expert_mm_grad(const void* a, const void* grad, void* db, const int64_t* seglen,
+                        int64_t n, int64_t d1, int64_t r, int64_t d2, void* workspace,
+                        int64_t workspace_bytes, int dtype, void* stream);
+int64_t mdgl_expert_mm_grad_workspace_bytes(int64_t n, int64_t d1, int64_t r, int64_t d2,
+                                            int dtype);
+
+/* mdgl_expert_mm of e4m3 values: a as mdgl_quantize_rows (a_scale [n][ceil(d1 / 128)])
+ * and b as mdgl_quantize_blocks writes them ([d2][d1] each, b_scale
+ * [r][ceil(d1 / 128)][ceil(d2 / 128)]):
+ *   dst[i][c] = sum over k of a_scale a[i][k] b_scale b[g(i)][c][k]
+ * summed in float block by block of 128; within eight neighbouring k products are cut
+ * off 13 binary places below the largest. A null seglen is one group of all rows
+ * (r = 1). dst_dtype: MDGL_FLOAT32, MDGL_BFLOAT16 or MDGL_FLOAT16. */
+int mdgl_scaled_mm(const void* a, const float* a_scale, const void* b, const float* b_scale,
+                   void* dst, const int64_t* seglen, int64_t n, int64_t d1, int64_t r, int64_t d2,
+                   void* workspace, int64_t workspace_bytes, int dst_dtype, void* stream);
+int64_t mdgl_scaled_mm_workspace_bytes(int64_t n, int64_t d1, int64_t r, int64_t d2);
+
 /* Routing rows to experts. For each of n rows of num_experts logits (at most
  * 2048), the k (at most 32) experts of the largest keys, falling, the lowest index
  * among equals, into ids, and their weights (state). Scores: softmax or sigmoid of

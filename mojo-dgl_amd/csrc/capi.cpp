@@ -1902,6 +1902,159 @@ int mdgl_quantize_blocks(const void* value, void* dst, float* scale, int64_t r, 
 
 namespace {
 
+int expert_mm_common(const char* what, int64_t n, int64_t d1, int64_t r, int64_t d2) {
+  if (n < 0 || d1 < 0 || r < 0 || d2 < 0) return fail(MDGL_EINVAL, "%s: negative size", what);
+  if (n >= (int64_t(1) << 31)) return fail(MDGL_EINVAL, "%s: 2**31 or more rows", what);
+  if (d1 >= EXPERT_MM_COLS || d2 >= EXPERT_MM_COLS)
+    return fail(MDGL_EINVAL, "%s: 2**20 or more columns", what);
+  if (r > EXPERT_MM_GROUPS)
+    return fail(MDGL_EINVAL, "%s: at most %lld groups, got %lld", what,
+                (long long)EXPERT_MM_GROUPS, (long long)r);
+  return MDGL_OK;
+}
+
+// Bytes that serve whichever way the operands are aligned; -1 for too many tiles.
+int64_t expert_mm_bytes(const ExpertMmPlan& a, const ExpertMmPlan& b) {
+  if (a.shape < 0 || b.shape < 0) return -1;
+  return a.bytes > b.bytes ? a.bytes : b.bytes;
+}
+
+int64_t expert_mm_need(int64_t n, int64_t d1, int64_t r, int64_t d2, int size) {
+  if (n == 0 || d2 == 0) return 0;
+  return expert_mm_bytes(expert_mm_plan(n, r, d1, d2, size, true),
+                         expert_mm_plan(n, r, d1, d2, size, false));
+}
+
+int64_t expert_mm_grad_need(int64_t n, int64_t d1, int64_t r, int64_t d2) {
+  if (r == 0 || d1 == 0 || d2 == 0) return 0;
+  return expert_mm_bytes(expert_mm_grad_plan(n, r, d1, d2, true),
+                         expert_mm_grad_plan(n, r, d1, d2, false));
+}
+
+int expert_mm_workspace(const char* what, int64_t need, const void* workspace,
+                        int64_t workspace_bytes) {
+  if (need < 0) return fail(MDGL_EINVAL, "%s: 2**31 or more tiles of results", what);
+  if (need > 0 && workspace && !aligned(workspace, WS_ALIGN))
+    return fail(MDGL_EINVAL, "workspace must be %lld-byte aligned", (long long)WS_ALIGN);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(MDGL_EWORKSPACE, "%s: workspace of %lld bytes needed, %lld given", what,
+                (long long)need, (long long)workspace_bytes);
+  return MDGL_OK;
+}
+
+}  // namespace
+
+int64_t mdgl_expert_mm_workspace_bytes(int64_t n, int64_t d1, int64_t r, int64_t d2, int dtype) {
+  if (!half_dtype(dtype) || expert_mm_common("expert_mm", n, d1, r, d2)) return -1;
+  return expert_mm_need(n, d1, r, d2, 2);
+}
+
+int mdgl_expert_mm(const void* a, const void* b, void* dst, const int64_t* seglen, int64_t n,
+                   int64_t d1, int64_t r, int64_t d2, int transposed, void* workspace,
+                   int64_t workspace_bytes, int dtype, void* stream) {
+  MDGL_RANGE();
+  if (!half_dtype(dtype)) return fail(MDGL_EINVAL, "expert_mm: bad dtype %d", dtype);
+  if (int rc = expert_mm_common("expert_mm", n, d1, r, d2)) return rc;
+  if (n == 0 || d2 == 0) return MDGL_OK;
+  if (!dst || (r > 0 && (!seglen || (d1 > 0 && (!a || !b)))))
+    return fail(MDGL_EINVAL, "expert_mm: null buffer");
+  if (int rc = expert_mm_workspace("expert_mm", expert_mm_need(n, d1, r, d2, 2), workspace,
+                                   workspace_bytes))
+    return rc;
+  ExpertMmParams q{};
+  q.a = a;
+  q.b = b;
+  q.out = dst;
+  q.seglen = seglen;
+  q.rows = n;
+  q.groups = r;
+  q.inner = d1;
+  q.cols = d2;
+  q.along = transposed != 0;
+  q.plan = expert_mm_plan(n, r, d1, d2, 2, aligned(a, 16) && aligned(b, 16) && d1 % 8 == 0 &&
+                                               (q.along || d2 % 8 == 0));
+  q.workspace = workspace;
+  q.stream = (hipStream_t)stream;
+  return hip_status(dtype == MDGL_BFLOAT16 ? launch_expert_mm_bf16(q) : launch_expert_mm_f16(q),
+                    "expert_mm");
+}
+
+int64_t mdgl_expert_mm_grad_workspace_bytes(int64_t n, int64_t d1, int64_t r, int64_t d2,
+                                            int dtype) {
+  if (!half_dtype(dtype) || expert_mm_common("expert_mm_grad", n, d1, r, d2)) return -1;
+  return expert_mm_grad_need(n, d1, r, d2);
+}
+
+int mdgl_expert_mm_grad(const void* a, const void* grad, void* db, const int64_t* seglen,
+                        int64_t n, int64_t d1, int64_t r, int64_t d2, void* workspace,
+                        int64_t workspace_bytes, int dtype, void* stream) {
+  MDGL_RANGE();
+  if (!half_dtype(dtype)) return fail(MDGL_EINVAL, "expert_mm_grad: bad dtype %d", dtype);
+  if (int rc = expert_mm_common("expert_mm_grad", n, d1, r, d2)) return rc;
+  if (r == 0 || d1 == 0 || d2 == 0) return MDGL_OK;
+  if (!db || !seglen || (n > 0 && (!a || !grad)))
+    return fail(MDGL_EINVAL, "expert_mm_grad: null buffer");
+  if (int rc = expert_mm_workspace("expert_mm_grad", expert_mm_grad_need(n, d1, r, d2), workspace,
+                                   workspace_bytes))
+    return rc;
+  ExpertMmParams q{};
+  q.a = a;
+  q.b = grad;
+  q.out = db;
+  q.seglen = seglen;
+  q.rows = n;
+  q.groups = r;
+  q.inner = d1;
+  q.cols = d2;
+  q.plan = expert_mm_grad_plan(
+      n, r, d1, d2, aligned(a, 16) && aligned(grad, 16) && d1 % 8 == 0 && d2 % 8 == 0);
+  q.workspace = q.plan.bytes > 0 ? workspace : nullptr;
+  q.stream = (hipStream_t)stream;
+  return hip_status(
+      dtype == MDGL_BFLOAT16 ? launch_expert_mm_grad_bf16(q) : launch_expert_mm_grad_f16(q),
+      "expert_mm_grad");
+}
+
+int64_t mdgl_scaled_mm_workspace_bytes(int64_t n, int64_t d1, int64_t r, int64_t d2) {
+  if (expert_mm_common("scaled_mm", n, d1, r, d2)) return -1;
+  return expert_mm_need(n, d1, r, d2, 1);
+}
+
+int mdgl_scaled_mm(const void* a, const float* a_scale, const void* b, const float* b_scale,
+                   void* dst, const int64_t* seglen, int64_t n, int64_t d1, int64_t r, int64_t d2,
+                   void* workspace, int64_t workspace_bytes, int dst_dtype, void* stream) {
+  MDGL_RANGE();
+  if (int rc = quant_dtype("scaled_mm", dst_dtype)) return rc;
+  if (int rc = expert_mm_common("scaled_mm", n, d1, r, d2)) return rc;
+  if (!seglen && r != 1)
+    return fail(MDGL_EINVAL, "scaled_mm: lengths are wanted for %lld groups", (long long)r);
+  if (n == 0 || d2 == 0) return MDGL_OK;
+  if (!dst || (r > 0 && d1 > 0 && (!a || !a_scale || !b || !b_scale)))
+    return fail(MDGL_EINVAL, "scaled_mm: null buffer");
+  if (int rc = expert_mm_workspace("scaled_mm", expert_mm_need(n, d1, r, d2, 1), workspace,
+                                   workspace_bytes))
+    return rc;
+  ExpertMmParams q{};
+  q.a = a;
+  q.b = b;
+  q.a_scale = a_scale;
+  q.b_scale = b_scale;
+  q.out = dst;
+  q.seglen = seglen;
+  q.rows = n;
+  q.groups = r;
+  q.inner = d1;
+  q.cols = d2;
+  q.along = true;
+  q.out_dtype = dst_dtype;
+  q.plan = expert_mm_plan(n, r, d1, d2, 1, aligned(a, 16) && aligned(b, 16) && d1 % 16 == 0);
+  q.workspace = workspace;
+  q.stream = (hipStream_t)stream;
+  return hip_status(launch_expert_mm_f8(q), "scaled_mm");
+}
+
+namespace {
+
 int route_common(const char* what, int64_t n, int64_t e, int64_t k, int score, int dtype) {
   if (!row_dtype_ok(dtype)) return fail(MDGL_EINVAL, "%s: bad dtype %d", what, dtype);
   if (n < 0) return fail(MDGL_EINVAL, "%s: negative size", what);
@@ -1916,8 +2069,10 @@ int route_common(const char* what, int64_t n, int64_t e, int64_t k, int score, i
   return MDGL_OK;
 }
 
-int move_common(const char* what, int64_t n, int64_t k, int64_t d, int dtype) {
-  if (!row_dtype_ok(dtype)) return fail(MDGL_EINVAL, "%s: bad dtype %d", what, dtype);
+int move_common(const char* what, int64_t n, int64_t k, int64_t d, int dtype,
+                bool bytes = false) {
+  if (!row_dtype_ok(dtype) && !(bytes && dtype == MDGL_FLOAT8))
+    return fail(MDGL_EINVAL, "%s: bad dtype %d", what, dtype);
   if (n < 0 || k < 0 || d < 0) return fail(MDGL_EINVAL, "%s: negative size", what);
   if (n >= (int64_t(1) << 31) || k >= (int64_t(1) << 31) || n * k >= (int64_t(1) << 31))
     return fail(MDGL_EINVAL, "%s: 2**31 or more entries", what);
@@ -2021,7 +2176,7 @@ int mdgl_route_plan(const int64_t* ids, int64_t num_entries, int64_t num_experts
 int mdgl_dispatch_rows(const void* src, const int32_t* slot, void* dst, int64_t n, int64_t k,
                        int64_t d, int dtype, void* stream) {
   MDGL_RANGE();
-  if (int rc = move_common("dispatch_rows", n, k, d, dtype)) return rc;
+  if (int rc = move_common("dispatch_rows", n, k, d, dtype, true)) return rc;
   if (n == 0 || k == 0 || d == 0) return MDGL_OK;
   if (!src || !slot || !dst) return fail(MDGL_EINVAL, "dispatch_rows: null buffer");
   const MoveParams q{src, slot, nullptr, nullptr, dst, nullptr, n, d, (int)k, (hipStream_t)stream};

@@ -382,6 +382,25 @@ hipError_t run_move(const MoveParams& q, MoveKind kind) {
   });
 }
 
+// Rows of e4m3 values, whose bytes are copied; they are never summed.
+hipError_t run_dispatch_bytes(const MoveParams& q) {
+  const int V = q.d >= 16 ? 16 : 1;
+  const int64_t lanes = (q.d + V - 1) / V;
+  return by_launches(q.n, MAX_LAUNCH_BLOCKS * BLOCK / lanes, [&](int64_t at, int64_t n) {
+    MoveArgs<uint8_t> p{};
+    p.src = (const uint8_t*)q.src + at * q.d;
+    p.slot = q.slot + at * q.k;
+    p.dst = (uint8_t*)q.dst;
+    p.n = n;
+    p.d = q.d;
+    p.lanes = lanes;
+    p.k = q.k;
+    const int64_t grid = (n * lanes + BLOCK - 1) / BLOCK;
+    if (V == 16) dispatch_kernel<uint8_t, 16><<<grid, BLOCK, 0, q.stream>>>(p);
+    else dispatch_kernel<uint8_t, 1><<<grid, BLOCK, 0, q.stream>>>(p);
+  });
+}
+
 template <class T>
 hipError_t run_move_width(const MoveParams& q, MoveKind kind) {
   if (q.d >= move_vec<T>()) return run_move<T, move_vec<T>()>(q, kind);
@@ -421,6 +440,7 @@ hipError_t launch_route_plan(const int64_t* ids, int64_t m, int experts, int64_t
 
 hipError_t launch_move(const MoveParams& q, MoveKind kind, int dtype) {
   switch (dtype) {
+    case DT_F8: return run_dispatch_bytes(q);
     case DT_F32: return run_move_width<float>(q, kind);
     case DT_F64: return run_move_width<double>(q, kind);
     case DT_BF16: return run_move_width<bf16_t>(q, kind);

@@ -15,8 +15,10 @@ template <> struct AccOf<double> { using type = double; };
 template <class T> using acc_t = typename AccOf<T>::type;
 
 // Dtype codes of include/mdgl.h.
-enum DType { DT_F32 = 0, DT_F64 = 1, DT_BF16 = 2, DT_F16 = 3 };
-inline int64_t dtype_bytes(int dtype) { return dtype == DT_F64 ? 8 : dtype == DT_F32 ? 4 : 2; }
+enum DType { DT_F32 = 0, DT_F64 = 1, DT_BF16 = 2, DT_F16 = 3, DT_F8 = 4 };
+inline int64_t dtype_bytes(int dtype) {
+  return dtype == DT_F64 ? 8 : dtype == DT_F32 ? 4 : dtype == DT_F8 ? 1 : 2;
+}
 
 // Values per 16 bytes of the accumulator type: the columns a lane of the
 // scan or of the row movers holds.

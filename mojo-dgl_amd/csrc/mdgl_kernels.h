@@ -430,6 +430,42 @@ hipError_t launch_quantize_rows(const void* src, void* dst, float* scale, int64_
 hipError_t launch_quantize_blocks(const void* src, void* dst, float* scale, int64_t r, int64_t d1,
                                   int64_t d2, bool transposed, int dtype, hipStream_t s);
 
+// Products with experts' matrices in 16 and 8 bits (expert_mm_impl.h), and the shape of
+// their tiles (expert_mm_plan.hip).
+constexpr int64_t EXPERT_MM_COLS = int64_t(1) << 20;  // columns: fewer
+constexpr int64_t EXPERT_MM_GROUPS = 65535;
+struct ExpertMmPlan {
+  int shape;       // -1: more tiles than can be counted
+  int splits;      // parts of the inner axis (forward)
+  int64_t piece;   // rows of a partial result (gradient of b)
+  int64_t tiles;   // at most
+  int64_t bytes;   // of the workspace
+};
+// direct: rows of both operands start on 16-byte boundaries. size: bytes of a value.
+ExpertMmPlan expert_mm_plan(int64_t rows, int64_t groups, int64_t inner, int64_t cols, int size,
+                            bool direct);
+ExpertMmPlan expert_mm_grad_plan(int64_t rows, int64_t groups, int64_t d1, int64_t d2,
+                                 bool direct);
+struct ExpertMmParams {
+  const void* a;
+  const void* b;  // gradient: the results' gradient
+  const float* a_scale;
+  const float* b_scale;
+  void* out;
+  const int64_t* seglen;  // null: one group of all rows
+  int64_t rows, groups, inner, cols;  // gradient: inner = D1, cols = D2
+  bool along;     // b's inner axis is contiguous
+  int out_dtype;  // 8 bits
+  ExpertMmPlan plan;
+  void* workspace;
+  hipStream_t stream;
+};
+hipError_t launch_expert_mm_bf16(const ExpertMmParams& q);
+hipError_t launch_expert_mm_f16(const ExpertMmParams& q);
+hipError_t launch_expert_mm_f8(const ExpertMmParams& q);
+hipError_t launch_expert_mm_grad_bf16(const ExpertMmParams& q);
+hipError_t launch_expert_mm_grad_f16(const ExpertMmParams& q);
+
 // Routing to experts (route_impl.h); the weights' gradient when `dlogits` is given.
 constexpr int ROUTE_MAX_EXPERTS = 2048;
 constexpr int ROUTE_MAX_K = 32;

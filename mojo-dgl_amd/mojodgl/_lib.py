@@ -159,6 +159,12 @@ _SIGNATURES = {
     "mdgl_rms_norm_grad_workspace_bytes": ([_I64, _I64, _C], _I64),
     "mdgl_quantize_rows": ([_P, _P, _P, _I64, _I64, _C, _P], _C),
     "mdgl_quantize_blocks": ([_P, _P, _P, _I64, _I64, _I64, _C, _C, _P], _C),
+    "mdgl_expert_mm": ([_P, _P, _P, _P, _I64, _I64, _I64, _I64, _C, _P, _I64, _C, _P], _C),
+    "mdgl_expert_mm_workspace_bytes": ([_I64, _I64, _I64, _I64, _C], _I64),
+    "mdgl_expert_mm_grad": ([_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _C, _P], _C),
+    "mdgl_expert_mm_grad_workspace_bytes": ([_I64, _I64, _I64, _I64, _C], _I64),
+    "mdgl_scaled_mm": ([_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _C, _P], _C),
+    "mdgl_scaled_mm_workspace_bytes": ([_I64, _I64, _I64, _I64], _I64),
     "mdgl_topk_route": ([_P, _P, _P, _P, _I64, _I64, _I64, _C, _I64, _I64, _C, _C,
                          ctypes.c_double, _C, _P], _C),
     "mdgl_topk_route_grad": ([_P, _P, _P, _P, _I64, _I64, _I64, _C, _C, ctypes.c_double, _C, _P],

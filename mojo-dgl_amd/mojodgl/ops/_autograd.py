@@ -47,7 +47,8 @@ these follow the calculus of the forward ops and run on the same kernels:
 * topk_route: the chosen experts' weights back to the logits
   (``mdgl_topk_route_grad``); dispatch_rows: the sum of a row's copies
   (``mdgl_combine_rows`` without weights); combine_rows:
-  ``mdgl_combine_rows_grad``.
+  ``mdgl_combine_rows_grad``; expert_mm: the product with the weights'
+  transposes (``mdgl_expert_mm``) and ``mdgl_expert_mm_grad``.
 
 The backward passes run on the library's kernels, outside torch's graph, so
 they are differentiable once: a second derivative through them raises. So does
@@ -74,7 +75,7 @@ from ..base import DGLError
 
 __all__ = ["needs_grad", "GSpMM", "GSDDMM", "EdgeSoftmax", "SegmentReduce", "SegmentSoftmax",
            "SegmentMM", "GatherMM", "SegmentScan", "LayerNorm", "RmsNorm",
-           "TopkRoute", "DispatchRows", "CombineRows"]
+           "TopkRoute", "DispatchRows", "ExpertMM", "CombineRows"]
 
 
 def needs_grad(*xs) -> bool:
@@ -824,6 +825,30 @@ class DispatchRows(torch.autograd.Function):
         from .route import _sum_rows
 
         return _back(_sum_rows(_gpu(grad).contiguous(), None, ctx.plan), ctx.like), None
+
+
+class ExpertMM(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, value, weight, plan):
+        from .expert_mm import _expert_mm
+
+        y, ctx.seglen = _expert_mm(value, weight, plan)
+        ctx.made_on = _lib.stream()
+        _save_some(ctx, value, weight)
+        where = _lib.caller_device(value, weight)
+        _made_here(ctx, where)
+        return _lib.hand_back(y, where)
+
+    @staticmethod
+    @once_differentiable
+    @_where_made
+    def backward(ctx, grad):
+        from .expert_mm import _expert_mm_grad
+
+        value, weight = _saved_some(ctx)
+        _lib.used_here(ctx.made_on, ctx.seglen)
+        dx, dw = _expert_mm_grad(value, weight, ctx.seglen, grad, ctx.needs_input_grad[:2])
+        return _back(dx, value), _back(dw, weight), None
 
 
 class CombineRows(torch.autograd.Function):

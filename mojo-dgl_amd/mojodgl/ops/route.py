@@ -1,14 +1,14 @@
 """Routing rows to experts, and the rows' way there and back (no counterpart in
-the reference): what chooses the block of `gather_mm` / `segment_mm` for each
+the reference): what chooses the block of `expert_mm` / `segment_mm` for each
 row, and puts the rows in that order.
 
     weights, ids = topk_route(logits, k)
     plan = route_plan(ids, num_experts)
-    y = combine_rows(segment_mm(dispatch_rows(x, plan), w, plan.seglen), weights, plan)
+    y = combine_rows(expert_mm(dispatch_rows(x, plan), w, plan), weights, plan)
 
 Rows keep float32, float64, bfloat16 or float16; weights and sums are float32
-(float64 for float64 rows). segment_mm takes 16-bit rows as float32 and returns
-float32: `.to(x.dtype)` behind it keeps such a layer's rows in their type.
+(float64 for float64 rows). (segment_mm, with ``plan.seglen``, takes 16-bit rows as
+float32, returns float32 and waits on the host for the lengths.)
 """
 
 from __future__ import annotations
@@ -20,6 +20,7 @@ import torch
 from .. import _lib
 from ..base import DGLError
 from . import _autograd
+from .quant import Quantized
 
 __all__ = ["RoutePlan", "topk_route", "route_plan", "dispatch_rows", "combine_rows"]
 
@@ -184,22 +185,29 @@ def dispatch_rows(value, plan):
 
     Parameters
     ----------
-    value : (N, ...) array or tensor
+    value : (N, ...) array or tensor, or `Quantized` rows, whose values and scales
+        are both copied
     plan : the `RoutePlan` of the N rows
 
     Returns
     -------
-    (N * k, ...) rows in the experts' order, for `segment_mm` with
-    ``plan.seglen``; zeros for entries of no expert. With a torch tensor that
-    requires grad the result takes part in autograd.
+    (N * k, ...) rows in the experts' order, for `expert_mm` or `scaled_mm` with the
+    plan, or `segment_mm` with ``plan.seglen``; zeros for entries of no expert. With a
+    torch tensor that requires grad the result takes part in autograd.
     """
+    if isinstance(value, Quantized):
+        if _autograd.needs_grad(*value):
+            raise DGLError("dispatch_rows has no gradient for quantized rows")
+        where = _lib.caller_device(*value)
+        return Quantized(*(_lib.hand_back(_dispatch_rows(t, plan), where) for t in value))
     if _autograd.needs_grad(value):
         return _autograd.DispatchRows.apply(value, plan)
     return _lib.hand_back(_dispatch_rows(value, plan), _lib.caller_device(value))
 
 
 def _dispatch_rows(value, plan):
-    x = _lib.rows(value)
+    bytes_ = isinstance(value, torch.Tensor) and value.dtype is torch.float8_e4m3fn
+    x = value if bytes_ else _lib.rows(value)
     if x.ndim < 1:
         raise DGLError("dispatch_rows wants rows, got a value without axes")
     _lib.device()
@@ -211,7 +219,7 @@ def _dispatch_rows(value, plan):
     out = torch.empty((n * k,) + tuple(shape[1:]), dtype=x.dtype, device=x.device)
     _lib.check(_lib.lib().mdgl_dispatch_rows(
         x.data_ptr(), plan.slot.data_ptr(), out.data_ptr(), n, k, math.prod(shape[1:]),
-        _lib.ROW_CODES[x.dtype], _lib.stream()), "dispatch_rows")
+        _lib.FLOAT8 if bytes_ else _lib.ROW_CODES[x.dtype], _lib.stream()), "dispatch_rows")
     return out
 
 

@@ -16,7 +16,11 @@ FLOAT, DOUBLE, BF16, F16 = "f", "d", "DF16b", "DF16_"
 KERNELS = {"rms_kernel": (FLOAT, DOUBLE, BF16, F16), "rms_grad_kernel": (FLOAT, DOUBLE, BF16, F16),
            "rms_wide_kernel": (FLOAT, DOUBLE, BF16, F16),
            "rms_cols_kernel": (FLOAT, DOUBLE, BF16, F16),
-           "quant_rows_kernel": (FLOAT, BF16, F16), "quant_blocks_kernel": (FLOAT, BF16, F16)}
+           "quant_rows_kernel": (FLOAT, BF16, F16), "quant_blocks_kernel": (FLOAT, BF16, F16),
+           "expert_mm_join_kernel": (FLOAT, BF16, F16), "expert_mm_sum_kernel": (BF16, F16),
+           # by a configuration, whose first argument is the type
+           "expert_mm_kernel": ("NS_6MmConfI" + BF16, "NS_6MmConfI" + F16, "NS_6MmConfINS_4f8_t"),
+           "expert_mm_grad_kernel": ("NS_6MmConfI" + BF16, "NS_6MmConfI" + F16)}
 
 
 @pytest.fixture(scope="module")
