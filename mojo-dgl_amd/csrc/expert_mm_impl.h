@@ -21,17 +21,18 @@
 // runs along the other axis (b as segment_mm has it; both operands of the gradient of
 // b) is kept as 64 rows, and read with the transposing LDS loads: 16 lanes read four
 // inner places of 16 columns and each gets the four values of its column; its pieces
-// of 64 bytes lie at piece ^ (row & 3).
+// of 32 bytes lie at piece ^ swizzle(row), so that the eight rows that 32 lanes read use
+// all banks.
 //
 // The product is formed transposed (b's values as the first operand), which leaves a
-// lane with four neighbouring columns of one row; two blocks of 16 columns are dealt
-// out so that a lane's two fours are eight neighbours: results leave in stores of 16
-// bytes.
+// lane with four neighbouring columns of one row; an exchange between lanes makes them
+// eight: results leave in stores of 16 bytes.
 //
 // Past the edges: rows past the tile's group and inner places past the end are read as
 // zeros by the buffer's own bounds check (a lane past the inner end is given an offset
 // behind the buffer), so no stage has a case of its own. Rows that start off a 16-byte
-// boundary (an odd width) go through registers instead, element by element at the ends.
+// boundary (an odd width) go through registers instead: a lane whose piece would pass its
+// row's end reads the last piece of the row and shifts it.
 //
 // Tiles are counted on the GPU from the experts' lengths, which the host need not know:
 // every wavefront walks them 64 experts at a time. A tile index in the order of the
@@ -58,7 +59,7 @@ typedef __attribute__((address_space(3))) char lds_char;
 struct f8_t { uint8_t v; };  // e4m3
 
 constexpr int MM_STAGE = 128;  // bytes of a row's inner axis a stage
-constexpr uint32_t MM_PAST = 0x80000000u;  // an offset behind every buffer
+constexpr uint32_t MM_PAST = 0x80000000u;  // this and more: an offset behind every buffer
 
 // ---------------------------------------------------------------- walking the experts
 
@@ -83,7 +84,7 @@ struct MmWalk {
   uint32_t rows, size;
   int base;                          // first group of the 64
   uint32_t rows_before, piece_before;  // in front of them
-  uint32_t start, end, first, last;  // a lane's group: its rows, its pieces
+  uint32_t end, last;  // a lane's group: where its rows and its pieces end
 
   __device__ __forceinline__ void init(const int64_t* lens, int n, int64_t m, uint32_t piece) {
     seglen = lens;
@@ -95,7 +96,9 @@ struct MmWalk {
     load();
   }
   __device__ __forceinline__ void load() {
-    const int g = base + (int)(threadIdx.x % WAVE);
+    int lane = threadIdx.x % WAVE;
+    asm volatile("" : "+v"(lane));  // its address is formed here, not held all along
+    const int g = base + lane;
     uint32_t len = 0;
     if (g < groups) {
       // lengths that do not fit the rows are cut: every access stays in bounds
@@ -106,11 +109,10 @@ struct MmWalk {
     }
     const uint32_t sum = __builtin_elementwise_add_sat(rows_before, mm_scan(len));
     end = sum < rows ? sum : rows;
-    start = sum - len < rows ? sum - len : rows;
+    const uint32_t start = sum - len < rows ? sum - len : rows;
     uint32_t pieces = (end - start) / size + ((end - start) % size != 0);
     if (!REST && g < groups && pieces == 0) pieces = 1;
     last = piece_before + mm_scan(pieces);
-    first = last - pieces;
   }
   // The next 64 groups; false behind the last.
   __device__ __forceinline__ bool next() {
@@ -134,14 +136,17 @@ struct MmWalk {
                                        uint32_t* p0, uint32_t* p1) {
     while (piece >= (uint32_t)readlane_int((int)last, WAVE - 1))
       if (!next()) return false;
-    const uint64_t at = __ballot(piece >= first && piece < last);
-    const int lane = __builtin_ctzll(at);
+    const int lane = __builtin_ctzll(__ballot(piece < last));
     *group = base + lane;
-    *s = (uint32_t)readlane_int((int)start, lane);
-    *e = (uint32_t)readlane_int((int)end, lane);
-    *p0 = (uint32_t)readlane_int((int)first, lane);
-    *p1 = (uint32_t)readlane_int((int)last, lane);
+    bounds(lane, s, e, p0, p1);
     return true;
+  }
+  __device__ __forceinline__ void bounds(int lane, uint32_t* s, uint32_t* e, uint32_t* p0,
+                                         uint32_t* p1) const {
+    *s = lane ? (uint32_t)readlane_int((int)end, lane - 1) : rows_before;
+    *e = (uint32_t)readlane_int((int)end, lane);
+    *p0 = lane ? (uint32_t)readlane_int((int)last, lane - 1) : piece_before;
+    *p1 = (uint32_t)readlane_int((int)last, lane);
   }
 };
 
@@ -196,23 +201,35 @@ __device__ __forceinline__ void mm_load4(mm_i32x4 buf, uint32_t off, uint32_t ld
                : "m0");
 }
 
-// The first `left` bytes of the 16 at p (of values of SIZE bytes), zeros behind them.
+// 16 bytes at p, which lie on a boundary of SIZE.
 template <int SIZE>
-__device__ __forceinline__ mm_i32x4 mm_read16(const char* p, int64_t left) {
+__device__ __forceinline__ mm_i32x4 mm_read16(const char* p) {
+  using U = std::conditional_t<SIZE == 2, uint16_t, uint8_t>;
+  U raw[16 / SIZE];
+  mm_i32x4 v;
+  load_any<false>(reinterpret_cast<const U*>(p), raw);
+  __builtin_memcpy(&v, raw, 16);
+  return v;
+}
+// The first `left` bytes at p, fewer than 16, one value after the other.
+template <int SIZE>
+__device__ __forceinline__ mm_i32x4 mm_read_some(const char* p, int64_t left) {
   using U = std::conditional_t<SIZE == 2, uint16_t, uint8_t>;
   mm_i32x4 v = {0, 0, 0, 0};
-  if (left >= 16) {
-    U raw[16 / SIZE];
-    load_any<false>(reinterpret_cast<const U*>(p), raw);
-    __builtin_memcpy(&v, raw, 16);
-  } else if (left > 0) {
 #pragma unroll
-    for (int i = 0; i < 16; i += SIZE) {
-      if (i >= left) continue;
-      v[i / 4] |= (int)((uint32_t)*reinterpret_cast<const U*>(p + i) << 8 * (i % 4));
-    }
-  }
+  for (int i = 0; i < 16; i += SIZE)
+    if (i < left) v[i / 4] |= (int)((uint32_t)*reinterpret_cast<const U*>(p + i) << 8 * (i % 4));
   return v;
+}
+// Without the first n bytes (all of them from 16 on), zeros behind.
+__device__ __forceinline__ mm_i32x4 mm_skip(mm_i32x4 v, int64_t n) {
+  typedef uint64_t V __attribute__((ext_vector_type(2)));
+  V x = __builtin_bit_cast(V, v);
+  const uint64_t lo = n >= 8 ? x[1] : x[0], hi = n >= 8 ? 0 : x[1];
+  const int s = (int)(n * 8) & 63;
+  x[0] = n >= 16 ? 0 : lo >> s | hi << 1 << (63 - s);
+  x[1] = n >= 16 ? 0 : hi >> s;
+  return __builtin_bit_cast(mm_i32x4, x);
 }
 
 // At most `n` of the wavefront's loads to LDS outstanding, and none of its LDS reads,
@@ -226,8 +243,7 @@ __device__ __forceinline__ void mm_wait() {
 }
 
 // An operand whose inner axis is contiguous: ROWS rows of a stage's 128 bytes.
-// SECOND: the operand whose rows are dealt out to lanes in fours of eight (b).
-template <int ROWS, int THREADS, int SIZE, bool SECOND, bool DIRECT>
+template <int ROWS, int THREADS, int SIZE, bool DIRECT>
 struct MmAlong {
   static constexpr int BYTES = ROWS * MM_STAGE;
   static constexpr int PIECES = ROWS * 8;
@@ -240,10 +256,9 @@ struct MmAlong {
   uint32_t stride;    // bytes of a row
   int col;            // bytes to its place in a row
   int row, live;
+  uint32_t first, from;  // of the stage being loaded: its place in a row, its offset
 
-  __device__ static __forceinline__ int swizzle(int r) {
-    return SECOND ? (r & 3) | (r >> 1 & 4) : r & 7;
-  }
+  __device__ static __forceinline__ int swizzle(int r) { return r & 7; }
   __device__ __forceinline__ void init(uint32_t row_bytes) {
     // with fewer pieces than threads some wavefronts load the same ones again
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE) % (PIECES / WAVE);
@@ -260,34 +275,45 @@ struct MmAlong {
     p = from;
     if constexpr (DIRECT) buf = mm_buffer(from, (int64_t)live * stride);
   }
-  __device__ __forceinline__ void issue(uint32_t at, uint32_t stage) {
-    const uint32_t in = stage * MM_STAGE;
+  // No tile: its loads give zeros.
+  __device__ __forceinline__ void none() { buf[2] = 0; }
+  __device__ __forceinline__ void begin(uint32_t stage) {
+    first = stage * MM_STAGE + (uint32_t)col;
+    from = first < stride ? off + stage * MM_STAGE : MM_PAST;
+  }
+  __device__ __forceinline__ void load(uint32_t at, int i) {
     if constexpr (DIRECT) {
-      const uint32_t o = in + (uint32_t)col < stride ? off + in : MM_PAST;
-      const uint32_t more = in + (uint32_t)col < stride ? STEP * stride : 0;
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) mm_load16(buf, o + i * more, at + lds + i * (THREADS * 16));
+      mm_load16(buf, from + i * (STEP * stride), at + lds + i * (THREADS * 16));
     } else {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int r = row + i * STEP;
-        held[i] = mm_read16<SIZE>(p + (int64_t)r * stride + in + col,
-                                  r < live ? (int64_t)stride - in - col : 0);
+      const int r = row + i * STEP;
+      if (stride >= 16) {
+        // the piece that ends with the row in place of one that would pass its end, and
+        // the last row in place of those behind it: no lane waits for another's branch
+        held[i] = mm_read16<SIZE>(p + (int64_t)(r < live ? r : live - 1) * stride +
+                                  (first < stride - 16 ? first : stride - 16));
+      } else {
+        held[i] = mm_read_some<SIZE>(p + (int64_t)r * stride + first,
+                                     r < live ? (int64_t)stride - first : 0);
       }
     }
   }
   __device__ __forceinline__ void commit(uint32_t at) {
+    const int64_t behind = stride >= 16 ? (int64_t)first - ((int64_t)stride - 16) : 0;
+    const bool end = first - col + MM_STAGE > stride;  // uniform
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i)
+    for (int i = 0; i < LOADS; ++i) {
+      if (end && behind > 0) held[i] = mm_skip(held[i], behind);
+      if (row + i * STEP >= live) held[i] = mm_i32x4{0, 0, 0, 0};
       *(__attribute__((address_space(3))) mm_i32x4*)(lds_char*)(uintptr_t)(
           at + lds + (threadIdx.x % WAVE) * 16 + i * (THREADS * 16)) = held[i];
+    }
   }
-  // Where this lane reads its pieces of row block 0 of its wavefront: [kk] of 16 bits,
-  // [half] of 8.
-  __device__ static __forceinline__ uint32_t read_at(int piece) {
-    const int l = threadIdx.x % 16;
-    const int r = SECOND ? 8 * (l / 4) + l % 4 : l;
-    return (uint32_t)(r * MM_STAGE + ((piece ^ swizzle(r)) * 16));
+  // Where this lane reads piece `first` of its row of a block of 16; the pieces
+  // 4 (of 16 bits) and 1 (of 8) behind it lie at the place xor 64 and 16, as stages start on
+  // multiples of 256.
+  __device__ static __forceinline__ uint32_t read_at(int first) {
+    const int r = threadIdx.x % 16;
+    return (uint32_t)(r * MM_STAGE + ((first ^ swizzle(r)) * 16));
   }
 };
 
@@ -299,22 +325,24 @@ struct MmAcross {
   static constexpr int PER = COLS / 8;  // pieces a row
   static constexpr int LOADS = 64 * PER / THREADS;
   static constexpr int STEP = THREADS / PER;
-  static_assert(STEP % 4 == 0 && COLS >= 64, "");
+  static_assert(STEP % 16 == 0 && COLS >= 128, "");
   mm_i32x4 buf;
   const char* p;
   mm_i32x4 held[DIRECT ? 1 : LOADS];
   uint32_t off, lds, stride;
   int row, col;
+  const char* from;  // of the stage being loaded: its first place,
+  int places;        // and how many it has
   int64_t left;   // inner places from the tile's first on
   int64_t width;  // bytes of a row from the tile's first column on
 
-  __device__ static __forceinline__ int swizzle(int r) { return COLS >= 128 ? r & 3 : r & 1; }
+  __device__ static __forceinline__ int swizzle(int r) { return (r & 3) | (r >> 1 & 4); }
   __device__ __forceinline__ void init(uint32_t row_bytes) {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
     const int piece = wave * WAVE + (int)(threadIdx.x % WAVE);
     row = piece / PER;
     const int at = piece % PER;
-    col = (((at >> 2) ^ swizzle(row)) * 4 + (at & 3)) * 16;
+    col = (((at >> 1) ^ swizzle(row)) * 2 + (at & 1)) * 16;
     stride = row_bytes;
     off = (uint32_t)row * stride + (uint32_t)col;
     lds = (uint32_t)wave * (WAVE * 16);
@@ -325,53 +353,61 @@ struct MmAcross {
     left = places;
     width = columns;
   }
-  __device__ __forceinline__ void issue(uint32_t at, uint32_t stage) {
+  __device__ __forceinline__ void none() { left = width = 0; }
+  __device__ __forceinline__ void begin(uint32_t stage) {
     const int64_t first = (int64_t)stage * 64;
-    const char* from = p + first * stride;
+    from = p + first * stride;
+    places = left - first < 64 ? (int)(left - first) : 64;
+    // columns past the width hold what follows in memory: they meet only results that are
+    // not written
+    if constexpr (DIRECT) buf = mm_buffer(from, (left - first - 1) * stride + width);
+  }
+  __device__ __forceinline__ void load(uint32_t at, int i) {
     if constexpr (DIRECT) {
-      // columns past the width hold what follows in memory: they meet only results
-      // that are not written
-      buf = mm_buffer(from, (left - first - 1) * stride + width);
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i)
-        mm_load16(buf, off + i * (STEP * stride), at + lds + i * (THREADS * 16));
+      mm_load16(buf, off + i * (STEP * stride), at + lds + i * (THREADS * 16));
     } else {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int r = row + i * STEP;
-        held[i] = mm_read16<2>(from + (int64_t)r * stride + col, first + r < left ? width - col : 0);
-      }
+      const int r = row + i * STEP;
+      if (stride >= 16)  // as in MmAlong
+        held[i] = mm_read16<2>(from + (int64_t)(r < places ? r : places - 1) * stride +
+                               (col < width - 16 ? col : width - 16));
+      else
+        held[i] = mm_read_some<2>(from + (int64_t)r * stride + col, r < places ? width - col : 0);
     }
   }
   __device__ __forceinline__ void commit(uint32_t at) {
+    const int64_t behind = stride >= 16 ? col - (width - 16) : 0;
+    const bool end = width < ROW;  // uniform
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i)
+    for (int i = 0; i < LOADS; ++i) {
+      if (end && behind > 0) held[i] = mm_skip(held[i], behind);
+      if (row + i * STEP >= places) held[i] = mm_i32x4{0, 0, 0, 0};
       *(__attribute__((address_space(3))) mm_i32x4*)(lds_char*)(uintptr_t)(
           at + lds + (threadIdx.x % WAVE) * 16 + i * (THREADS * 16)) = held[i];
+    }
   }
-  // Where this lane reads block `unit` of 32 columns: inner places 8 q + l / 4. FOURS:
-  // the lane's four columns of eight (b), else 16 columns after one another.
-  template <bool FOURS>
+  // Where this lane reads block `unit` of 16 columns, inner places 8 q + l / 4; block
+  // unit + n, n below the power of two that divides `unit`, lies at the place xor 32 n.
   __device__ static __forceinline__ uint32_t read_at(int unit) {
     const int l = threadIdx.x % 16, q = threadIdx.x % WAVE / 16, r = 8 * q + l / 4;
-    return (uint32_t)(r * ROW + (unit ^ swizzle(r)) * 64 + (l % 4) * (FOURS ? 16 : 8));
+    return (uint32_t)(r * ROW + (unit ^ swizzle(r)) * 32 + (l % 4) * 8);
   }
 };
 
 // ---------------------------------------------------------------- operands and products
 
-__device__ __forceinline__ mm_i32x4 mm_lds16(uint32_t at) {
-  return *(__attribute__((address_space(3))) mm_i32x4*)(lds_char*)(uintptr_t)at;
+// `more` is a constant: as a pointer's offset it goes into the instruction.
+__device__ __forceinline__ mm_i32x4 mm_lds16(uint32_t at, int more) {
+  return *(__attribute__((address_space(3))) mm_i32x4*)((lds_char*)(uintptr_t)at + more);
 }
-__device__ __forceinline__ float mm_lds4(uint32_t at) {
-  return *(__attribute__((address_space(3))) float*)(lds_char*)(uintptr_t)at;
+__device__ __forceinline__ float mm_lds4(uint32_t at, int more) {
+  return *(__attribute__((address_space(3))) float*)((lds_char*)(uintptr_t)at + more);
 }
 // Eight inner places of this lane's column: two transposing loads, four rows apart.
-__device__ __forceinline__ mm_i32x4 mm_lds_turned(uint32_t at, uint32_t four_rows) {
+__device__ __forceinline__ mm_i32x4 mm_lds_turned(uint32_t at, int more, int four_rows) {
   typedef __attribute__((address_space(3))) mm_i16x4 L;
-  const mm_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(lds_char*)(uintptr_t)at);
-  const mm_i16x4 hi =
-      __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(lds_char*)(uintptr_t)(at + four_rows));
+  lds_char* p = (lds_char*)(uintptr_t)at + more;
+  const mm_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)p);
+  const mm_i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(p + four_rows));
   return __builtin_bit_cast(mm_i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
@@ -398,33 +434,41 @@ __device__ __forceinline__ mm_f32x4 mm_mul8(mm_i32x8 x, mm_i32x8 y) {
 }
 
 // The sums of a wavefront's MI by NJ blocks (lane: row l % 16, columns 4 (l / 16) ..)
-// written from (row, n) on, rows below `end`, columns below N.
+// written from (row, n) on, rows below `end`, columns below N. Two blocks of columns
+// exchange fours between neighbouring rows of 16 lanes, which leaves a lane with eight
+// columns in a row.
 template <int MI, int NJ, class O>
 __device__ __forceinline__ void mm_write(const mm_f32x4 (&acc)[MI][NJ], O* out, int64_t row,
                                          int64_t end, int64_t n, int64_t N) {
   const int l = threadIdx.x % 16, q = threadIdx.x % WAVE / 16;
+  const int64_t c = n + (q & 1) * 16 + (q >> 1) * 8;
+  O* to = out + (row + l) * N + c;
+  const int rows = (int)(end - row < MI * 16 ? end - row : MI * 16);
+  const int cols = (int)(N - c < NJ * 16 ? N - c : NJ * 16);
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    const int64_t r = row + i * 16 + l;
-    if (r >= end) continue;
 #pragma unroll
     for (int j = 0; j < NJ; j += 2) {
-      const int64_t c = n + j * 16 + q * 8;
-      O* to = out + r * N + c;
       float v[8];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        v[k] = acc[i][j][k];
-        v[k + 4] = acc[i][j + 1][k];
+        const auto both = __builtin_amdgcn_permlane16_swap(
+            __float_as_uint(acc[i][j][k]), __float_as_uint(acc[i][j + 1][k]), false, false);
+        v[k] = __uint_as_float(both[0]);
+        v[k + 4] = __uint_as_float(both[1]);
       }
-      if (c + 8 <= N) {
-        store_acc<O, float, 8>(to, v);
+      if (l + i * 16 >= rows) continue;
+      if (j * 16 + 8 <= cols) {
+        store_acc<O, float, 8>(to + j * 16, v);
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (c + k < N) to[k] = (O)v[k];
+          if (j * 16 + k < cols) to[j * 16 + k] = (O)v[k];
       }
     }
+    to += 16 * N;
+    // one row block's values and addresses at a time: the registers are full
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -435,6 +479,152 @@ __device__ __forceinline__ void mm_zero(mm_f32x4 (&acc)[MI][NJ]) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
+
+// What a wavefront multiplies of half a stage in 16 bits, and its products.
+template <int MI, int NJ>
+struct MmHalf {
+  mm_i32x4 x[MI], y[NJ];
+};
+// Among them, in this order: read(0 .. MI + NJ - 1), the next half from LDS, over the first
+// three quarters, and load(0 .. LOADS - 1), a stage from memory, over all. The memory
+// pipeline takes a load to LDS every 16 cycles and LDS a read every 4, and a wavefront
+// that issues its own one behind the other, as all do behind a barrier, multiplies nothing
+// meanwhile; left to itself the compiler puts reads right in front of the wait for them.
+template <class E, int LOADS, int MI, int NJ, class Read, class Load>
+__device__ __forceinline__ void mm_half(const MmHalf<MI, NJ>& f, mm_f32x4 (&acc)[MI][NJ],
+                                        Read read, Load load) {
+  constexpr int N = MI * NJ, READS = MI + NJ;
+#pragma unroll
+  for (int m = 0; m < N; ++m) {
+#pragma unroll
+    for (int k = 0; k < READS; ++k)
+      if (k * N * 3 / 4 / READS == m) read(k);
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k)
+      if (k * N / (LOADS ? LOADS : 1) == m) load(k);
+    __builtin_amdgcn_sched_barrier(0);
+    acc[m / NJ][m % NJ] = mm_mul(E{}, f.y[m % NJ], f.x[m / NJ], acc[m / NJ][m % NJ]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// What a wavefront has of a stage in 8 bits: values and the rows' scales.
+template <int MI, int NJ>
+struct MmHalf8 {
+  static constexpr int W = 4;  // row blocks
+  mm_i32x8 x[W], y[NJ];
+  float s[W];
+};
+
+// The ring of stages in LDS. While one half of a stage is multiplied the next half is
+// read from LDS: the second half of the stage, then the first of the next one. Between
+// the two the wavefronts meet, once a stage: the next stage is there, and nobody reads
+// the one whose second half all have in registers, so its place is filled again.
+// Behind the last stage of the last tile it goes on with loads of nothing, so that as
+// many are outstanding at every wait. `Loader`: begin(), load(place, i) for its LOADS loads,
+// end(place).
+template <int ST, int BYTES, bool DIRECT, class Loader>
+struct MmRing {
+  Loader& loader;
+  uint32_t base;
+  uint32_t use = 0;     // the place of the stage
+  bool stored = false;  // STORES stores are newer than all loads
+
+  // All but the `N` newest loads are there, and all LDS reads; all wavefronts are here. The
+  // stores of a tile's results need not have ended.
+  template <int N, int STORES>
+  __device__ __forceinline__ void wait() {
+    if (DIRECT && stored) mm_wait<N + STORES>();
+    else mm_wait<DIRECT ? N : 0>();
+    stored = false;
+  }
+  template <class Read>
+  __device__ __forceinline__ void start(Read first) {
+#pragma unroll
+    for (int i = 0; i < ST; ++i) {
+      if (i) loader.end(base + (i - 1) * BYTES);
+      loader.begin();
+#pragma unroll
+      for (int k = 0; k < Loader::LOADS; ++k) loader.load(base + i * BYTES, k);
+    }
+    mm_wait<DIRECT ? (ST - 1) * Loader::LOADS : 0>();
+    first(base);
+  }
+  // The place before `use`: its loads are the newest.
+  __device__ __forceinline__ uint32_t newest() const {
+    return base + (use ? use - 1 : ST - 1) * BYTES;
+  }
+  // A stage in 16 bits. read(half, place, h, k): part k of half h.
+  template <class E, int MI, int NJ, class Read>
+  __device__ __forceinline__ void step(E, MmHalf<MI, NJ>& f0, MmHalf<MI, NJ>& f1,
+                                       mm_f32x4 (&acc)[MI][NJ], Read read) {
+    const uint32_t at = base + use * BYTES, loaded = newest();
+    use = use + 1 == ST ? 0 : use + 1;
+    const uint32_t next = base + use * BYTES;
+    mm_half<E, 0>(f0, acc, [&](int k) { read(f1, at, 1, k); }, [](int) {});
+    loader.end(loaded);
+    loader.begin();
+    wait<(ST - 2) * Loader::LOADS, MI * NJ / 2>();
+    mm_half<E, Loader::LOADS>(f1, acc, [&](int k) { read(f0, next, 0, k); },
+                              [&](int k) { loader.load(at, k); });
+  }
+  // A stage in 8 bits, row block by row block: at most four of them are in registers, and
+  // a block's place takes the fourth behind it, of this stage or the next; y takes the
+  // next stage's values behind its last use. The wavefronts meet behind block MEET, when
+  // all of the stage is in registers. A product is scaled and added while the one behind it
+  // is formed.
+  template <int MI, int NJ, class ReadX, class ReadY>
+  __device__ __forceinline__ void step8(MmHalf8<MI, NJ>& f, mm_f32x4 (&acc)[MI][NJ], float sb,
+                                        ReadX read_x, ReadY read_y) {
+    constexpr int W = MmHalf8<MI, NJ>::W, MEET = MI == 8 ? 4 : 1, N = (MI - 1 - MEET) * NJ;
+    static_assert(MI == 8 || MI == 4, "");
+    const uint32_t at = base + use * BYTES, loaded = newest();
+    use = use + 1 == ST ? 0 : use + 1;
+    const uint32_t next = base + use * BYTES;
+    mm_f32x4 before;
+    float s = 0.0f;
+    auto add = [&](int i, int j, float by) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[i][j][k] = __builtin_fmaf(before[k], by, acc[i][j][k]);
+      // here and not behind the stage, where the compiler would move all of them
+      asm volatile("" : "+v"(acc[i][j]));
+      __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const float last = s;
+      s = sb * f.s[i % W];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int m = (i - 1 - MEET) * NJ + j;
+#pragma unroll
+        for (int k = 0; k < Loader::LOADS; ++k)
+          if (m >= 0 && k * N / Loader::LOADS == m) loader.load(at, k);
+        __builtin_amdgcn_sched_barrier(0);
+        const mm_f32x4 t = mm_mul8(f.y[j], f.x[i % W]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (j) add(i, j - 1, s);
+        else if (i) add(i - 1, NJ - 1, last);
+        before = t;
+        if (i == MI - 1) read_y(next, j);
+      }
+      if (i + W < MI) read_x(at, i + W);
+      if (i == MEET) {
+        loader.end(loaded);
+        loader.begin();
+        wait<(ST - 2) * Loader::LOADS, MI * NJ / 2>();
+#pragma unroll
+        for (int r = 0; r <= MEET; ++r)
+          if (r + W >= MI) read_x(next, r + W - MI);
+      } else if (i > MEET) {
+        read_x(next, i + W - MI);
+      }
+    }
+    add(MI - 1, NJ - 1, s);
+  }
+  // Nothing is left on its way to LDS.
+  __device__ __forceinline__ void finish() const { mm_wait<0>(); }
+};
 
 template <class E, int BM_, int BN_, int WM_, int WN_, int ST_, bool ALONG_, bool DIRECT_>
 struct MmConf {
@@ -448,8 +638,8 @@ struct MmConf {
   static constexpr bool EIGHT = sizeof(E) == 1;
   static constexpr int SIZE = (int)sizeof(E);
   static constexpr int INNER = MM_STAGE / SIZE;  // inner places a stage
-  using A = MmAlong<BM, THREADS, SIZE, false, DIRECT>;
-  using B = std::conditional_t<ALONG, MmAlong<BN, THREADS, SIZE, true, DIRECT>,
+  using A = MmAlong<BM, THREADS, SIZE, DIRECT>;
+  using B = std::conditional_t<ALONG, MmAlong<BN, THREADS, SIZE, DIRECT>,
                                MmAcross<BN, THREADS, DIRECT>>;
   static constexpr int SCALES = EIGHT ? (BM < WAVE ? WAVE : BM) * 4 : 0;
   static constexpr int STAGE_BYTES = A::BYTES + B::BYTES + SCALES;
@@ -477,6 +667,139 @@ struct MmArgs {
   int splits;     // parts of the inner axis, each a tile of its own
 };
 
+// A tile of results: rows [row, end) of its group (BM at most), columns from `col` on,
+// stages [stage0, stage1) of the inner axis.
+template <class C>
+struct MmTile {
+  MmWalk<true> walk;
+  MmOrder order;
+  int group, part, stage0, stage1;
+  uint32_t row, end, col;
+  bool any;
+
+  __device__ __forceinline__ void init(const MmArgs& p) {
+    walk.init(p.seglen, p.groups, p.rows, C::BM);
+    order.init(walk.total() * across(p) * p.splits);
+  }
+  __device__ static __forceinline__ uint32_t across(const MmArgs& p) {
+    return (uint32_t)((p.N + C::BN - 1) / C::BN);
+  }
+  __device__ __forceinline__ void seek(const MmArgs& p) {
+    any = false;
+    if (order.at >= order.end) return;
+    uint32_t s, p0, p1, i, j;
+    const uint32_t at = order.at / p.splits, wide = across(p);
+    part = (int)(order.at - at * p.splits);
+    order.at += order.step;
+    if (!walk.find(at / wide, &group, &s, &end, &p0, &p1)) return;
+    mm_band(at - p0 * wide, p1 - p0, wide, &i, &j);
+    const int stages = (p.K + C::INNER - 1) / C::INNER;
+    stage0 = (int)((int64_t)stages * part / p.splits);
+    // the rest has no inner axis
+    stage1 = group < p.groups ? (int)((int64_t)stages * (part + 1) / p.splits) : stage0;
+    row = s + i * C::BM;
+    col = j * C::BN;
+    any = true;
+  }
+};
+
+// The stages of a workgroup's tiles, one after the other, on their way to LDS.
+template <class C>
+struct MmSource {
+  static constexpr int LOADS = C::LOADS;
+  const MmArgs& p;
+  MmTile<C> tile;
+  typename C::A A;
+  typename C::B B;
+  int stage;
+  int64_t row_bytes;
+  // 8 bits: a row's scale a thread
+  mm_i32x4 scales;
+  uint32_t scale_off, scale_lds;
+  int scale_row, kb;
+  float scale_held;
+  float b_scale;  // of the tile's first 64 stages, one a lane
+
+  // b's scale of stage s + lane for the tile's columns of this wavefront.
+  __device__ static __forceinline__ float b_scales(const MmArgs& p, const MmTile<C>& t, int s) {
+    const int kb = (p.K + 127) / 128, nb = (p.N + 127) / 128;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
+    const int c = ((int)t.col + wave % C::WN * (C::BN / C::WN)) / 128;
+    const int k = s + (int)(threadIdx.x % WAVE);
+    return k < kb ? p.sb[((int64_t)t.group * kb + k) * nb + (c < nb ? c : nb - 1)] : 0.0f;
+  }
+  __device__ __forceinline__ void init(const MmTile<C>& first) {
+    tile = first;
+    row_bytes = (int64_t)p.K * C::SIZE;
+    A.init((uint32_t)row_bytes);
+    B.init(C::ALONG ? (uint32_t)row_bytes : (uint32_t)p.N * 2);
+    if constexpr (C::EIGHT) {
+      const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
+      const int part = wave % (C::SCALES / 256);
+      kb = (p.K + 127) / 128;
+      scale_row = part * WAVE + (int)(threadIdx.x % WAVE);
+      scale_off = (uint32_t)scale_row * kb * 4;
+      scale_lds = C::A::BYTES + C::B::BYTES + part * 256;
+    }
+    open();
+  }
+  __device__ __forceinline__ void open() {
+    do tile.seek(p);
+    while (tile.any && tile.stage0 == tile.stage1);
+    stage = tile.stage0;
+    if (!tile.any) {
+      A.none();
+      B.none();
+      if constexpr (C::EIGHT) scales[2] = 0;
+      return;
+    }
+    const int rows = (int)(tile.end - tile.row);
+    A.tile(p.a + tile.row * row_bytes, rows);
+    const char* block = p.b + tile.group * (row_bytes * p.N);
+    if constexpr (C::ALONG) {
+      B.tile(block + tile.col * row_bytes, p.N - (int)tile.col);
+    } else {
+      B.tile(block + (int64_t)tile.col * 2, p.K, (int64_t)(p.N - (int)tile.col) * 2);
+    }
+    if constexpr (C::EIGHT) {
+      scales = mm_buffer((const char*)(p.sa + (int64_t)tile.row * kb),
+                         (int64_t)(rows < C::BM ? rows : C::BM) * kb * 4);
+      b_scale = b_scales(p, tile, tile.stage0);
+    }
+  }
+  __device__ __forceinline__ void begin() {
+    A.begin(stage);
+    B.begin(stage);
+  }
+  __device__ __forceinline__ void load(uint32_t at, int i) {
+    if (!C::DIRECT && !tile.any) return;
+    if (i < C::A::LOADS) {
+      A.load(at, i);
+    } else if (i < C::A::LOADS + C::B::LOADS) {
+      B.load(at + C::A::BYTES, i - C::A::LOADS);
+    } else if constexpr (C::EIGHT) {
+      if constexpr (C::DIRECT) {
+        mm_load4(scales, scale_off + stage * 4, at + scale_lds);
+      } else {
+        const int rows = (int)(tile.end - tile.row);
+        scale_held = scale_row < (rows < C::BM ? rows : C::BM)
+                         ? p.sa[(int64_t)(tile.row + scale_row) * kb + stage] : 0.0f;
+      }
+    }
+  }
+  __device__ __forceinline__ void end(uint32_t at) {
+    if (!tile.any) return;
+    if constexpr (!C::DIRECT) {
+      A.commit(at);
+      B.commit(at + C::A::BYTES);
+      if constexpr (C::EIGHT)
+        *(__attribute__((address_space(3))) float*)(lds_char*)(uintptr_t)(
+            at + scale_lds + (threadIdx.x % WAVE) * 4) = scale_held;
+    }
+    if (++stage == tile.stage1) open();
+  }
+};
+
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_kernel(MmArgs p) {
   using E = typename C::Elem;
@@ -485,199 +808,29 @@ __global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_kernel(MmArgs 
       (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(lds_char*)lds);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
   const int wm = wave / C::WN, wn = wave % C::WN;
-  const int l = threadIdx.x % 16, q = threadIdx.x % WAVE / 16;
-  const int64_t row_bytes = (int64_t)p.K * C::SIZE;
-  const uint32_t across = (uint32_t)((p.N + C::BN - 1) / C::BN);
-  const int stages = (p.K + C::INNER - 1) / C::INNER;
-
-  struct Tile {
-    MmWalk<true> walk;
-    MmOrder order;
-    int group, part, stage0, stage1;
-    uint32_t row, end, col;
-    bool any;
-  };
-  auto seek = [&](Tile& t) {
-    t.any = false;
-    if (t.order.at >= t.order.end) return;
-    uint32_t s, e, p0, p1, i, j;
-    const uint32_t at = t.order.at / p.splits;
-    t.part = (int)(t.order.at - at * p.splits);
-    t.order.at += t.order.step;
-    if (!t.walk.find(at / across, &t.group, &s, &e, &p0, &p1)) return;
-    mm_band(at - p0 * across, p1 - p0, across, &i, &j);
-    t.stage0 = (int)((int64_t)stages * t.part / p.splits);
-    // the rest has no inner axis
-    t.stage1 = t.group < p.groups ? (int)((int64_t)stages * (t.part + 1) / p.splits) : t.stage0;
-    t.row = s + i * C::BM;
-    t.end = e;
-    t.col = j * C::BN;
-    t.any = true;
-  };
-  Tile mine;  // what is multiplied
-  mine.walk.init(p.seglen, p.groups, p.rows, C::BM);
-  mine.order.init(mine.walk.total() * across * p.splits);
-  Tile ahead = mine;  // what is loaded
-
-  typename C::A A;
-  typename C::B B;
-  A.init((uint32_t)row_bytes);
-  B.init(C::ALONG ? (uint32_t)row_bytes : (uint32_t)p.N * 2);
-  [[maybe_unused]] mm_i32x4 scales;
-  [[maybe_unused]] uint32_t scale_off = 0, scale_lds = 0;
-  [[maybe_unused]] float scale_held = 0.0f;
-  const int kb = (p.K + 127) / 128, nb = (p.N + 127) / 128;
-  [[maybe_unused]] const int scale_row =
-      wave % (C::SCALES / 256 + !C::EIGHT) * WAVE + (int)(threadIdx.x % WAVE);
-  if constexpr (C::EIGHT) {
-    scale_off = (uint32_t)scale_row * kb * 4;
-    scale_lds = C::A::BYTES + C::B::BYTES + wave % (C::SCALES / 256) * 256;
-  }
-  int ahead_stage = 0;
-  auto open = [&]() {  // the tile to load from
-    do seek(ahead);
-    while (ahead.any && ahead.stage0 == ahead.stage1);
-    if (!ahead.any) return;
-    const int rows = (int)(ahead.end - ahead.row);
-    A.tile(p.a + ahead.row * row_bytes, rows);
-    const char* block = p.b + ahead.group * (row_bytes * p.N);
-    if constexpr (C::ALONG) {
-      B.tile(block + ahead.col * row_bytes, p.N - (int)ahead.col);
-    } else {
-      B.tile(block + (int64_t)ahead.col * 2, p.K, (int64_t)(p.N - (int)ahead.col) * 2);
-    }
-    if constexpr (C::EIGHT) {
-      const char* from = (const char*)(p.sa + (int64_t)ahead.row * kb);
-      scales = mm_buffer(from, (int64_t)(rows < C::BM ? rows : C::BM) * kb * 4);
-    }
-    ahead_stage = ahead.stage0;
-  };
-  uint32_t fill = 0, use = 0;  // places in the ring
-  auto issue = [&]() {
-    if (!ahead.any) return;
-    const uint32_t at = lds0 + fill * C::STAGE_BYTES;
-    A.issue(at, ahead_stage);
-    B.issue(at + C::A::BYTES, ahead_stage);
-    if constexpr (C::EIGHT) {
-      if constexpr (C::DIRECT) {
-        mm_load4(scales, scale_off + ahead_stage * 4, at + scale_lds);
-      } else {
-        const int rows = (int)(ahead.end - ahead.row);
-        scale_held = scale_row < (rows < C::BM ? rows : C::BM)
-                         ? p.sa[(int64_t)(ahead.row + scale_row) * kb + ahead_stage] : 0.0f;
-      }
-    }
-    if constexpr (C::DIRECT) {
-      fill = fill + 1 == C::ST ? 0 : fill + 1;
-      if (++ahead_stage == ahead.stage1) open();
-    }
-  };
-  // through registers: what was issued before goes to LDS behind the products
-  auto commit = [&]() {
-    if constexpr (!C::DIRECT) {
-      if (!ahead.any) return;
-      const uint32_t at = lds0 + fill * C::STAGE_BYTES;
-      A.commit(at);
-      B.commit(at + C::A::BYTES);
-      if constexpr (C::EIGHT)
-        *(__attribute__((address_space(3))) float*)(lds_char*)(uintptr_t)(
-            at + scale_lds + (threadIdx.x % WAVE) * 4) = scale_held;
-      fill ^= 1;
-      if (++ahead_stage == ahead.stage1) open();
-    }
-  };
+  const int q = threadIdx.x % WAVE / 16;
 
   // what this lane reads, from a stage's start on
-  uint32_t a_at[2], b_at[C::ALONG ? 4 : C::NJ / 2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int piece = C::EIGHT ? 2 * q + h : 4 * h + q;
-    a_at[h] = (uint32_t)(wm * (C::BM / C::WM) * MM_STAGE) + C::A::read_at(piece);
-    if constexpr (C::ALONG) {
-      const uint32_t at = (uint32_t)C::A::BYTES + wn * (C::BN / C::WN) * MM_STAGE;
-      b_at[h] = at + C::B::read_at(piece);
-      // the second four of eight: four rows on, whose swizzle does not change
-      b_at[h + 2] = b_at[h] + 4 * MM_STAGE;
-    }
-  }
-  if constexpr (!C::ALONG)
-#pragma unroll
-    for (int j = 0; j < C::NJ / 2; ++j)
-      b_at[j] = (uint32_t)C::A::BYTES +
-                C::B::template read_at<true>(wn * (C::BN / C::WN / 32) + j);
+  const uint32_t a_at = (uint32_t)(wm * (C::BM / C::WM) * MM_STAGE) +
+                        C::A::read_at(C::EIGHT ? 2 * q : q);
+  uint32_t b_at = C::A::BYTES;
+  if constexpr (C::ALONG)
+    b_at += wn * (C::BN / C::WN) * MM_STAGE + C::B::read_at(C::EIGHT ? 2 * q : q);
+  else
+    b_at += C::B::read_at(wn * C::NJ);
 
+  MmTile<C> mine;  // what is multiplied
+  mine.init(p);
+  MmSource<C> source{p};  // what is loaded
+  source.init(mine);
+  MmRing<C::ST, C::STAGE_BYTES, C::DIRECT, MmSource<C>> ring{source, lds0};
   mm_f32x4 acc[C::MI][C::NJ];
-  auto multiply = [&](uint32_t at, [[maybe_unused]] int stage) {
-    if constexpr (C::EIGHT) {
-      typedef const __attribute__((address_space(4))) float CF;
-      const int n = (int)mine.col + wn * (C::BN / C::WN);
-      const int c = n / 128 < nb ? n / 128 : nb - 1;
-      const float sb = *(CF*)(p.sb + ((int64_t)mine.group * kb + stage) * nb + c);
-      mm_i32x8 x[C::MI];
-      float s[C::MI];
-#pragma unroll
-      for (int i = 0; i < C::MI; ++i) {
-        const mm_i32x4 lo = mm_lds16(at + a_at[0] + i * 16 * MM_STAGE);
-        const mm_i32x4 hi = mm_lds16(at + a_at[1] + i * 16 * MM_STAGE);
-        x[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        s[i] = sb * mm_lds4(at + C::A::BYTES + C::B::BYTES +
-                            (wm * (C::BM / C::WM) + i * 16 + l) * 4);
-      }
-#pragma unroll
-      for (int j = 0; j < C::NJ; ++j) {
-        const uint32_t more = j / 2 * 32 * MM_STAGE;
-        const mm_i32x4 lo = mm_lds16(at + b_at[j % 2 * 2] + more);
-        const mm_i32x4 hi = mm_lds16(at + b_at[j % 2 * 2 + 1] + more);
-        const mm_i32x8 y = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-        for (int i = 0; i < C::MI; ++i) {
-          const mm_f32x4 t = mm_mul8(y, x[i]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            acc[i][j][k] = __builtin_fmaf(t[k], s[i], acc[i][j][k]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        mm_i32x4 x[C::MI], y[C::NJ];
-#pragma unroll
-        for (int i = 0; i < C::MI; ++i) x[i] = mm_lds16(at + a_at[h] + i * 16 * MM_STAGE);
-#pragma unroll
-        for (int j = 0; j < C::NJ; ++j) {
-          if constexpr (C::ALONG)
-            y[j] = mm_lds16(at + b_at[h + j % 2 * 2] + j / 2 * 32 * MM_STAGE);
-          else
-            y[j] = mm_lds_turned(at + b_at[j / 2] + j % 2 * 8 + h * 32 * C::B::ROW, 4 * C::B::ROW);
-        }
-#pragma unroll
-        for (int i = 0; i < C::MI; ++i)
-#pragma unroll
-          for (int j = 0; j < C::NJ; ++j) acc[i][j] = mm_mul(E{}, y[j], x[i], acc[i][j]);
-      }
-    }
-  };
-
-  open();
-  if constexpr (C::DIRECT) {
-    for (int i = 0; i < C::ST - 1; ++i) issue();
-  } else {
-    issue();
-    commit();
-  }
-  for (seek(mine); mine.any; seek(mine)) {
-    mm_zero(acc);
-    for (int s = mine.stage0; s < mine.stage1; ++s) {
-      // behind the last load fewer are outstanding than the ring holds
-      if (C::ST > 2 && ahead.any) mm_wait<(C::ST - 2) * C::LOADS>();
-      else mm_wait<0>();
-      issue();
-      multiply(lds0 + use * C::STAGE_BYTES, s);
-      commit();
-      use = use + 1 == C::ST ? 0 : use + 1;
-    }
+  auto write = [&]() {
     const int64_t row = (int64_t)mine.row + wm * (C::BM / C::WM);
     const int64_t n = (int64_t)mine.col + wn * (C::BN / C::WN);
+    // a whole tile of 16 bits is one store for every two blocks
+    ring.stored = p.splits == 1 && (!C::EIGHT || p.out_dtype != DT_F32) &&
+                  row + C::MI * 16 <= mine.end && n + C::NJ * 16 <= p.N;
     if (p.splits > 1) {
       mm_write(acc, p.part + mine.part * (p.rows * p.N), row, mine.end, n, p.N);
     } else if constexpr (C::EIGHT) {
@@ -687,7 +840,70 @@ __global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_kernel(MmArgs 
     } else {
       mm_write(acc, (E*)p.out, row, mine.end, n, p.N);
     }
+  };
+  if constexpr (C::EIGHT) {
+    MmHalf8<C::MI, C::NJ> f;
+    const uint32_t s_at = (uint32_t)C::A::BYTES + C::B::BYTES +
+                          (wm * (C::BM / C::WM) + threadIdx.x % 16) * 4;
+    auto read_x = [&](uint32_t at, int i) {
+      const mm_i32x4 lo = mm_lds16(at + a_at, i * 16 * MM_STAGE);
+      const mm_i32x4 hi = mm_lds16((at + a_at) ^ 16, i * 16 * MM_STAGE);
+      f.x[i % f.W] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      f.s[i % f.W] = mm_lds4(at + s_at, i * 16 * 4);
+    };
+    auto read_y = [&](uint32_t at, int j) {
+      const mm_i32x4 lo = mm_lds16(at + b_at, j * 16 * MM_STAGE);
+      const mm_i32x4 hi = mm_lds16((at + b_at) ^ 16, j * 16 * MM_STAGE);
+      f.y[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    ring.start([&](uint32_t at) {
+#pragma unroll
+      for (int i = 0; i < f.W; ++i) read_x(at, i);
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j) read_y(at, j);
+    });
+    for (mine.seek(p); mine.any; mine.seek(p)) {
+      mm_zero(acc);
+      // a tile of few stages may be written before the loads of another begin
+      const MmTile<C>& t = source.tile;
+      float sb = 0.0f;
+      if (t.any && t.group == mine.group && t.row == mine.row && t.col == mine.col &&
+          t.part == mine.part)
+        sb = source.b_scale;
+      else if (mine.stage0 < mine.stage1)
+        sb = source.b_scales(p, mine, mine.stage0);
+      for (int s = mine.stage0; s < mine.stage1; ++s) {
+        const int k = (s - mine.stage0) % WAVE;
+        if (k == 0 && s > mine.stage0) sb = source.b_scales(p, mine, s);
+        ring.step8(f, acc, readlane_val(sb, k), read_x, read_y);
+      }
+      write();
+    }
+  } else {
+    // half a stage: 32 inner places
+    using Half = MmHalf<C::MI, C::NJ>;
+    Half f0, f1;
+    auto read = [&](Half& f, uint32_t at, int h, int k) {
+      const int j = k - C::MI;
+      if (j < 0)
+        f.x[k] = mm_lds16((at + a_at) ^ h * 64, k * 16 * MM_STAGE);
+      else if constexpr (C::ALONG)
+        f.y[j] = mm_lds16((at + b_at) ^ h * 64, j * 16 * MM_STAGE);
+      else
+        f.y[j] = mm_lds_turned((at + b_at) ^ j * 32, h * 32 * C::B::ROW, 4 * C::B::ROW);
+    };
+    ring.start([&](uint32_t at) {
+#pragma unroll
+      for (int k = 0; k < C::MI + C::NJ; ++k) read(f0, at, 0, k);
+    });
+    for (mine.seek(p); mine.any; mine.seek(p)) {
+      mm_zero(acc);
+      for (int s = mine.stage0; s < mine.stage1; ++s)
+        ring.step(E{}, f0, f1, acc, read);
+      write();
+    }
   }
+  ring.finish();
 }
 
 // The parts of the inner axis added in order.
@@ -731,129 +947,126 @@ struct MmGradArgs {
 };
 
 template <class C>
-__global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_grad_kernel(MmGradArgs p) {
-  using E = typename C::Elem;
+struct MmGradTile {
+  MmWalk<false> walk;
+  MmOrder order;
+  int group, stages, rows;
+  uint32_t start, row, col, piece;  // first row of the piece; the tile's place
+  bool any, alone;
+
+  __device__ static __forceinline__ uint32_t down(const MmGradArgs& p) {
+    return (uint32_t)((p.D1 + C::BM - 1) / C::BM);
+  }
+  __device__ static __forceinline__ uint32_t across(const MmGradArgs& p) {
+    return (uint32_t)((p.D2 + C::BN - 1) / C::BN);
+  }
+  __device__ __forceinline__ void init(const MmGradArgs& p) {
+    walk.init(p.seglen, p.groups, p.rows, p.piece);
+    order.init(walk.total() * (down(p) * across(p)));
+  }
+  __device__ __forceinline__ void seek(const MmGradArgs& p) {
+    any = false;
+    if (order.at >= order.end) return;
+    uint32_t s, e, p0, p1, i, j;
+    const uint32_t at = order.at, tiles = down(p) * across(p);
+    order.at += order.step;
+    piece = at / tiles;
+    if (!walk.find(piece, &group, &s, &e, &p0, &p1)) return;
+    mm_band(at - piece * tiles, down(p), across(p), &i, &j);
+    start = s + (piece - p0) * p.piece;
+    rows = (int)(e - start < p.piece ? e - start : p.piece);
+    stages = (rows + 63) / 64;
+    row = i * C::BM;
+    col = j * C::BN;
+    alone = p1 - p0 == 1;
+    any = true;
+  }
+};
+
+template <class C>
+struct MmGradSource {
   using A = MmAcross<C::BM, C::THREADS, C::DIRECT>;
   using B = MmAcross<C::BN, C::THREADS, C::DIRECT>;
-  constexpr int BYTES = A::BYTES + B::BYTES, LOADS = A::LOADS + B::LOADS;
-  __shared__ __align__(256) char lds[C::ST * BYTES];
+  static constexpr int LOADS = A::LOADS + B::LOADS, BYTES = A::BYTES + B::BYTES;
+  const MmGradArgs& p;
+  MmGradTile<C> tile;
+  A a;
+  B b;
+  int stage;
+
+  __device__ __forceinline__ void init(const MmGradTile<C>& first) {
+    tile = first;
+    a.init((uint32_t)p.D1 * 2);
+    b.init((uint32_t)p.D2 * 2);
+    open();
+  }
+  __device__ __forceinline__ void open() {  // pieces without rows have nothing to load
+    do tile.seek(p);
+    while (tile.any && tile.stages == 0);
+    stage = 0;
+    if (!tile.any) {
+      a.none();
+      b.none();
+      return;
+    }
+    a.tile(p.a + ((int64_t)tile.start * p.D1 + tile.row) * 2, tile.rows,
+           (int64_t)(p.D1 - (int)tile.row) * 2);
+    b.tile(p.grad + ((int64_t)tile.start * p.D2 + tile.col) * 2, tile.rows,
+           (int64_t)(p.D2 - (int)tile.col) * 2);
+  }
+  __device__ __forceinline__ void begin() {
+    a.begin(stage);
+    b.begin(stage);
+  }
+  __device__ __forceinline__ void load(uint32_t at, int i) {
+    if (!C::DIRECT && !tile.any) return;
+    if (i < A::LOADS) a.load(at, i);
+    else b.load(at + A::BYTES, i - A::LOADS);
+  }
+  __device__ __forceinline__ void end(uint32_t at) {
+    if (!tile.any) return;
+    if constexpr (!C::DIRECT) {
+      a.commit(at);
+      b.commit(at + A::BYTES);
+    }
+    if (++stage == tile.stages) open();
+  }
+};
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_grad_kernel(MmGradArgs p) {
+  using E = typename C::Elem;
+  using S = MmGradSource<C>;
+  __shared__ __align__(256) char lds[C::ST * S::BYTES];
   const uint32_t lds0 =
       (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(lds_char*)lds);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
   const int wm = wave / C::WN, wn = wave % C::WN;
-  const uint32_t down = (uint32_t)((p.D1 + C::BM - 1) / C::BM);
-  const uint32_t across = (uint32_t)((p.D2 + C::BN - 1) / C::BN);
-
-  struct Tile {
-    MmWalk<false> walk;
-    MmOrder order;
-    int group;
-    uint32_t start, row, col, piece;  // first row of the piece; the tile's place
-    int stages, rows;
-    bool any, alone;
-  };
-  auto seek = [&](Tile& t) {
-    t.any = false;
-    if (t.order.at >= t.order.end) return;
-    uint32_t s, e, p0, p1, i, j;
-    const uint32_t at = t.order.at;
-    t.order.at += t.order.step;
-    t.piece = at / (down * across);
-    if (!t.walk.find(t.piece, &t.group, &s, &e, &p0, &p1)) return;
-    mm_band(at - t.piece * (down * across), down, across, &i, &j);
-    t.start = s + (t.piece - p0) * p.piece;
-    const uint32_t rows = e - t.start;
-    t.rows = (int)(rows < p.piece ? rows : p.piece);
-    t.stages = (t.rows + 63) / 64;
-    t.row = i * C::BM;
-    t.col = j * C::BN;
-    t.alone = p1 - p0 == 1;
-    t.any = true;
-  };
-  Tile mine;
-  mine.walk.init(p.seglen, p.groups, p.rows, p.piece);
-  mine.order.init(mine.walk.total() * (down * across));
-  Tile ahead = mine;
-
-  A la;
-  B lb;
-  la.init((uint32_t)p.D1 * 2);
-  lb.init((uint32_t)p.D2 * 2);
-  int ahead_stage = 0;
-  auto open = [&]() {  // pieces without rows have nothing to load
-    do seek(ahead);
-    while (ahead.any && ahead.stages == 0);
-    if (!ahead.any) return;
-    la.tile(p.a + ((int64_t)ahead.start * p.D1 + ahead.row) * 2, ahead.rows,
-            (int64_t)(p.D1 - (int)ahead.row) * 2);
-    lb.tile(p.grad + ((int64_t)ahead.start * p.D2 + ahead.col) * 2, ahead.rows,
-            (int64_t)(p.D2 - (int)ahead.col) * 2);
-    ahead_stage = 0;
-  };
-  uint32_t fill = 0, use = 0;
-  auto issue = [&]() {
-    if (!ahead.any) return;
-    const uint32_t at = lds0 + fill * BYTES;
-    la.issue(at, ahead_stage);
-    lb.issue(at + A::BYTES, ahead_stage);
-    if constexpr (C::DIRECT) {
-      fill = fill + 1 == C::ST ? 0 : fill + 1;
-      if (++ahead_stage == ahead.stages) open();
-    }
-  };
-  auto commit = [&]() {
-    if constexpr (!C::DIRECT) {
-      if (!ahead.any) return;
-      const uint32_t at = lds0 + fill * BYTES;
-      la.commit(at);
-      lb.commit(at + A::BYTES);
-      fill ^= 1;
-      if (++ahead_stage == ahead.stages) open();
-    }
+  const uint32_t a_at = S::A::read_at(wm * C::MI);
+  const uint32_t b_at = (uint32_t)S::A::BYTES + S::B::read_at(wn * C::NJ);
+  using Half = MmHalf<C::MI, C::NJ>;
+  Half f0, f1;
+  auto read = [&](Half& f, uint32_t at, int h, int k) {
+    const int j = k - C::MI;
+    if (j < 0)
+      f.x[k] = mm_lds_turned((at + a_at) ^ k * 32, h * 32 * S::A::ROW, 4 * S::A::ROW);
+    else
+      f.y[j] = mm_lds_turned((at + b_at) ^ j * 32, h * 32 * S::B::ROW, 4 * S::B::ROW);
   };
 
-  uint32_t a_at[C::MI / 2], b_at[C::NJ / 2];
-#pragma unroll
-  for (int i = 0; i < C::MI / 2; ++i)
-    a_at[i] = A::template read_at<false>(wm * (C::BM / C::WM / 32) + i);
-#pragma unroll
-  for (int j = 0; j < C::NJ / 2; ++j)
-    b_at[j] = (uint32_t)A::BYTES + B::template read_at<true>(wn * (C::BN / C::WN / 32) + j);
+  MmGradTile<C> mine;
+  mine.init(p);
+  S source{p};
+  source.init(mine);
+  MmRing<C::ST, S::BYTES, C::DIRECT, S> ring{source, lds0};
   mm_f32x4 acc[C::MI][C::NJ];
-  auto multiply = [&](uint32_t at) {
+  ring.start([&](uint32_t at) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      mm_i32x4 x[C::MI], y[C::NJ];
-#pragma unroll
-      for (int i = 0; i < C::MI; ++i)
-        x[i] = mm_lds_turned(at + a_at[i / 2] + i % 2 * 32 + h * 32 * A::ROW, 4 * A::ROW);
-#pragma unroll
-      for (int j = 0; j < C::NJ; ++j)
-        y[j] = mm_lds_turned(at + b_at[j / 2] + j % 2 * 8 + h * 32 * B::ROW, 4 * B::ROW);
-#pragma unroll
-      for (int i = 0; i < C::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < C::NJ; ++j) acc[i][j] = mm_mul(E{}, y[j], x[i], acc[i][j]);
-    }
-  };
-
-  open();
-  if constexpr (C::DIRECT) {
-    for (int i = 0; i < C::ST - 1; ++i) issue();
-  } else {
-    issue();
-    commit();
-  }
-  for (seek(mine); mine.any; seek(mine)) {
+    for (int k = 0; k < C::MI + C::NJ; ++k) read(f0, at, 0, k);
+  });
+  for (mine.seek(p); mine.any; mine.seek(p)) {
     mm_zero(acc);
-    for (int s = 0; s < mine.stages; ++s) {
-      if (C::ST > 2 && ahead.any) mm_wait<(C::ST - 2) * LOADS>();
-      else mm_wait<0>();
-      issue();
-      multiply(lds0 + use * BYTES);
-      commit();
-      use = use + 1 == C::ST ? 0 : use + 1;
-    }
+    for (int s = 0; s < mine.stages; ++s) ring.step(E{}, f0, f1, acc, read);
     const int64_t row = (int64_t)mine.row + wm * (C::BM / C::WM);
     const int64_t n = (int64_t)mine.col + wn * (C::BN / C::WN);
     const int64_t size = (int64_t)p.D1 * p.D2;
@@ -862,6 +1075,7 @@ __global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_grad_kernel(Mm
     else
       mm_write(acc, p.part + mine.piece * size, row, p.D1, n, p.D2);
   }
+  ring.finish();
 }
 
 // Results of groups of several pieces: blockIdx.y a group, four values a thread.
@@ -871,8 +1085,8 @@ __global__ void __launch_bounds__(BLOCK) expert_mm_sum_kernel(MmGradArgs p) {
   walk.init(p.seglen, p.groups, p.rows, p.piece);
   const int g = blockIdx.y;
   while (g >= walk.base + WAVE) walk.next();
-  const uint32_t p0 = (uint32_t)readlane_int((int)walk.first, g - walk.base);
-  const uint32_t p1 = (uint32_t)readlane_int((int)walk.last, g - walk.base);
+  uint32_t s, e, p0, p1;
+  walk.bounds(g - walk.base, &s, &e, &p0, &p1);
   if (p1 - p0 == 1) return;
   const int64_t size = (int64_t)p.D1 * p.D2;
   for (int64_t i = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) * 4; i < size;

@@ -12,13 +12,13 @@ struct Shape {
   float stage[2];  // us a stage of a tile with all slots taken
 };
 
-// us a stage from products of 8,192 rows by 8,192 by 8,192: 820, 1,050, 1,200 TFLOP/s in 16
-// bits through LDS; through registers 600 and 800.
-constexpr Shape shapes[] = {{64, 128, true, {512, 512}, {0.65f, 1.1f}},
-                            {128, 128, true, {512, 512}, {1.02f, 1.54f}},
-                            {256, 256, true, {256, 256}, {1.79f, 2.5f}},
-                            {64, 128, false, {512, 512}, {0.9f, 1.4f}},
-                            {128, 128, false, {512, 256}, {1.34f, 1.0f}}};
+// us a stage from products of 8,192 rows by 8,192 by 8,192: 810, 1,090 and 1,330 TFLOP/s in
+// 16 bits, 1,000, 1,650 and 1,900 in 8 bits; through registers 450 and 580.
+constexpr Shape shapes[] = {{64, 128, true, {512, 512}, {0.66f, 1.07f}},
+                            {128, 128, true, {512, 512}, {0.98f, 1.30f}},
+                            {256, 256, true, {256, 256}, {1.61f, 2.26f}},
+                            {64, 128, false, {512, 512}, {1.2f, 1.4f}},
+                            {128, 128, false, {512, 256}, {1.85f, 1.0f}}};
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
