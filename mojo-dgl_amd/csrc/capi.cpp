@@ -1913,22 +1913,29 @@ int expert_mm_common(const char* what, int64_t n, int64_t d1, int64_t r, int64_t
   return MDGL_OK;
 }
 
-// Bytes that serve whichever way the operands are aligned; -1 for too many tiles.
-int64_t expert_mm_bytes(const ExpertMmPlan& a, const ExpertMmPlan& b) {
-  if (a.shape < 0 || b.shape < 0) return -1;
-  return a.bytes > b.bytes ? a.bytes : b.bytes;
+int64_t expert_mm_bytes(const ExpertMmPlan& plan) { return plan.shape < 0 ? -1 : plan.bytes; }
+
+bool expert_mm_whole(int64_t d1, int64_t d2, bool along) {
+  return d1 % 8 == 0 && (along || d2 % 2 == 0);
 }
 
-int64_t expert_mm_need(int64_t n, int64_t d1, int64_t r, int64_t d2, int size) {
+// Bytes that serve b either way round; -1 for too many tiles.
+int64_t expert_mm_need(int64_t n, int64_t d1, int64_t r, int64_t d2) {
   if (n == 0 || d2 == 0) return 0;
-  return expert_mm_bytes(expert_mm_plan(n, r, d1, d2, size, true),
-                         expert_mm_plan(n, r, d1, d2, size, false));
+  const int64_t x = expert_mm_bytes(expert_mm_plan(n, r, d1, d2, 2, d1 % 8 == 0));
+  const int64_t y =
+      expert_mm_bytes(expert_mm_plan(n, r, d1, d2, 2, expert_mm_whole(d1, d2, false)));
+  return x < 0 || y < 0 ? -1 : x > y ? x : y;
 }
 
 int64_t expert_mm_grad_need(int64_t n, int64_t d1, int64_t r, int64_t d2) {
   if (r == 0 || d1 == 0 || d2 == 0) return 0;
-  return expert_mm_bytes(expert_mm_grad_plan(n, r, d1, d2, true),
-                         expert_mm_grad_plan(n, r, d1, d2, false));
+  return expert_mm_bytes(expert_mm_grad_plan(n, r, d1, d2, d1 % 2 == 0 && d2 % 2 == 0));
+}
+
+int64_t scaled_mm_need(int64_t n, int64_t d1, int64_t r, int64_t d2) {
+  if (n == 0 || d2 == 0) return 0;
+  return expert_mm_bytes(expert_mm_plan(n, r, d1, d2, 1, d1 % 16 == 0));
 }
 
 int expert_mm_workspace(const char* what, int64_t need, const void* workspace,
@@ -1946,7 +1953,7 @@ int expert_mm_workspace(const char* what, int64_t need, const void* workspace,
 
 int64_t mdgl_expert_mm_workspace_bytes(int64_t n, int64_t d1, int64_t r, int64_t d2, int dtype) {
   if (!half_dtype(dtype) || expert_mm_common("expert_mm", n, d1, r, d2)) return -1;
-  return expert_mm_need(n, d1, r, d2, 2);
+  return expert_mm_need(n, d1, r, d2);
 }
 
 int mdgl_expert_mm(const void* a, const void* b, void* dst, const int64_t* seglen, int64_t n,
@@ -1958,7 +1965,7 @@ int mdgl_expert_mm(const void* a, const void* b, void* dst, const int64_t* segle
   if (n == 0 || d2 == 0) return MDGL_OK;
   if (!dst || (r > 0 && (!seglen || (d1 > 0 && (!a || !b)))))
     return fail(MDGL_EINVAL, "expert_mm: null buffer");
-  if (int rc = expert_mm_workspace("expert_mm", expert_mm_need(n, d1, r, d2, 2), workspace,
+  if (int rc = expert_mm_workspace("expert_mm", expert_mm_need(n, d1, r, d2), workspace,
                                    workspace_bytes))
     return rc;
   ExpertMmParams q{};
@@ -1971,8 +1978,7 @@ int mdgl_expert_mm(const void* a, const void* b, void* dst, const int64_t* segle
   q.inner = d1;
   q.cols = d2;
   q.along = transposed != 0;
-  q.plan = expert_mm_plan(n, r, d1, d2, 2, aligned(a, 16) && aligned(b, 16) && d1 % 8 == 0 &&
-                                               (q.along || d2 % 8 == 0));
+  q.plan = expert_mm_plan(n, r, d1, d2, 2, expert_mm_whole(d1, d2, q.along));
   q.workspace = workspace;
   q.stream = (hipStream_t)stream;
   return hip_status(dtype == MDGL_BFLOAT16 ? launch_expert_mm_bf16(q) : launch_expert_mm_f16(q),
@@ -2006,8 +2012,7 @@ int mdgl_expert_mm_grad(const void* a, const void* grad, void* db, const int64_t
   q.groups = r;
   q.inner = d1;
   q.cols = d2;
-  q.plan = expert_mm_grad_plan(
-      n, r, d1, d2, aligned(a, 16) && aligned(grad, 16) && d1 % 8 == 0 && d2 % 8 == 0);
+  q.plan = expert_mm_grad_plan(n, r, d1, d2, d1 % 2 == 0 && d2 % 2 == 0);
   q.workspace = q.plan.bytes > 0 ? workspace : nullptr;
   q.stream = (hipStream_t)stream;
   return hip_status(
@@ -2017,7 +2022,7 @@ int mdgl_expert_mm_grad(const void* a, const void* grad, void* db, const int64_t
 
 int64_t mdgl_scaled_mm_workspace_bytes(int64_t n, int64_t d1, int64_t r, int64_t d2) {
   if (expert_mm_common("scaled_mm", n, d1, r, d2)) return -1;
-  return expert_mm_need(n, d1, r, d2, 1);
+  return scaled_mm_need(n, d1, r, d2);
 }
 
 int mdgl_scaled_mm(const void* a, const float* a_scale, const void* b, const float* b_scale,
@@ -2031,7 +2036,7 @@ int mdgl_scaled_mm(const void* a, const float* a_scale, const void* b, const flo
   if (n == 0 || d2 == 0) return MDGL_OK;
   if (!dst || (r > 0 && d1 > 0 && (!a || !a_scale || !b || !b_scale)))
     return fail(MDGL_EINVAL, "scaled_mm: null buffer");
-  if (int rc = expert_mm_workspace("scaled_mm", expert_mm_need(n, d1, r, d2, 1), workspace,
+  if (int rc = expert_mm_workspace("scaled_mm", scaled_mm_need(n, d1, r, d2), workspace,
                                    workspace_bytes))
     return rc;
   ExpertMmParams q{};
@@ -2047,7 +2052,7 @@ int mdgl_scaled_mm(const void* a, const float* a_scale, const void* b, const flo
   q.cols = d2;
   q.along = true;
   q.out_dtype = dst_dtype;
-  q.plan = expert_mm_plan(n, r, d1, d2, 1, aligned(a, 16) && aligned(b, 16) && d1 % 16 == 0);
+  q.plan = expert_mm_plan(n, r, d1, d2, 1, d1 % 16 == 0);
   q.workspace = workspace;
   q.stream = (hipStream_t)stream;
   return hip_status(launch_expert_mm_f8(q), "scaled_mm");

@@ -30,9 +30,9 @@
 //
 // Past the edges: rows past the tile's group and inner places past the end are read as
 // zeros by the buffer's own bounds check (a lane past the inner end is given an offset
-// behind the buffer), so no stage has a case of its own. Rows that start off a 16-byte
-// boundary (an odd width) go through registers instead: a lane whose piece would pass its
-// row's end reads the last piece of the row and shifts it.
+// behind the buffer), so no stage has a case of its own. The loads take any alignment. Where
+// a row may end inside a piece of 16 bytes, or an operand inside four of them, the tile's
+// last stage is mended in LDS before it is read (kernels of their own: !WHOLE).
 //
 // Tiles are counted on the GPU from the experts' lengths, which the host need not know:
 // every wavefront walks them 64 experts at a time. A tile index in the order of the
@@ -201,37 +201,6 @@ __device__ __forceinline__ void mm_load4(mm_i32x4 buf, uint32_t off, uint32_t ld
                : "m0");
 }
 
-// 16 bytes at p, which lie on a boundary of SIZE.
-template <int SIZE>
-__device__ __forceinline__ mm_i32x4 mm_read16(const char* p) {
-  using U = std::conditional_t<SIZE == 2, uint16_t, uint8_t>;
-  U raw[16 / SIZE];
-  mm_i32x4 v;
-  load_any<false>(reinterpret_cast<const U*>(p), raw);
-  __builtin_memcpy(&v, raw, 16);
-  return v;
-}
-// The first `left` bytes at p, fewer than 16, one value after the other.
-template <int SIZE>
-__device__ __forceinline__ mm_i32x4 mm_read_some(const char* p, int64_t left) {
-  using U = std::conditional_t<SIZE == 2, uint16_t, uint8_t>;
-  mm_i32x4 v = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 16; i += SIZE)
-    if (i < left) v[i / 4] |= (int)((uint32_t)*reinterpret_cast<const U*>(p + i) << 8 * (i % 4));
-  return v;
-}
-// Without the first n bytes (all of them from 16 on), zeros behind.
-__device__ __forceinline__ mm_i32x4 mm_skip(mm_i32x4 v, int64_t n) {
-  typedef uint64_t V __attribute__((ext_vector_type(2)));
-  V x = __builtin_bit_cast(V, v);
-  const uint64_t lo = n >= 8 ? x[1] : x[0], hi = n >= 8 ? 0 : x[1];
-  const int s = (int)(n * 8) & 63;
-  x[0] = n >= 16 ? 0 : lo >> s | hi << 1 << (63 - s);
-  x[1] = n >= 16 ? 0 : hi >> s;
-  return __builtin_bit_cast(mm_i32x4, x);
-}
-
 // At most `n` of the wavefront's loads to LDS outstanding, and none of its LDS reads,
 // then all wavefronts of the workgroup here.
 template <int N>
@@ -243,69 +212,76 @@ __device__ __forceinline__ void mm_wait() {
 }
 
 // An operand whose inner axis is contiguous: ROWS rows of a stage's 128 bytes.
-template <int ROWS, int THREADS, int SIZE, bool DIRECT>
+template <int ROWS, int THREADS, bool WHOLE>
 struct MmAlong {
   static constexpr int BYTES = ROWS * MM_STAGE;
   static constexpr int PIECES = ROWS * 8;
   static constexpr int LOADS = PIECES < THREADS ? 1 : PIECES / THREADS;
   static constexpr int STEP = THREADS / 8;  // rows a load of the workgroup
   mm_i32x4 buf;
-  const char* p;
-  mm_i32x4 held[DIRECT ? 1 : LOADS];
   uint32_t off, lds;  // this lane's source; this wavefront's place
   uint32_t stride;    // bytes of a row
   int col;            // bytes to its place in a row
-  int row, live;
-  uint32_t first, from;  // of the stage being loaded: its place in a row, its offset
+  uint32_t from;      // of the stage being loaded: this lane's source
+  const char* lost;   // the last row's end, if the row's last bytes are not read
+  int live;           // rows
 
   __device__ static __forceinline__ int swizzle(int r) { return r & 7; }
   __device__ __forceinline__ void init(uint32_t row_bytes) {
     // with fewer pieces than threads some wavefronts load the same ones again
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE) % (PIECES / WAVE);
     const int piece = wave * WAVE + (int)(threadIdx.x % WAVE);
-    row = piece / 8;
+    const int row = piece / 8;
     col = ((piece & 7) ^ swizzle(row)) * 16;
     stride = row_bytes;
     off = (uint32_t)row * stride + (uint32_t)col;
     lds = (uint32_t)wave * (WAVE * 16);
   }
-  // `rows` rows from `from` on.
-  __device__ __forceinline__ void tile(const char* from, int rows) {
+  // `rows` rows from `at` on, where the operand has `left` bytes.
+  __device__ __forceinline__ void tile(const char* at, int rows, int64_t left) {
     live = rows < ROWS ? rows : ROWS;
-    p = from;
-    if constexpr (DIRECT) buf = mm_buffer(from, (int64_t)live * stride);
+    int64_t bytes = (int64_t)live * stride;
+    if constexpr (!WHOLE) {
+      // the bounds check is by four bytes: those that begin in the last row are wanted
+      lost = nullptr;
+      if (left >= bytes + 3) {
+        bytes += 3;
+      } else if (stride % 4) {
+        lost = at + bytes;
+      }
+    }
+    buf = mm_buffer(at, bytes);
   }
   // No tile: its loads give zeros.
   __device__ __forceinline__ void none() { buf[2] = 0; }
   __device__ __forceinline__ void begin(uint32_t stage) {
-    first = stage * MM_STAGE + (uint32_t)col;
-    from = first < stride ? off + stage * MM_STAGE : MM_PAST;
+    from = stage * MM_STAGE + (uint32_t)col < stride ? off + stage * MM_STAGE : MM_PAST;
   }
   __device__ __forceinline__ void load(uint32_t at, int i) {
-    if constexpr (DIRECT) {
-      mm_load16(buf, from + i * (STEP * stride), at + lds + i * (THREADS * 16));
-    } else {
-      const int r = row + i * STEP;
-      if (stride >= 16) {
-        // the piece that ends with the row in place of one that would pass its end, and
-        // the last row in place of those behind it: no lane waits for another's branch
-        held[i] = mm_read16<SIZE>(p + (int64_t)(r < live ? r : live - 1) * stride +
-                                  (first < stride - 16 ? first : stride - 16));
-      } else {
-        held[i] = mm_read_some<SIZE>(p + (int64_t)r * stride + first,
-                                     r < live ? (int64_t)stride - first : 0);
-      }
-    }
+    mm_load16(buf, from + i * (STEP * stride), at + lds + i * (THREADS * 16));
   }
-  __device__ __forceinline__ void commit(uint32_t at) {
-    const int64_t behind = stride >= 16 ? (int64_t)first - ((int64_t)stride - 16) : 0;
-    const bool end = first - col + MM_STAGE > stride;  // uniform
+  // The last stage, where a row's last piece holds what follows in memory: zeros in its
+  // place (not left to the other operand's zeros: what follows may be infinite).
+  __device__ __forceinline__ void mend(uint32_t at) {
+    const int end = (int)(stride % MM_STAGE), word = end % 16 / 4, more = end % 4;
+    if (end % 16 == 0) return;
+    int r = threadIdx.x;
+    asm volatile("" : "+v"(r));  // its places are formed here, not held all along
+    for (; r < ROWS; r += THREADS) {
+      auto* piece = (__attribute__((address_space(3))) mm_i32x4*)(lds_char*)(uintptr_t)(
+          at + r * MM_STAGE + ((end / 16 ^ swizzle(r)) * 16));
+      mm_i32x4 v = *piece;
+      uint32_t last = 0;
+      // (rows of one byte: the last three end inside the operand's last four)
+      const int behind = (live - 1 - r) * (int)stride;
+      if (lost && behind >= 0 && behind + more < 4)
+        for (int i = 0; i < more; ++i) last |= (uint32_t)(uint8_t)lost[i - more - behind] << 8 * i;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      if (end && behind > 0) held[i] = mm_skip(held[i], behind);
-      if (row + i * STEP >= live) held[i] = mm_i32x4{0, 0, 0, 0};
-      *(__attribute__((address_space(3))) mm_i32x4*)(lds_char*)(uintptr_t)(
-          at + lds + (threadIdx.x % WAVE) * 16 + i * (THREADS * 16)) = held[i];
+      for (int k = 0; k < 4; ++k) {
+        if (k == word) v[k] = (int)(((uint32_t)v[k] & ((1u << 8 * more) - 1)) | last);
+        if (k > word) v[k] = 0;
+      }
+      *piece = v;
     }
   }
   // Where this lane reads piece `first` of its row of a block of 16; the pieces
@@ -318,7 +294,7 @@ struct MmAlong {
 };
 
 // An operand whose other axis is contiguous (16 bits): 64 inner places of COLS columns.
-template <int COLS, int THREADS, bool DIRECT>
+template <int COLS, int THREADS, bool WHOLE>
 struct MmAcross {
   static constexpr int BYTES = COLS * MM_STAGE;
   static constexpr int ROW = COLS * 2;  // bytes
@@ -328,62 +304,55 @@ struct MmAcross {
   static_assert(STEP % 16 == 0 && COLS >= 128, "");
   mm_i32x4 buf;
   const char* p;
-  mm_i32x4 held[DIRECT ? 1 : LOADS];
   uint32_t off, lds, stride;
-  int row, col;
-  const char* from;  // of the stage being loaded: its first place,
-  int places;        // and how many it has
-  int64_t left;   // inner places from the tile's first on
-  int64_t width;  // bytes of a row from the tile's first column on
+  int64_t bytes;  // to be read, from the tile's first on
+  const char* lost;       // the operand's end, if its last value is not read
+  uint32_t lost_at;       // that value's place in the stage
 
   __device__ static __forceinline__ int swizzle(int r) { return (r & 3) | (r >> 1 & 4); }
+  // Piece `at` of row r lies at this place of it, and the other way round.
+  __device__ static __forceinline__ int placed(int r, int at) {
+    return ((at >> 1) ^ swizzle(r)) * 2 + (at & 1);
+  }
   __device__ __forceinline__ void init(uint32_t row_bytes) {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
     const int piece = wave * WAVE + (int)(threadIdx.x % WAVE);
-    row = piece / PER;
-    const int at = piece % PER;
-    col = (((at >> 1) ^ swizzle(row)) * 2 + (at & 1)) * 16;
+    const int row = piece / PER;
     stride = row_bytes;
-    off = (uint32_t)row * stride + (uint32_t)col;
+    off = (uint32_t)row * stride + (uint32_t)placed(row, piece % PER) * 16;
     lds = (uint32_t)wave * (WAVE * 16);
   }
-  // `places` inner places from `from` on, `columns` (bytes) of each wanted.
-  __device__ __forceinline__ void tile(const char* from, int64_t places, int64_t columns) {
-    p = from;
-    left = places;
-    width = columns;
-  }
-  __device__ __forceinline__ void none() { left = width = 0; }
-  __device__ __forceinline__ void begin(uint32_t stage) {
-    const int64_t first = (int64_t)stage * 64;
-    from = p + first * stride;
-    places = left - first < 64 ? (int)(left - first) : 64;
+  // `n` inner places from `at` on, `width` bytes to the end of a row; the operand has `left`
+  // bytes there.
+  __device__ __forceinline__ void tile(const char* at, int64_t n, int64_t width, int64_t left) {
+    p = at;
     // columns past the width hold what follows in memory: they meet only results that are
     // not written
-    if constexpr (DIRECT) buf = mm_buffer(from, (left - first - 1) * stride + width);
+    bytes = (n - 1) * stride + width;
+    if constexpr (!WHOLE) {  // as in MmAlong
+      lost = nullptr;
+      if (left >= bytes + 3) {
+        bytes += 3;
+      } else if (width % 4 && width <= ROW) {
+        const int r = (int)(n - 1) % 64, c = (int)width - 2;
+        lost = at + bytes;
+        lost_at = (uint32_t)(r * ROW + placed(r, c / 16) * 16 + c % 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void none() { bytes = 0; }
+  __device__ __forceinline__ void begin(uint32_t stage) {
+    const int64_t first = (int64_t)stage * 64;
+    buf = mm_buffer(p + first * stride, bytes - first * stride);
+    asm volatile("" : "+v"(off));  // the loads' offsets are formed anew, not held all along
   }
   __device__ __forceinline__ void load(uint32_t at, int i) {
-    if constexpr (DIRECT) {
-      mm_load16(buf, off + i * (STEP * stride), at + lds + i * (THREADS * 16));
-    } else {
-      const int r = row + i * STEP;
-      if (stride >= 16)  // as in MmAlong
-        held[i] = mm_read16<2>(from + (int64_t)(r < places ? r : places - 1) * stride +
-                               (col < width - 16 ? col : width - 16));
-      else
-        held[i] = mm_read_some<2>(from + (int64_t)r * stride + col, r < places ? width - col : 0);
-    }
+    mm_load16(buf, off + i * (STEP * stride), at + lds + i * (THREADS * 16));
   }
-  __device__ __forceinline__ void commit(uint32_t at) {
-    const int64_t behind = stride >= 16 ? col - (width - 16) : 0;
-    const bool end = width < ROW;  // uniform
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      if (end && behind > 0) held[i] = mm_skip(held[i], behind);
-      if (row + i * STEP >= places) held[i] = mm_i32x4{0, 0, 0, 0};
-      *(__attribute__((address_space(3))) mm_i32x4*)(lds_char*)(uintptr_t)(
-          at + lds + (threadIdx.x % WAVE) * 16 + i * (THREADS * 16)) = held[i];
-    }
+  __device__ __forceinline__ void mend(uint32_t at) {
+    if (lost && threadIdx.x == 0)
+      *(__attribute__((address_space(3))) uint16_t*)(lds_char*)(uintptr_t)(at + lost_at) =
+          *reinterpret_cast<const uint16_t*>(lost - 2);
   }
   // Where this lane reads block `unit` of 16 columns, inner places 8 q + l / 4; block
   // unit + n, n below the power of two that divides `unit`, lies at the place xor 32 n.
@@ -522,9 +491,10 @@ struct MmHalf8 {
 // the one whose second half all have in registers, so its place is filled again.
 // Behind the last stage of the last tile it goes on with loads of nothing, so that as
 // many are outstanding at every wait. `Loader`: begin(), load(place, i) for its LOADS loads,
-// end(place).
-template <int ST, int BYTES, bool DIRECT, class Loader>
+// next() to the stage behind, mend(place) of the newest one when it is there.
+template <int ST, int BYTES, class Loader>
 struct MmRing {
+  static_assert(Loader::WHOLE || ST == 2, "");  // what is read next is the newest
   Loader& loader;
   uint32_t base;
   uint32_t use = 0;     // the place of the stage
@@ -534,37 +504,49 @@ struct MmRing {
   // stores of a tile's results need not have ended.
   template <int N, int STORES>
   __device__ __forceinline__ void wait() {
-    if (DIRECT && stored) mm_wait<N + STORES>();
-    else mm_wait<DIRECT ? N : 0>();
+    if (stored) mm_wait<N + STORES>();
+    else mm_wait<N>();
     stored = false;
   }
   template <class Read>
   __device__ __forceinline__ void start(Read first) {
 #pragma unroll
     for (int i = 0; i < ST; ++i) {
-      if (i) loader.end(base + (i - 1) * BYTES);
+      if (i) loader.next();
       loader.begin();
 #pragma unroll
       for (int k = 0; k < Loader::LOADS; ++k) loader.load(base + i * BYTES, k);
+      if (!Loader::WHOLE && i == 0) {
+        mm_wait<0>();
+        loader.mend(base);
+      }
     }
-    mm_wait<DIRECT ? (ST - 1) * Loader::LOADS : 0>();
+    if (Loader::WHOLE) mm_wait<(ST - 1) * Loader::LOADS>();
     first(base);
   }
-  // The place before `use`: its loads are the newest.
-  __device__ __forceinline__ uint32_t newest() const {
-    return base + (use ? use - 1 : ST - 1) * BYTES;
+  // The stage at `place` is there for all, and the loads of the one behind the newest begin.
+  template <int STORES>
+  __device__ __forceinline__ void turn(uint32_t place) {
+    if constexpr (Loader::WHOLE) {
+      loader.next();
+      loader.begin();
+      wait<(ST - 2) * Loader::LOADS, STORES>();
+    } else {
+      wait<0, STORES>();
+      loader.mend(place);
+      loader.next();
+      loader.begin();
+    }
   }
   // A stage in 16 bits. read(half, place, h, k): part k of half h.
   template <class E, int MI, int NJ, class Read>
   __device__ __forceinline__ void step(E, MmHalf<MI, NJ>& f0, MmHalf<MI, NJ>& f1,
                                        mm_f32x4 (&acc)[MI][NJ], Read read) {
-    const uint32_t at = base + use * BYTES, loaded = newest();
+    const uint32_t at = base + use * BYTES;
     use = use + 1 == ST ? 0 : use + 1;
     const uint32_t next = base + use * BYTES;
     mm_half<E, 0>(f0, acc, [&](int k) { read(f1, at, 1, k); }, [](int) {});
-    loader.end(loaded);
-    loader.begin();
-    wait<(ST - 2) * Loader::LOADS, MI * NJ / 2>();
+    turn<MI * NJ / 2>(next);
     mm_half<E, Loader::LOADS>(f1, acc, [&](int k) { read(f0, next, 0, k); },
                               [&](int k) { loader.load(at, k); });
   }
@@ -578,7 +560,7 @@ struct MmRing {
                                         ReadX read_x, ReadY read_y) {
     constexpr int W = MmHalf8<MI, NJ>::W, MEET = MI == 8 ? 4 : 1, N = (MI - 1 - MEET) * NJ;
     static_assert(MI == 8 || MI == 4, "");
-    const uint32_t at = base + use * BYTES, loaded = newest();
+    const uint32_t at = base + use * BYTES;
     use = use + 1 == ST ? 0 : use + 1;
     const uint32_t next = base + use * BYTES;
     mm_f32x4 before;
@@ -610,9 +592,7 @@ struct MmRing {
       }
       if (i + W < MI) read_x(at, i + W);
       if (i == MEET) {
-        loader.end(loaded);
-        loader.begin();
-        wait<(ST - 2) * Loader::LOADS, MI * NJ / 2>();
+        turn<MI * NJ / 2>(next);
 #pragma unroll
         for (int r = 0; r <= MEET; ++r)
           if (r + W >= MI) read_x(next, r + W - MI);
@@ -626,30 +606,28 @@ struct MmRing {
   __device__ __forceinline__ void finish() const { mm_wait<0>(); }
 };
 
-template <class E, int BM_, int BN_, int WM_, int WN_, int ST_, bool ALONG_, bool DIRECT_>
+template <class E, int BM_, int BN_, int WM_, int WN_, int ST_, bool ALONG_, bool WHOLE_>
 struct MmConf {
   using Elem = E;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr bool ALONG = ALONG_;    // b's inner axis is contiguous
-  static constexpr bool DIRECT = DIRECT_;  // from memory to LDS past the registers
+  static constexpr bool WHOLE = WHOLE_;  // nothing is to be mended
   static constexpr int ST = ST_;
   static constexpr int THREADS = WM * WN * WAVE;
   static constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
   static constexpr bool EIGHT = sizeof(E) == 1;
   static constexpr int SIZE = (int)sizeof(E);
   static constexpr int INNER = MM_STAGE / SIZE;  // inner places a stage
-  using A = MmAlong<BM, THREADS, SIZE, DIRECT>;
-  using B = std::conditional_t<ALONG, MmAlong<BN, THREADS, SIZE, DIRECT>,
-                               MmAcross<BN, THREADS, DIRECT>>;
+  using A = MmAlong<BM, THREADS, WHOLE>;
+  using B =
+      std::conditional_t<ALONG, MmAlong<BN, THREADS, WHOLE>, MmAcross<BN, THREADS, WHOLE>>;
   static constexpr int SCALES = EIGHT ? (BM < WAVE ? WAVE : BM) * 4 : 0;
   static constexpr int STAGE_BYTES = A::BYTES + B::BYTES + SCALES;
   static constexpr int LOADS = A::LOADS + B::LOADS + (EIGHT ? 1 : 0);
-  // workgroups on a compute unit, two at most (their LDS: 160 KB); one of eight
-  // wavefronts that load 8-bit values through registers
-  static constexpr int PER_CU =
-      2 * ST * STAGE_BYTES <= 163840 && !(EIGHT && !DIRECT && THREADS > 256) ? 2 : 1;
+  // workgroups on a compute unit, two at most (their LDS: 160 KB)
+  static constexpr int PER_CU = 2 * ST * STAGE_BYTES <= 163840 ? 2 : 1;
   static constexpr int WAVES = PER_CU * THREADS / 256 > 0 ? PER_CU * THREADS / 256 : 1;
-  static_assert(NJ % 2 == 0 && (DIRECT || ST == 2) && (ST - 2) * LOADS < 64, "");
+  static_assert(NJ % 2 == 0 && (ST - 2) * LOADS + MI * NJ / 2 < 64, "");
   static_assert(!EIGHT || (ALONG && BM / WAVE <= WM * WN && 128 % (BN / WN) == 0), "");
 };
 
@@ -707,6 +685,7 @@ struct MmTile {
 template <class C>
 struct MmSource {
   static constexpr int LOADS = C::LOADS;
+  static constexpr bool WHOLE = C::WHOLE;
   const MmArgs& p;
   MmTile<C> tile;
   typename C::A A;
@@ -717,7 +696,6 @@ struct MmSource {
   mm_i32x4 scales;
   uint32_t scale_off, scale_lds;
   int scale_row, kb;
-  float scale_held;
   float b_scale;  // of the tile's first 64 stages, one a lane
 
   // b's scale of stage s + lane for the tile's columns of this wavefront.
@@ -754,13 +732,14 @@ struct MmSource {
       return;
     }
     const int rows = (int)(tile.end - tile.row);
-    A.tile(p.a + tile.row * row_bytes, rows);
+    A.tile(p.a + tile.row * row_bytes, rows, (p.rows - tile.row) * row_bytes);
     const char* block = p.b + tile.group * (row_bytes * p.N);
-    if constexpr (C::ALONG) {
-      B.tile(block + tile.col * row_bytes, p.N - (int)tile.col);
-    } else {
-      B.tile(block + (int64_t)tile.col * 2, p.K, (int64_t)(p.N - (int)tile.col) * 2);
-    }
+    const int64_t left = (p.groups - tile.group) * (row_bytes * p.N);
+    const int64_t col = tile.col;
+    if constexpr (C::ALONG)
+      B.tile(block + col * row_bytes, p.N - (int)col, left - col * row_bytes);
+    else
+      B.tile(block + col * 2, p.K, (p.N - (int)col) * (int64_t)2, left - col * 2);
     if constexpr (C::EIGHT) {
       scales = mm_buffer((const char*)(p.sa + (int64_t)tile.row * kb),
                          (int64_t)(rows < C::BM ? rows : C::BM) * kb * 4);
@@ -772,31 +751,22 @@ struct MmSource {
     B.begin(stage);
   }
   __device__ __forceinline__ void load(uint32_t at, int i) {
-    if (!C::DIRECT && !tile.any) return;
     if (i < C::A::LOADS) {
       A.load(at, i);
     } else if (i < C::A::LOADS + C::B::LOADS) {
       B.load(at + C::A::BYTES, i - C::A::LOADS);
     } else if constexpr (C::EIGHT) {
-      if constexpr (C::DIRECT) {
-        mm_load4(scales, scale_off + stage * 4, at + scale_lds);
-      } else {
-        const int rows = (int)(tile.end - tile.row);
-        scale_held = scale_row < (rows < C::BM ? rows : C::BM)
-                         ? p.sa[(int64_t)(tile.row + scale_row) * kb + stage] : 0.0f;
-      }
+      mm_load4(scales, scale_off + stage * 4, at + scale_lds);
     }
   }
-  __device__ __forceinline__ void end(uint32_t at) {
-    if (!tile.any) return;
-    if constexpr (!C::DIRECT) {
-      A.commit(at);
-      B.commit(at + C::A::BYTES);
-      if constexpr (C::EIGHT)
-        *(__attribute__((address_space(3))) float*)(lds_char*)(uintptr_t)(
-            at + scale_lds + (threadIdx.x % WAVE) * 4) = scale_held;
-    }
-    if (++stage == tile.stage1) open();
+  __device__ __forceinline__ void next() {
+    if (tile.any && ++stage == tile.stage1) open();
+  }
+  __device__ __forceinline__ void mend(uint32_t at) {
+    if (!tile.any || (stage + 1) * C::INNER < p.K) return;
+    A.mend(at);
+    B.mend(at + C::A::BYTES);
+    mm_wait<63>();
   }
 };
 
@@ -823,7 +793,7 @@ __global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_kernel(MmArgs 
   mine.init(p);
   MmSource<C> source{p};  // what is loaded
   source.init(mine);
-  MmRing<C::ST, C::STAGE_BYTES, C::DIRECT, MmSource<C>> ring{source, lds0};
+  MmRing<C::ST, C::STAGE_BYTES, MmSource<C>> ring{source, lds0};
   mm_f32x4 acc[C::MI][C::NJ];
   auto write = [&]() {
     const int64_t row = (int64_t)mine.row + wm * (C::BM / C::WM);
@@ -985,8 +955,9 @@ struct MmGradTile {
 
 template <class C>
 struct MmGradSource {
-  using A = MmAcross<C::BM, C::THREADS, C::DIRECT>;
-  using B = MmAcross<C::BN, C::THREADS, C::DIRECT>;
+  using A = MmAcross<C::BM, C::THREADS, C::WHOLE>;
+  using B = MmAcross<C::BN, C::THREADS, C::WHOLE>;
+  static constexpr bool WHOLE = C::WHOLE;
   static constexpr int LOADS = A::LOADS + B::LOADS, BYTES = A::BYTES + B::BYTES;
   const MmGradArgs& p;
   MmGradTile<C> tile;
@@ -1009,27 +980,28 @@ struct MmGradSource {
       b.none();
       return;
     }
+    const int64_t rows = p.rows - tile.start;
     a.tile(p.a + ((int64_t)tile.start * p.D1 + tile.row) * 2, tile.rows,
-           (int64_t)(p.D1 - (int)tile.row) * 2);
+           (int64_t)(p.D1 - (int)tile.row) * 2, (rows * p.D1 - tile.row) * 2);
     b.tile(p.grad + ((int64_t)tile.start * p.D2 + tile.col) * 2, tile.rows,
-           (int64_t)(p.D2 - (int)tile.col) * 2);
+           (int64_t)(p.D2 - (int)tile.col) * 2, (rows * p.D2 - tile.col) * 2);
   }
   __device__ __forceinline__ void begin() {
     a.begin(stage);
     b.begin(stage);
   }
   __device__ __forceinline__ void load(uint32_t at, int i) {
-    if (!C::DIRECT && !tile.any) return;
     if (i < A::LOADS) a.load(at, i);
     else b.load(at + A::BYTES, i - A::LOADS);
   }
-  __device__ __forceinline__ void end(uint32_t at) {
-    if (!tile.any) return;
-    if constexpr (!C::DIRECT) {
-      a.commit(at);
-      b.commit(at + A::BYTES);
-    }
-    if (++stage == tile.stages) open();
+  __device__ __forceinline__ void next() {
+    if (tile.any && ++stage == tile.stages) open();
+  }
+  __device__ __forceinline__ void mend(uint32_t at) {
+    if (!tile.any || stage + 1 < tile.stages) return;
+    a.mend(at);
+    b.mend(at + A::BYTES);
+    mm_wait<63>();
   }
 };
 
@@ -1058,7 +1030,7 @@ __global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_grad_kernel(Mm
   mine.init(p);
   S source{p};
   source.init(mine);
-  MmRing<C::ST, S::BYTES, C::DIRECT, S> ring{source, lds0};
+  MmRing<C::ST, S::BYTES, S> ring{source, lds0};
   mm_f32x4 acc[C::MI][C::NJ];
   ring.start([&](uint32_t at) {
 #pragma unroll
@@ -1170,10 +1142,8 @@ hipError_t run_expert_mm_shape(const ExpertMmParams& q) {
     case 1: return run_expert_mm<MmConf<E, 128, 128, 2, 2, 2, ALONG, true>>(p, tiles, s);
     case 2: return run_expert_mm<MmConf<E, 256, 256, 2, 4, 2, ALONG, true>>(p, tiles, s);
     case 3: return run_expert_mm<MmConf<E, 64, 128, 1, 4, 2, ALONG, false>>(p, tiles, s);
-    default:
-      // eight wavefronts where four would hold more values than they have registers
-      return run_expert_mm<MmConf<E, 128, 128, 2, sizeof(E) == 1 ? 4 : 2, 2, ALONG, false>>(
-          p, tiles, s);
+    case 4: return run_expert_mm<MmConf<E, 128, 128, 2, 2, 2, ALONG, false>>(p, tiles, s);
+    default: return run_expert_mm<MmConf<E, 256, 256, 2, 4, 2, ALONG, false>>(p, tiles, s);
   }
 }
 
@@ -1195,7 +1165,8 @@ hipError_t run_expert_mm_grad_shape(const ExpertMmParams& q) {
   switch (q.plan.shape) {
     case 1: return run_expert_mm_grad<MmConf<E, 128, 128, 2, 2, 2, false, true>>(p, tiles, s);
     case 2: return run_expert_mm_grad<MmConf<E, 256, 256, 2, 4, 2, false, true>>(p, tiles, s);
-    default: return run_expert_mm_grad<MmConf<E, 128, 128, 2, 2, 2, false, false>>(p, tiles, s);
+    case 4: return run_expert_mm_grad<MmConf<E, 128, 128, 2, 2, 2, false, false>>(p, tiles, s);
+    default: return run_expert_mm_grad<MmConf<E, 256, 256, 2, 4, 2, false, false>>(p, tiles, s);
   }
 }
 

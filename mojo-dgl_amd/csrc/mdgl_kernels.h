@@ -441,11 +441,12 @@ struct ExpertMmPlan {
   int64_t tiles;   // at most
   int64_t bytes;   // of the workspace
 };
-// direct: rows of both operands start on 16-byte boundaries. size: bytes of a value.
+// whole: rows along the inner axis are multiples of 16 bytes, others of 4. size: bytes of a
+// value.
 ExpertMmPlan expert_mm_plan(int64_t rows, int64_t groups, int64_t inner, int64_t cols, int size,
-                            bool direct);
+                            bool whole);
 ExpertMmPlan expert_mm_grad_plan(int64_t rows, int64_t groups, int64_t d1, int64_t d2,
-                                 bool direct);
+                                 bool whole);
 struct ExpertMmParams {
   const void* a;
   const void* b;  // gradient: the results' gradient

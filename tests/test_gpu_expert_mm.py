@@ -168,6 +168,88 @@ def test_what_is_not_a_number_stays_in_its_row(dtype, d1, d2):
     assert torch.equal(y[70:200, 5:], clean[70:200, 5:])
 
 
+def island(t, before):
+    """The values of t, contiguous, `before` values into memory that is NaN around them."""
+    sea = torch.full((before + t.numel() + 64,), NAN, device="cuda").to(t.dtype)
+    it = sea[before:before + t.numel()].view(t.shape)
+    it.copy_(t)
+    return it
+
+
+@pytest.mark.parametrize("before", [0, 1, 2, 5, 8])
+@pytest.mark.parametrize("lens,behind", [([1], 0), ([3], 0), ([40, 0, 65], 0), ([40, 65], 6)])
+@pytest.mark.parametrize("d1,d2", [(1, 1), (1, 2), (2, 3), (3, 130), (7, 8), (63, 9), (65, 127),
+                                   (130, 129), (129, 64), (200, 33), (301, 602)])
+def test_operands_are_read_to_their_ends_and_no_further(d1, d2, lens, behind, before):
+    """Rows that end anywhere in 16 bytes, operands that begin and end anywhere in four."""
+    g = gen(d1 * 1000 + d2)
+    n, r = sum(lens) + behind, len(lens)
+    x, dy = (island(rand(g, n, d, dtype=BF16), before) for d in (d1, d2))
+    for turned in (False, True):
+        if turned:
+            w = island(rand(g, r, d2, d1, dtype=BF16), before).transpose(1, 2)
+        else:
+            w = island(rand(g, r, d1, d2, dtype=BF16), before)
+        X, W = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = ops.expert_mm(X, W, lens)
+        dx, dw = torch.autograd.grad(y, (X, W), dy)
+        want, size = products(x, w, lens)
+        check(y.detach(), want, (d1 + 64) * U * size, "y")
+        want, size = products(dy, w.transpose(1, 2).contiguous(), lens)
+        check(dx, want, (d2 + 64) * U * size, "dx")
+        want, size = weight_gradients(x, dy, lens, r)
+        check(dw, want, (max(lens) + 64) * U * size, "dw")
+    qx, qw = ops.quantize_rows(x), ops.quantize_blocks(w)
+    inner = island(qw.data.transpose(1, 2).contiguous(), before).transpose(1, 2)
+    y = ops.scaled_mm(ops.Quantized(island(qx.data, before), qx.scale),
+                      ops.Quantized(inner, qw.scale), lens, dtype=F32)
+    want, size = products(values(qx, (1,)), values(qw, (1, 2)), lens)
+    check(y, want, (d1 + 68) * U * size + cut(qx, qw, lens), "8 bits")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lens,behind,d1,d2", [
+    ([1], 0, 4096, 512), ([64], 0, 2048, 130), ([65], 0, 4104, 257), ([20], 44, 4103, 301),
+    ([5, 0, 3], 9, 8200, 129), ([1, 2], 3, 1024, 4), ([300], 0, 1999, 64)])
+def test_few_rows_of_long_inner_axes(lens, behind, d1, d2, dtype):
+    """The inner axis in parts; a captured call has its own workspace."""
+    g = gen(d1 + d2)
+    n, r = sum(lens) + behind, len(lens)
+    x, dy = rand(g, n, d1, dtype=dtype), rand(g, n, d1, dtype=dtype)
+    w, v = rand(g, r, d1, d2, dtype=dtype), rand(g, r, d2, d1, dtype=dtype)
+    qx, qw = ops.quantize_rows(x), ops.quantize_blocks(w)
+    ids = torch.repeat_interleave(torch.arange(r + 1), torch.tensor(lens + [behind])).cuda()
+    plan = ops.route_plan(ids, r)
+
+    def run():
+        return [ops.expert_mm(x, w, plan), ops.expert_mm(dy, v.transpose(1, 2), plan),
+                ops.scaled_mm(qx, qw, plan, dtype=F32), ops.scaled_mm(qx, qw, plan, dtype=dtype)]
+
+    y, z, eight, short = run()
+    want, size = products(x, w, lens)
+    check(y, want, (d1 + 64) * U * size, "y")
+    want, size = products(dy, v.transpose(1, 2).contiguous(), lens)
+    check(z, want, (d1 + 64) * U * size, "z")
+    want, size = products(values(qx, (1,)), values(qw, (1, 2)), lens)
+    check(eight, want, (d1 + 68) * U * size + cut(qx, qw, lens), "8 bits")
+    assert torch.equal(short, eight.to(dtype))
+    assert not any(t[sum(lens):].any() for t in (y, z, eight))
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(run())
+    for seed in range(3):
+        x.copy_(rand(gen(seed), n, d1, dtype=dtype))
+        want = run()
+        torch.cuda.synchronize()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), seed
+
+
 def test_subnormal_values_and_large_ones():
     """Products and sums keep float32's range: float16 subnormals count, and a result past
     the type's range is infinite."""
