@@ -748,21 +748,20 @@ class LayerNorm(torch.autograd.Function):
 class RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, value, weight, residual, eps):
-        from .norm import _rms_norm, _rms_operands
+        from .norm import _rms_norm
 
-        y, total, rstd = _rms_norm(value, weight, residual, eps, False, True)
-        ctx.types = _rms_operands(value, weight, residual)[3:6]
+        y, total, rstd, ctx.types = _rms_norm(value, weight, residual, eps, False, True)
         ctx.set_materialize_grads(False)
         where = _lib.caller_device(value, weight, residual)
         y = _lib.hand_back(y, where)
         total = None if total is None else _lib.hand_back(total, where)
-        ctx.like = tuple(x if x is None or not isinstance(x, torch.Tensor)
-                         else torch.empty(0, dtype=x.dtype, device=x.device)
-                         for x in (value, residual))
         # of the rows and the residual their sum will do unless it is rounded to 16 bits
         if residual is None or ctx.types[2].itemsize == 2:
+            ctx.like = None
             _save_some(ctx, value, residual, weight, rstd)
         else:
+            ctx.like = tuple(torch.empty(0, dtype=x.dtype, device=x.device)
+                             if isinstance(x, torch.Tensor) else None for x in (value, residual))
             _save_some(ctx, total, None, weight, rstd)
         _made_here(ctx, where)
         return y, total
@@ -778,7 +777,7 @@ class RmsNorm(torch.autograd.Function):
         total, added, weight, rstd = _saved_some(ctx)
         dx, dw, dr = _rms_norm_grad(total, added, weight, rstd, grad, grad_total, *ctx.types,
                                     ctx.needs_input_grad[:3])
-        value, residual = ctx.like
+        value, residual = ctx.like or (total, added)
         return _back(dx, value), _back(dw, weight), _back(dr, residual), None
 
 

@@ -148,7 +148,7 @@ def rms_norm(value, weight=None, residual=None, eps=1e-6, quantize=False):
             raise DGLError("rms_norm has no gradient with quantize=True")
         y, total = _autograd.RmsNorm.apply(value, weight, residual, eps)
         return y if residual is None else (y, total)
-    y, total, _ = _rms_norm(value, weight, residual, eps, bool(quantize), False)
+    y, total, _, _ = _rms_norm(value, weight, residual, eps, bool(quantize), False)
     where = _lib.caller_device(value, weight, residual)
     y = _quant.hand_back(y, where) if quantize else _lib.hand_back(y, where)
     return y if residual is None else (y, _lib.hand_back(total, where))
@@ -168,7 +168,7 @@ def _rms_operands(value, weight, residual):
 
 
 def _rms_norm(value, weight, residual, eps, quantize, want_stats):
-    """(y, total, rstd) on the GPU."""
+    """(y, total, rstd) on the GPU and the types (rows, weight, residual)."""
     x, w, r, vt, wt, rt, d = _rms_operands(value, weight, residual)
     eps = float(eps)
     if not eps >= 0.0:
@@ -187,7 +187,8 @@ def _rms_norm(value, weight, residual, eps, quantize, want_stats):
         x.data_ptr(), _lib.ptr(r), _lib.ptr(w), y.data_ptr(), _lib.ptr(scale), _lib.ptr(total),
         _lib.ptr(rstd), n, d, eps, _lib.ROW_CODES[vt], _lib.ROW_CODES[wt], _lib.ROW_CODES[rt],
         _lib.stream()), "rms_norm")
-    return _quant.Quantized(y, scale) if quantize else y, total, rstd
+    y = _quant.Quantized(y, scale) if quantize else y
+    return y, total, rstd, (vt, wt, rt)
 
 
 def _rms_norm_grad(total, residual, weight, rstd, grad, grad_total, vt, wt, rt, need):
