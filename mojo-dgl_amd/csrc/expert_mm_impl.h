@@ -212,7 +212,7 @@ __device__ __forceinline__ void mm_wait() {
 }
 
 // An operand whose inner axis is contiguous: ROWS rows of a stage's 128 bytes.
-template <int ROWS, int THREADS, bool WHOLE>
+template <int ROWS, int THREADS, int SIZE, bool WHOLE>
 struct MmAlong {
   static constexpr int BYTES = ROWS * MM_STAGE;
   static constexpr int PIECES = ROWS * 8;
@@ -226,7 +226,11 @@ struct MmAlong {
   const char* lost;   // the last row's end, if the row's last bytes are not read
   int live;           // rows
 
-  __device__ static __forceinline__ int swizzle(int r) { return r & 7; }
+  // 16 lanes are served at a time: two neighbouring q (read_at) of 8 rows, two rows to all
+  // banks. In 16 bits they read pieces q and q + 1, in 8 bits 2 q and 2 q + 2.
+  __device__ static __forceinline__ int swizzle(int r) {
+    return SIZE == 1 ? (r >> 1 & 1) | (r & 4) : r & 7;
+  }
   __device__ __forceinline__ void init(uint32_t row_bytes) {
     // with fewer pieces than threads some wavefronts load the same ones again
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE) % (PIECES / WAVE);
@@ -618,9 +622,9 @@ struct MmConf {
   static constexpr bool EIGHT = sizeof(E) == 1;
   static constexpr int SIZE = (int)sizeof(E);
   static constexpr int INNER = MM_STAGE / SIZE;  // inner places a stage
-  using A = MmAlong<BM, THREADS, WHOLE>;
+  using A = MmAlong<BM, THREADS, SIZE, WHOLE>;
   using B =
-      std::conditional_t<ALONG, MmAlong<BN, THREADS, WHOLE>, MmAcross<BN, THREADS, WHOLE>>;
+      std::conditional_t<ALONG, MmAlong<BN, THREADS, SIZE, WHOLE>, MmAcross<BN, THREADS, WHOLE>>;
   static constexpr int SCALES = EIGHT ? (BM < WAVE ? WAVE : BM) * 4 : 0;
   static constexpr int STAGE_BYTES = A::BYTES + B::BYTES + SCALES;
   static constexpr int LOADS = A::LOADS + B::LOADS + (EIGHT ? 1 : 0);
