@@ -481,12 +481,12 @@ __device__ __forceinline__ void mm_half(const MmHalf<MI, NJ>& f, mm_f32x4 (&acc)
   }
 }
 
-// What a wavefront has of a stage in 8 bits: values and the rows' scales.
+// What a wavefront has of a stage in 8 bits: values, the rows' scales and its columns'.
 template <int MI, int NJ>
 struct MmHalf8 {
   static constexpr int W = 4;  // row blocks
   mm_i32x8 x[W], y[NJ];
-  float s[W];
+  float s[W], sb;
 };
 
 // The ring of stages in LDS. While one half of a stage is multiplied the next half is
@@ -557,41 +557,43 @@ struct MmRing {
   // A stage in 8 bits, row block by row block: at most four of them are in registers, and
   // a block's place takes the fourth behind it, of this stage or the next; y takes the
   // next stage's values behind its last use. The wavefronts meet behind block MEET, when
-  // all of the stage is in registers. A product is scaled and added while the one behind it
-  // is formed.
+  // all of the stage is in registers. A product is scaled and added while the LAG behind it
+  // are formed: with one, every second sum waited for its product (8,192 rows by 8,192 by
+  // 8,192: 548 us, with two 528).
   template <int MI, int NJ, class ReadX, class ReadY>
-  __device__ __forceinline__ void step8(MmHalf8<MI, NJ>& f, mm_f32x4 (&acc)[MI][NJ], float sb,
+  __device__ __forceinline__ void step8(MmHalf8<MI, NJ>& f, mm_f32x4 (&acc)[MI][NJ],
                                         ReadX read_x, ReadY read_y) {
     constexpr int W = MmHalf8<MI, NJ>::W, MEET = MI == 8 ? 4 : 1, N = (MI - 1 - MEET) * NJ;
     static_assert(MI == 8 || MI == 4, "");
     const uint32_t at = base + use * BYTES;
     use = use + 1 == ST ? 0 : use + 1;
     const uint32_t next = base + use * BYTES;
-    mm_f32x4 before;
-    float s = 0.0f;
-    auto add = [&](int i, int j, float by) {
+    constexpr int LAG = 2;
+    mm_f32x4 before[LAG];
+    float scale[LAG];
+    auto add = [&](int m) {  // the stage's product m
+      mm_f32x4& to = acc[m / NJ][m % NJ];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[i][j][k] = __builtin_fmaf(before[k], by, acc[i][j][k]);
+      for (int k = 0; k < 4; ++k)
+        to[k] = __builtin_fmaf(before[m % LAG][k], scale[m / NJ % LAG], to[k]);
       // here and not behind the stage, where the compiler would move all of them
-      asm volatile("" : "+v"(acc[i][j]));
+      asm volatile("" : "+v"(to));
       __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const float last = s;
-      s = sb * f.s[i % W];
+      scale[i % LAG] = f.sb * f.s[i % W];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const int m = (i - 1 - MEET) * NJ + j;
+        const int m = (i - 1 - MEET) * NJ + j, n = i * NJ + j;
 #pragma unroll
         for (int k = 0; k < Loader::LOADS; ++k)
           if (m >= 0 && k * N / Loader::LOADS == m) loader.load(at, k);
         __builtin_amdgcn_sched_barrier(0);
         const mm_f32x4 t = mm_mul8(f.y[j], f.x[i % W]);
         __builtin_amdgcn_sched_barrier(0);
-        if (j) add(i, j - 1, s);
-        else if (i) add(i - 1, NJ - 1, last);
-        before = t;
+        if (n >= LAG) add(n - LAG);
+        before[n % LAG] = t;
         if (i == MI - 1) read_y(next, j);
       }
       if (i + W < MI) read_x(at, i + W);
@@ -604,7 +606,8 @@ struct MmRing {
         read_x(next, i + W - MI);
       }
     }
-    add(MI - 1, NJ - 1, s);
+#pragma unroll
+    for (int n = MI * NJ - LAG; n < MI * NJ; ++n) add(n);
   }
   // Nothing is left on its way to LDS.
   __device__ __forceinline__ void finish() const { mm_wait<0>(); }
@@ -625,14 +628,16 @@ struct MmConf {
   using A = MmAlong<BM, THREADS, SIZE, WHOLE>;
   using B =
       std::conditional_t<ALONG, MmAlong<BN, THREADS, SIZE, WHOLE>, MmAcross<BN, THREADS, WHOLE>>;
-  static constexpr int SCALES = EIGHT ? (BM < WAVE ? WAVE : BM) * 4 : 0;
-  static constexpr int STAGE_BYTES = A::BYTES + B::BYTES + SCALES;
+  // the rows' scales, then those of the tile's blocks of 128 columns
+  static constexpr int SCALES = EIGHT ? BM * 4 : 0;
+  static constexpr int STAGE_BYTES = A::BYTES + B::BYTES + SCALES + (EIGHT ? 256 : 0);
   static constexpr int LOADS = A::LOADS + B::LOADS + (EIGHT ? 1 : 0);
   // workgroups on a compute unit, two at most (their LDS: 160 KB)
   static constexpr int PER_CU = 2 * ST * STAGE_BYTES <= 163840 ? 2 : 1;
   static constexpr int WAVES = PER_CU * THREADS / 256 > 0 ? PER_CU * THREADS / 256 : 1;
   static_assert(NJ % 2 == 0 && (ST - 2) * LOADS + MI * NJ / 2 < 64, "");
-  static_assert(!EIGHT || (ALONG && BM / WAVE <= WM * WN && 128 % (BN / WN) == 0), "");
+  static_assert(!EIGHT || (ALONG && BM / WAVE < WM * WN && 128 % (BN / WN) == 0 && BN % 128 == 0),
+                "");
 };
 
 struct MmArgs {
@@ -696,20 +701,12 @@ struct MmSource {
   typename C::B B;
   int stage;
   int64_t row_bytes;
-  // 8 bits: a row's scale a thread
+  // 8 bits: the first wavefronts load the rows' scales, one a lane, the others the columns'
   mm_i32x4 scales;
-  uint32_t scale_off, scale_lds;
-  int scale_row, kb;
-  float b_scale;  // of the tile's first 64 stages, one a lane
+  uint32_t scale_off, scale_step, scale_lds;
+  int kb, nb;  // blocks of K and N
+  bool of_rows;
 
-  // b's scale of stage s + lane for the tile's columns of this wavefront.
-  __device__ static __forceinline__ float b_scales(const MmArgs& p, const MmTile<C>& t, int s) {
-    const int kb = (p.K + 127) / 128, nb = (p.N + 127) / 128;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
-    const int c = ((int)t.col + wave % C::WN * (C::BN / C::WN)) / 128;
-    const int k = s + (int)(threadIdx.x % WAVE);
-    return k < kb ? p.sb[((int64_t)t.group * kb + k) * nb + (c < nb ? c : nb - 1)] : 0.0f;
-  }
   __device__ __forceinline__ void init(const MmTile<C>& first) {
     tile = first;
     row_bytes = (int64_t)p.K * C::SIZE;
@@ -717,11 +714,14 @@ struct MmSource {
     B.init(C::ALONG ? (uint32_t)row_bytes : (uint32_t)p.N * 2);
     if constexpr (C::EIGHT) {
       const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
-      const int part = wave % (C::SCALES / 256);
+      const int lane = (int)(threadIdx.x % WAVE);
+      of_rows = wave < C::BM / WAVE;
       kb = (p.K + 127) / 128;
-      scale_row = part * WAVE + (int)(threadIdx.x % WAVE);
-      scale_off = (uint32_t)scale_row * kb * 4;
-      scale_lds = C::A::BYTES + C::B::BYTES + part * 256;
+      nb = (p.N + 127) / 128;
+      scale_off = of_rows ? (uint32_t)(threadIdx.x * kb * 4)
+                          : lane < C::BN / 128 ? (uint32_t)lane * 4 : MM_PAST;
+      scale_step = of_rows ? 4 : nb * 4;
+      scale_lds = C::A::BYTES + C::B::BYTES + (of_rows ? wave * 256 : C::SCALES);
     }
     open();
   }
@@ -745,9 +745,10 @@ struct MmSource {
     else
       B.tile(block + col * 2, p.K, (p.N - (int)col) * (int64_t)2, left - col * 2);
     if constexpr (C::EIGHT) {
-      scales = mm_buffer((const char*)(p.sa + (int64_t)tile.row * kb),
-                         (int64_t)(rows < C::BM ? rows : C::BM) * kb * 4);
-      b_scale = b_scales(p, tile, tile.stage0);
+      const int64_t c = tile.col / 128, block = (int64_t)kb * nb;
+      const float* from = of_rows ? p.sa + (int64_t)tile.row * kb : p.sb + tile.group * block + c;
+      scales = mm_buffer((const char*)from,
+                         (of_rows ? (int64_t)(rows < C::BM ? rows : C::BM) * kb : block - c) * 4);
     }
   }
   __device__ __forceinline__ void begin() {
@@ -760,7 +761,7 @@ struct MmSource {
     } else if (i < C::A::LOADS + C::B::LOADS) {
       B.load(at + C::A::BYTES, i - C::A::LOADS);
     } else if constexpr (C::EIGHT) {
-      mm_load4(scales, scale_off + stage * 4, at + scale_lds);
+      mm_load4(scales, scale_off + stage * scale_step, at + scale_lds);
     }
   }
   __device__ __forceinline__ void next() {
@@ -819,6 +820,8 @@ __global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_kernel(MmArgs 
     MmHalf8<C::MI, C::NJ> f;
     const uint32_t s_at = (uint32_t)C::A::BYTES + C::B::BYTES +
                           (wm * (C::BM / C::WM) + threadIdx.x % 16) * 4;
+    const uint32_t sb_at = (uint32_t)C::A::BYTES + C::B::BYTES + C::SCALES +
+                           wn * (C::BN / C::WN) / 128 * 4;
     auto read_x = [&](uint32_t at, int i) {
       const mm_i32x4 lo = mm_lds16(at + a_at, i * 16 * MM_STAGE);
       const mm_i32x4 hi = mm_lds16((at + a_at) ^ 16, i * 16 * MM_STAGE);
@@ -829,6 +832,7 @@ __global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_kernel(MmArgs 
       const mm_i32x4 lo = mm_lds16(at + b_at, j * 16 * MM_STAGE);
       const mm_i32x4 hi = mm_lds16((at + b_at) ^ 16, j * 16 * MM_STAGE);
       f.y[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      if (j == 0) f.sb = mm_lds4(at + sb_at, 0);
     };
     ring.start([&](uint32_t at) {
 #pragma unroll
@@ -838,19 +842,7 @@ __global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_kernel(MmArgs 
     });
     for (mine.seek(p); mine.any; mine.seek(p)) {
       mm_zero(acc);
-      // a tile of few stages may be written before the loads of another begin
-      const MmTile<C>& t = source.tile;
-      float sb = 0.0f;
-      if (t.any && t.group == mine.group && t.row == mine.row && t.col == mine.col &&
-          t.part == mine.part)
-        sb = source.b_scale;
-      else if (mine.stage0 < mine.stage1)
-        sb = source.b_scales(p, mine, mine.stage0);
-      for (int s = mine.stage0; s < mine.stage1; ++s) {
-        const int k = (s - mine.stage0) % WAVE;
-        if (k == 0 && s > mine.stage0) sb = source.b_scales(p, mine, s);
-        ring.step8(f, acc, readlane_val(sb, k), read_x, read_y);
-      }
+      for (int k = mine.stage0; k < mine.stage1; ++k) ring.step8(f, acc, read_x, read_y);
       write();
     }
   } else {

@@ -13,14 +13,15 @@ struct Shape {
 };
 
 // us a stage from products of 8,192 rows by 8,192 by 8,192: 842, 1,120 and 1,290 TFLOP/s in
-// 16 bits and 1,156, 1,642 and 1,910 in 8; of 8,191 by 8,191: 498, 680 and 980, and 790,
-// 1,074 and 1,448.
-constexpr Shape shapes[] = {{64, 128, true, 512, {0.64f, 0.93f}},
-                            {128, 128, true, 512, {0.96f, 1.31f}},
-                            {256, 256, true, 256, {1.67f, 2.25f}},
-                            {64, 128, false, 512, {1.08f, 1.36f}},
-                            {128, 128, false, 512, {1.58f, 2.00f}},
-                            {256, 256, false, 256, {2.19f, 2.97f}}};
+// 16 bits and 1,250, 1,760 and 2,000 in 8; of 8,191 by 8,191: 498, 680 and 980, and 824,
+// 1,038 and 1,530. At 8 to 1,024 rows of 2,048 to 1,536 for each of 64 experts the choice is
+// the fastest of the three or within 11 % of it (16 bits, 192 rows: 151 and 136 us).
+constexpr Shape shapes[] = {{64, 128, true, 512, {0.64f, 0.86f}},
+                            {128, 128, true, 512, {0.96f, 1.22f}},
+                            {256, 256, true, 256, {1.67f, 2.15f}},
+                            {64, 128, false, 512, {1.08f, 1.30f}},
+                            {128, 128, false, 512, {1.58f, 2.07f}},
+                            {256, 256, false, 256, {2.19f, 2.81f}}};
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
