@@ -250,6 +250,20 @@ def test_few_rows_of_long_inner_axes(lens, behind, d1, d2, dtype):
             assert all(torch.equal(a, b) for a, b in zip(out, want)), seed
 
 
+def test_no_experts_and_no_inner_axis():
+    x = torch.ones(5, 8, device="cuda", dtype=BF16)
+    none = torch.ones(0, 8, 4, device="cuda", dtype=BF16)
+    assert torch.equal(ops.expert_mm(x, none, []), torch.zeros_like(x[:, :4]))
+    assert torch.equal(ops.scaled_mm(x, ops.quantize_blocks(none), []), torch.zeros_like(x[:, :4]))
+    x, w = x[:, :0], torch.ones(2, 0, 4, device="cuda", dtype=BF16)
+    for y in (ops.expert_mm(x, w, [2, 1]), ops.scaled_mm(x, ops.quantize_blocks(w), [2, 1]),
+              ops.scaled_mm(x, ops.quantize_blocks(w[0]))):
+        assert y.shape == (5, 4) and not y.any()
+    X, W = x.clone().requires_grad_(), w.clone().requires_grad_()
+    dx, dw = torch.autograd.grad(ops.expert_mm(X, W, [2, 1]).sum(), (X, W))
+    assert dx.shape == x.shape and dw.shape == w.shape
+
+
 def test_subnormal_values_and_large_ones():
     """Products and sums keep float32's range: float16 subnormals count, and a result past
     the type's range is infinite."""
