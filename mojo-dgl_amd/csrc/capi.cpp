@@ -2031,7 +2031,7 @@ int mdgl_scaled_mm(const void* a, const float* a_scale, const void* b, const flo
   MDGL_RANGE();
   if (int rc = quant_dtype("scaled_mm", dst_dtype)) return rc;
   if (int rc = expert_mm_common("scaled_mm", n, d1, r, d2)) return rc;
-  if (!seglen && r > 1)
+  if (!seglen && r != 1)
     return fail(MDGL_EINVAL, "scaled_mm: lengths are wanted for %lld groups", (long long)r);
   if (n == 0 || d2 == 0) return MDGL_OK;
   if (!dst || (r > 0 && d1 > 0 && (!a || !a_scale || !b || !b_scale)))

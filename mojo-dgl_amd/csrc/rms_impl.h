@@ -63,6 +63,16 @@ struct RmsCols {
   __device__ __forceinline__ int skip(int j) const { return at(j) + V <= d ? 0 : at(j) - (d - V); }
 };
 
+// 1 / sqrt(v). In float the root's and the quotient's roundings, exact in one fma each, are
+// put right: a row's values all carry this error (y's is 15 % less so).
+__device__ __forceinline__ double rms_rsqrt(double v) { return 1.0 / sqrt(v); }
+__device__ __forceinline__ float rms_rsqrt(float v) {
+  const float s = sqrtf(v), r = 1.0f / s;
+  const float e = __builtin_fmaf(-s, s, v), d = __builtin_fmaf(-s, r, 1.0f);
+  const float c = r * (d - 0.5f * e * (r * r));
+  return __builtin_fabsf(c) < r ? r + c : r;  // not where v is 0 or infinite
+}
+
 // One sum over the G threads of a group.
 template <int G, class A>
 __device__ __forceinline__ A rms_sum(A a, A* lds, int& turn) {
@@ -120,7 +130,7 @@ __global__ void __launch_bounds__(norm_block<G>()) rms_kernel(RmsArgs<T, W, R> p
     for (int j = 0; j < K; ++j)
 #pragma unroll
       for (int k = 0; k < V; ++k) q = fma_of(x[j][k], k >= own.skip(j) ? x[j][k] : A(0), q);
-    const A r = norm_rsqrt(rms_sum<G>(q, lds, turn) * inv + (A)p.eps);
+    const A r = rms_rsqrt(rms_sum<G>(q, lds, turn) * inv + (A)p.eps);
     if (p.rstd && t == 0) p.rstd[row] = r;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
@@ -331,7 +341,7 @@ __global__ void __launch_bounds__(NORM_WIDE) rms_wide_kernel(RmsArgs<T, W, R> p)
         const A v = value(c);
         q = fma_of(v, v, q);
       }
-      const A r = norm_rsqrt(rms_sum<NORM_WIDE>(q, lds, turn) * inv + (A)p.eps);
+      const A r = rms_rsqrt(rms_sum<NORM_WIDE>(q, lds, turn) * inv + (A)p.eps);
       if (p.rstd && threadIdx.x == 0) p.rstd[row] = r;
       if constexpr (!Q) {
         for (int64_t c = threadIdx.x; c < p.d; c += NORM_WIDE) {

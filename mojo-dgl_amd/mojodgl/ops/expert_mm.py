@@ -255,6 +255,8 @@ def scaled_mm(value, weight, plan=None, dtype=None):
     scale = _lib.rows_on_device(q.scale, torch.float32)
     w = _inner_last(w)
     ws_ = _lib.rows_on_device(weight.scale, torch.float32)
+    if r == 0:  # and no lengths, which would be one group of all rows
+        return _lib.hand_back(torch.zeros(n, d2, dtype=dtype, device=dev), where)
     y = torch.empty(n, d2, dtype=dtype, device=dev)
     L = _lib.lib()
     nbytes = L.mdgl_scaled_mm_workspace_bytes(n, d1, r, d2)
