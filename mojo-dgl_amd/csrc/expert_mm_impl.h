@@ -39,6 +39,14 @@
 // experts, each in bands of 8 column tiles; an XCD takes one contiguous run of tiles,
 // so that the rows and blocks its workgroups share lie in its own L2. Rows behind the
 // last expert's form a group without an inner axis: they are written as zeros.
+//
+// Measured: 8,192 rows by 8,192 by 8,192 in 816 us (bfloat16, b's inner axis contiguous; 850
+// the other way; 866 the gradient of b), where the matrix cores are busy for 55 % of the
+// cycles, and in 528 us in 8 bits. 65,536 rows of 2,048 to 1,536 through 64 experts: 435 us
+// forward, 450 and 450 the gradients. There loads that came from L2 alone would save 11 to
+// 19 %, no stores 6 to 16 %: the tiles of a round end together, and their results' burst delays
+// the loads behind it. Few rows are bound by reading the experts called: 64 of them by 8
+// rows each in 76 us (5.3 TB/s).
 #pragma once
 
 #include "mdgl_half.h"
