@@ -713,7 +713,8 @@ int mdgl_quantize_blocks(const void* value, void* dst, float* scale, int64_t r, 
  * rows, negative ones are 0); rows behind the last group are written as zeros. With
  * `transposed` b holds [d2][d1] each: with the same b, a gradient of dst and d1 and d2
  * exchanged that is the gradient of a. Fewer than 2**31 rows and 2**20 columns, at
- * most 65535 groups. Without any group or d1 dst is zeros. */
+ * most 65535 groups. Without any group or d1 dst is zeros. Operands may begin at any
+ * value. The workspace is one that no other running call uses. */
 int mdgl_expert_mm(const void* a, const void* b, void* dst, const int64_t* seglen, int64_t n,
                    int64_t d1, int64_t r, int64_t d2, int transposed, void* workspace,
                    int64_t workspace_bytes, int dtype, void* stream);
