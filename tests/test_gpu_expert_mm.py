@@ -135,6 +135,28 @@ def test_large_tiles_of_every_product(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
+def test_large_tiles_of_odd_widths(dtype):
+    g = gen(11)
+    lens, d1, d2 = [9001, 0, 700, 3], 2049, 2051
+    n = sum(lens) + 5
+    x, dy = rand(g, n, d1, dtype=dtype), rand(g, n, d2, dtype=dtype)
+    w = rand(g, 4, d1, d2, dtype=dtype)
+    X, W = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = ops.expert_mm(X, W, lens)
+    dx, dw = torch.autograd.grad(y, (X, W), dy)
+    want, size = products(x, w, lens)
+    check(y.detach(), want, (d1 + 64) * U * size, "y")
+    want, size = products(dy, w.transpose(1, 2).contiguous(), lens)
+    check(dx, want, (d2 + 64) * U * size, "dx")
+    want, size = weight_gradients(x, dy, lens, 4)
+    check(dw, want, (max(lens) + 64) * U * size, "dw")
+    qx, qw = ops.quantize_rows(x), ops.quantize_blocks(w)
+    y = ops.scaled_mm(qx, qw, lens, dtype=F32)
+    want, size = products(values(qx, (1,)), values(qw, (1, 2)), lens)
+    check(y, want, (d1 + 68) * U * size + cut(qx, qw, lens), "8 bits")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("d1,d2", [(72, 40), (71, 41), (136, 264)])
 def test_what_is_not_a_number_stays_in_its_row(dtype, d1, d2):
     """NaN and infinities in one group's rows, at its borders, and behind the last."""
