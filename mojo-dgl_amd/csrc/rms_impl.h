@@ -8,12 +8,12 @@
 //
 // y is formed from the unrounded sum, and so are the gradients: from `total` where that
 // is float (double for double rows), else from x and the residual once more (dw of
-// 32,768 rows is off by 2e-7 of its size so, by 1e-5 from a bfloat16 total). Rows lie on threads as layer norm's do
-// (norm_geometry): a group of threads holds a row in registers, so each row is read
-// and written once, with the next one's loads in flight; the weight's gradient is
-// summed in registers, one row of sums a workgroup, added by norm_sum_kernel in a
-// fixed order. In 8 bits the 128 columns of a block lie on 128 / V neighbouring
-// lanes, whose maximum goes through DPP.
+// 32,768 rows is off by 2e-7 of its size so, by 1e-5 from a bfloat16 total). Rows lie on
+// threads as layer norm's do (norm_geometry): a group of threads holds a row in
+// registers, so each row is read and written once, with the next one's loads in flight;
+// the weight's gradient is summed in registers, one row of sums a workgroup, added by
+// norm_sum_kernel in a fixed order. In 8 bits the 128 columns of a block lie on 128 / V
+// neighbouring lanes, whose maximum goes through DPP.
 //
 // Bound by memory: 32,768 bfloat16 rows of 4,096 with a bfloat16 residual take 473 us
 // forward and backward (nine rows of 268 MB read and written, 5.1 TB/s), 200,000 float32

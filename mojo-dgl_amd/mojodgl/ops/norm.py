@@ -218,7 +218,7 @@ def _rms_norm_grad(total, residual, weight, rstd, grad, grad_total, vt, wt, rt, 
         nbytes = L.mdgl_rms_norm_grad_workspace_bytes(n, d, code)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes > 0 else None
     _lib.check(L.mdgl_rms_norm_grad(
-        t.data_ptr(), _lib.ptr(r), _lib.ptr(w), rstd.data_ptr(), g.data_ptr(), _lib.ptr(gt), _lib.ptr(dx),
-        _lib.ptr(dr), _lib.ptr(dw), n, d, _lib.ptr(ws), nbytes, code, _lib.ROW_CODES[wt],
+        t.data_ptr(), _lib.ptr(r), _lib.ptr(w), rstd.data_ptr(), g.data_ptr(), _lib.ptr(gt),
+        _lib.ptr(dx), _lib.ptr(dr), _lib.ptr(dw), n, d, _lib.ptr(ws), nbytes, code, _lib.ROW_CODES[wt],
         _lib.ROW_CODES[rt], _lib.stream()), "rms_norm_grad")
     return dx if need_x else None, dw, (dx if one else dr) if need_r else None
