@@ -662,12 +662,12 @@ class GatherMM(torch.autograd.Function):
 
 def _save_some(ctx, *xs):
     """`_save_operands` for any number of operands."""
-    ctx.save_for_backward(*(x if isinstance(x, torch.Tensor) else None for x in xs))
-    ctx.host = tuple(None if isinstance(x, torch.Tensor) else x for x in xs)
+    ctx.save_for_backward(*[x if isinstance(x, torch.Tensor) else None for x in xs])
+    ctx.host = [None if isinstance(x, torch.Tensor) else x for x in xs]
 
 
 def _saved_some(ctx):
-    return tuple(h if t is None else t for t, h in zip(ctx.saved_tensors, ctx.host))
+    return [h if t is None else t for t, h in zip(ctx.saved_tensors, ctx.host)]
 
 
 def _made_here(ctx, where):
@@ -690,6 +690,18 @@ def _where_made(backward):
             with torch.cuda.device(ctx.gpu):
                 return backward(ctx, *grads)
         return backward(ctx, *grads)
+
+    return run
+
+
+def _first_order(backward):
+    """`once_differentiable`, past its cost where no second derivative can follow (with
+    `_where_made` 4 us of the 20 that a small backward call takes)."""
+    checked = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
 
@@ -767,7 +779,7 @@ class RmsNorm(torch.autograd.Function):
         return y, total
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     @_where_made
     def backward(ctx, grad, grad_total):
         from .norm import _rms_norm_grad
@@ -839,7 +851,7 @@ class ExpertMM(torch.autograd.Function):
         return _lib.hand_back(y, where)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     @_where_made
     def backward(ctx, grad):
         from .expert_mm import _expert_mm_grad
