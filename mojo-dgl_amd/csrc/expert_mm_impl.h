@@ -1122,7 +1122,7 @@ hipError_t run_expert_mm(const MmArgs& p, int64_t most_tiles, hipStream_t s) {
   }
 }
 
-// The shapes of mm_shapes (expert_mm_plan.hip).
+// The shapes as expert_mm_plan.hip lists them.
 template <class E, bool ALONG>
 hipError_t run_expert_mm_shape(const ExpertMmParams& q) {
   MmArgs p{};
