@@ -264,8 +264,9 @@ struct MmAlong {
     }
     buf = mm_buffer(at, bytes);
   }
-  // No tile: its loads give zeros.
-  __device__ __forceinline__ void none() { buf[2] = 0; }
+  // No tile: its loads give zeros. A workgroup may never have one, so nothing is left from
+  // the tile before.
+  __device__ __forceinline__ void none() { buf = mm_buffer(nullptr, 0); }
   __device__ __forceinline__ void begin(uint32_t stage) {
     from = stage * MM_STAGE + (uint32_t)col < stride ? off + stage * MM_STAGE : MM_PAST;
   }
@@ -352,7 +353,10 @@ struct MmAcross {
       }
     }
   }
-  __device__ __forceinline__ void none() { bytes = 0; }
+  __device__ __forceinline__ void none() {
+    p = nullptr;
+    bytes = 0;
+  }
   __device__ __forceinline__ void begin(uint32_t stage) {
     const int64_t first = (int64_t)stage * 64;
     buf = mm_buffer(p + first * stride, bytes - first * stride);
@@ -673,6 +677,9 @@ struct MmTile {
   bool any;
 
   __device__ __forceinline__ void init(const MmArgs& p) {
+    group = part = stage0 = stage1 = 0;
+    row = end = col = 0;
+    any = false;
     walk.init(p.seglen, p.groups, p.rows, C::BM);
     order.init(walk.total() * across(p) * p.splits);
   }
@@ -682,7 +689,7 @@ struct MmTile {
   __device__ __forceinline__ void seek(const MmArgs& p) {
     any = false;
     if (order.at >= order.end) return;
-    uint32_t s, p0, p1, i, j;
+    uint32_t s = 0, p0 = 0, p1 = 0, i, j;
     const uint32_t at = order.at / p.splits, wide = across(p);
     part = (int)(order.at - at * p.splits);
     order.at += order.step;
@@ -736,13 +743,14 @@ struct MmSource {
   __device__ __forceinline__ void open() {
     do tile.seek(p);
     while (tile.any && tile.stage0 == tile.stage1);
-    stage = tile.stage0;
+    stage = 0;
     if (!tile.any) {
       A.none();
       B.none();
-      if constexpr (C::EIGHT) scales[2] = 0;
+      if constexpr (C::EIGHT) scales = mm_buffer(nullptr, 0);
       return;
     }
+    stage = tile.stage0;
     const int rows = (int)(tile.end - tile.row);
     A.tile(p.a + tile.row * row_bytes, rows, (p.rows - tile.row) * row_bytes);
     const char* block = p.b + tile.group * (row_bytes * p.N);
@@ -935,13 +943,16 @@ struct MmGradTile {
     return (uint32_t)((p.D2 + C::BN - 1) / C::BN);
   }
   __device__ __forceinline__ void init(const MmGradArgs& p) {
+    group = stages = rows = 0;
+    start = row = col = piece = 0;
+    any = alone = false;
     walk.init(p.seglen, p.groups, p.rows, p.piece);
     order.init(walk.total() * (down(p) * across(p)));
   }
   __device__ __forceinline__ void seek(const MmGradArgs& p) {
     any = false;
     if (order.at >= order.end) return;
-    uint32_t s, e, p0, p1, i, j;
+    uint32_t s = 0, e = 0, p0 = 0, p1 = 0, i, j;
     const uint32_t at = order.at, tiles = down(p) * across(p);
     order.at += order.step;
     piece = at / tiles;
