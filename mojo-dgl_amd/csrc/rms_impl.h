@@ -125,11 +125,13 @@ __global__ void __launch_bounds__(norm_block<G>()) rms_kernel(RmsArgs<T, W, R> p
       }
     const int64_t next = row + step;
     fetch(next);
+    // columns that the vector before has are left out of the sum, not multiplied by 0,
+    // which an infinity turns into a NaN
     A q = A(0);
 #pragma unroll
     for (int j = 0; j < K; ++j)
 #pragma unroll
-      for (int k = 0; k < V; ++k) q = fma_of(x[j][k], k >= own.skip(j) ? x[j][k] : A(0), q);
+      for (int k = 0; k < V; ++k) q = k >= own.skip(j) ? fma_of(x[j][k], x[j][k], q) : q;
     const A r = rms_rsqrt(rms_sum<G>(q, lds, turn) * inv + (A)p.eps);
     if (p.rstd && t == 0) p.rstd[row] = r;
 #pragma unroll
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(norm_block<G>()) rms_grad_kernel(RmsArgs<T, W,
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         dw[j][k] = fma_of(dy[k], xh[k], dw[j][k]);
-        q = fma_of(k >= own.skip(j) ? gw[k] : A(0), xh[k], q);
+        q = k >= own.skip(j) ? fma_of(gw[k], xh[k], q) : q;
       }
     }
     if (p.dx || p.dr) {
