@@ -734,8 +734,10 @@ int64_t mdgl_expert_mm_grad_workspace_bytes(int64_t n, int64_t d1, int64_t r, in
  * [r][ceil(d1 / 128)][ceil(d2 / 128)]):
  *   dst[i][c] = sum over k of a_scale a[i][k] b_scale b[g(i)][c][k]
  * summed in float block by block of 128; within eight neighbouring k products are cut
- * off 13 binary places below the largest. A null seglen is one group of all rows
- * (r = 1). dst_dtype: MDGL_FLOAT32, MDGL_BFLOAT16 or MDGL_FLOAT16. */
+ * off 13 binary places below the largest. A product of two scales below 2^-126 is rounded
+ * to a multiple of 2^-149; where it is past float's range a block's sum takes one scale
+ * after the other. A null seglen is one group of all rows (r = 1). dst_dtype:
+ * MDGL_FLOAT32, MDGL_BFLOAT16 or MDGL_FLOAT16. */
 int mdgl_scaled_mm(const void* a, const float* a_scale, const void* b, const float* b_scale,
                    void* dst, const int64_t* seglen, int64_t n, int64_t d1, int64_t r, int64_t d2,
                    void* workspace, int64_t workspace_bytes, int dst_dtype, void* stream);

@@ -621,6 +621,8 @@ struct MmRing {
 #pragma unroll
     for (int n = MI * NJ - LAG; n < MI * NJ; ++n) add(n);
   }
+  // Where the stage that is multiplied next lies.
+  __device__ __forceinline__ uint32_t place() const { return base + use * BYTES; }
   // Nothing is left on its way to LDS.
   __device__ __forceinline__ void finish() const { mm_wait<0>(); }
 };
@@ -791,6 +793,69 @@ struct MmSource {
   }
 };
 
+// 32 bytes of row `i` of `rows` from place k on, zeros past the end of it or of the rows.
+__device__ __forceinline__ mm_i32x8 mm_bytes(const char* p, int64_t i, int64_t rows, int K, int k) {
+  mm_i32x8 v;
+#pragma unroll
+  for (int w = 0; w < 8; ++w, k += 4) {
+    uint32_t word = 0;
+    if (i < rows) {
+      const char* at = p + i * K + k;
+      if (k + 4 <= K) {
+        __builtin_memcpy(&word, at, 4);
+      } else {
+        for (int b = 0; b < K - k; ++b) word |= (uint32_t)(uint8_t)at[b] << 8 * b;
+      }
+    }
+    v[w] = (int)word;
+  }
+  return v;
+}
+
+// Two finite scales whose product is not: both are above 1, and one is 2^64 at least.
+__device__ __forceinline__ bool mm_apart(float a, float b) {
+  return __builtin_isinf(a * b) && !__builtin_isinf(a) && !__builtin_isinf(b);
+}
+// A wavefront's part of a tile that has such, block of 16 by 16 after block, straight from
+// memory: there a block's sum takes one scale after the other, so that 0 stays 0 and what is
+// in float's range stays.
+template <class C>
+__device__ __forceinline__ void mm_write_apart(const MmArgs& p, const MmTile<C>& t, int64_t row0,
+                                               int64_t n0) {
+  int lane = threadIdx.x % WAVE;
+  asm volatile("" : "+v"(lane));  // nothing of this is formed in front of the tiles
+  const int l = lane % 16, q = lane / 16;
+  const int kb = (p.K + 127) / 128, nb = (p.N + 127) / 128;
+  const char* b = p.b + t.group * ((int64_t)p.K * p.N);
+  const float* sb = p.sb + t.group * ((int64_t)kb * nb) + n0 / 128;
+  if (n0 >= p.N) return;  // none of the wavefront's columns are there
+#pragma unroll 1
+  for (int block = 0; block < C::MI * C::NJ; ++block) {
+    const int64_t r = row0 + block / C::NJ * 16 + l, n = n0 + block % C::NJ * 16;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+    for (int s = t.stage0; s < t.stage1; ++s) {
+      const mm_i32x8 x = mm_bytes(p.a, r, t.end, p.K, s * 128 + q * 32);
+      const mm_i32x8 y = mm_bytes(b, n + l, p.N, p.K, s * 128 + q * 32);
+      const mm_f32x4 sum = mm_mul8(y, x);
+      const float sr = r < t.end ? p.sa[r * kb + s] : 0.0f, sc = sb[s * nb];
+      const bool apart = mm_apart(sr, sc);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v[k] = __builtin_fmaf(apart ? sum[k] * sr : sum[k], apart ? sc : sr * sc, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t c = n + 4 * q + k, at = r * p.N + c;
+      if (r >= t.end || c >= p.N) continue;
+      if (p.splits > 1) p.part[t.part * (p.rows * p.N) + at] = v[k];
+      else if (p.out_dtype == DT_F32) ((float*)p.out)[at] = v[k];
+      else if (p.out_dtype == DT_BF16) ((bf16_t*)p.out)[at] = (bf16_t)v[k];
+      else ((f16_t*)p.out)[at] = (f16_t)v[k];
+    }
+  }
+}
+
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_kernel(MmArgs p) {
   using E = typename C::Elem;
@@ -858,7 +923,29 @@ __global__ void __launch_bounds__(C::THREADS, C::WAVES) expert_mm_kernel(MmArgs 
     });
     for (mine.seek(p); mine.any; mine.seek(p)) {
       mm_zero(acc);
-      for (int k = mine.stage0; k < mine.stage1; ++k) ring.step8(f, acc, read_x, read_y);
+      bool apart = false;
+      for (int k = mine.stage0; k < mine.stage1; ++k) {
+        // one scale for the wavefront's columns; only one above 1 (of weights above 448) can
+        // have an infinite product, and others cost this comparison (10,001 rows by 4,096
+        // by 8,192: 335 us without it, 338 with it; 348 with the scales' powers of two in
+        // the matrix instruction)
+        const float sb = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(f.sb)));
+        if (__builtin_expect(__builtin_fabsf(sb) > 1.0f, 0)) {
+          const uint32_t rows = ring.place() + C::A::BYTES + C::B::BYTES +
+                                (wm * (C::BM / C::WM) + threadIdx.x % WAVE) * 4;
+          bool any = false;
+#pragma unroll
+          for (int i = 0; i < C::MI * 16 / WAVE; ++i) any |= mm_apart(mm_lds4(rows, i * 256), sb);
+          apart |= __builtin_amdgcn_readfirstlane(__any(any)) != 0;
+        }
+        ring.step8(f, acc, read_x, read_y);
+      }
+      if (__builtin_expect(apart, 0)) {
+        mm_write_apart(p, mine, (int64_t)mine.row + wm * (C::BM / C::WM),
+                       (int64_t)mine.col + wn * (C::BN / C::WN));
+        ring.stored = false;
+        continue;
+      }
       write();
     }
   } else {

@@ -211,7 +211,9 @@ def scaled_mm(value, weight, plan=None, dtype=None):
     (N, D2) products, summed in float32 block by block, zeros for rows behind the last
     group. Within eight neighbouring k the matrix cores cut products off 13 binary
     places below the largest, so a sum is off by 7 * 2 ** -13 of these largest at most.
-    It has no gradient (`expert_mm` has).
+    Any finite scales may meet: a product of two below 2 ** -126 is rounded to a multiple
+    of 2 ** -149, and where it is past float32's range a block's sum takes one after the
+    other. It has no gradient (`expert_mm` has).
     """
     if not isinstance(weight, _quant.Quantized):
         raise DGLError("scaled_mm wants weights made by quantize_blocks")
