@@ -701,8 +701,8 @@ int mdgl_quantize_rows(const void* value, void* dst, float* scale, int64_t n, in
 
 /* r matrices of [d1][d2] values ([d2][d1] with `transposed`) as e4m3 bytes, always
  * [d2][d1], with a scale for each block of 128 by 128,
- * [r][ceil(d1 / 128)][ceil(d2 / 128)]: the weights of mdgl_scaled_mm. Fewer than
- * 2**24 blocks a matrix. */
+ * [r][ceil(d1 / 128)][ceil(d2 / 128)]: the weights of mdgl_scaled_mm. At most
+ * 16777208 blocks a matrix (a launch's workgroups of 256 work-items). */
 int mdgl_quantize_blocks(const void* value, void* dst, float* scale, int64_t r, int64_t d1,
                          int64_t d2, int transposed, int dtype, void* stream);
 

@@ -1891,8 +1891,9 @@ int mdgl_quantize_blocks(const void* value, void* dst, float* scale, int64_t r, 
   if (int rc = quant_dtype("quantize_blocks", dtype)) return rc;
   if (r < 0 || d1 < 0 || d2 < 0) return fail(MDGL_EINVAL, "quantize_blocks: negative size");
   if (!row_widths_fit(d1, dtype_bytes(dtype)) || !row_widths_fit(d2, dtype_bytes(dtype)) ||
-      ((d1 + 127) / 128) * ((d2 + 127) / 128) >= (int64_t(1) << 24))
-    return fail(MDGL_EINVAL, "quantize_blocks: 2**24 or more blocks a matrix");
+      ((d1 + 127) / 128) * ((d2 + 127) / 128) > MAX_LAUNCH_BLOCKS)
+    return fail(MDGL_EINVAL, "quantize_blocks: more than %lld blocks a matrix",
+                (long long)MAX_LAUNCH_BLOCKS);
   if (r == 0 || d1 == 0 || d2 == 0) return MDGL_OK;
   if (!value || !dst || !scale) return fail(MDGL_EINVAL, "quantize_blocks: null buffer");
   return hip_status(launch_quantize_blocks(value, dst, scale, r, d1, d2, transposed != 0, dtype,

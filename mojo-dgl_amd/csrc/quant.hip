@@ -141,7 +141,7 @@ template <class T>
 hipError_t run_quant_blocks(const void* src, void* dst, float* scale, int64_t r, int64_t d1,
                             int64_t d2, bool transposed, hipStream_t s) {
   const int64_t per = ((d1 + Q_BLOCK - 1) / Q_BLOCK) * ((d2 + Q_BLOCK - 1) / Q_BLOCK);
-  const int64_t most = MAX_LAUNCH_BLOCKS / per;  // at least 1: per < 2^24 (checked before)
+  const int64_t most = MAX_LAUNCH_BLOCKS / per;  // at least 1 (checked before)
   for (int64_t at = 0; at < r; at += most) {
     const int64_t grid = (r - at < most ? r - at : most) * per, skip = at * d1 * d2;
     const T* from = (const T*)src + skip;
