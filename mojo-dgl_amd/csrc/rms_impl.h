@@ -11,8 +11,8 @@
 // 32,768 rows is off by 2e-7 of its size so, by 1e-5 from a bfloat16 total). Rows lie on
 // threads as layer norm's do (norm_geometry): a group of threads holds a row in
 // registers, so each row is read and written once, with the next one's loads in flight;
-// the weight's gradient is summed in registers, one row of sums a workgroup, added by
-// norm_sum_kernel in a fixed order. In 8 bits the 128 columns of a block lie on 128 / V
+// the weight's gradient is summed in registers, 16 rows at a time, these sums in LDS,
+// one row of sums a workgroup, added by norm_sum_kernel in a fixed order. In 8 bits the 128 columns of a block lie on 128 / V
 // neighbouring lanes, whose maximum goes through DPP.
 //
 // Bound by memory: 32,768 bfloat16 rows of 4,096 with a bfloat16 residual take 473 us
@@ -187,7 +187,13 @@ __global__ void __launch_bounds__(norm_block<G>()) rms_grad_kernel(RmsArgs<T, W,
   constexpr bool HOLD = K < 4, AHEAD = K < 4 || (G < 1024 && sizeof(R) == sizeof(T));
   __shared__ A lds[G > WAVE ? 4 * (G / WAVE) : 1];
   __shared__ A sums[GROUPS > 1 ? G * K * V : 1];
-  int turn = 0;
+  // dw's sums of RUN rows each are added up here, a thread's own: one chain over all of its
+  // rows loses bits (200,000 float32 rows of 602, 195 in a chain: dw is off by 3.2e-7 of its
+  // size, so by 2.1e-7, at the same time)
+  constexpr int RUN = 16;
+  __shared__ A kept[K * V][norm_block<G>()];
+  int turn = 0, run = 0;
+  bool some = false;  // in `kept`
   const int t = threadIdx.x % G, group = threadIdx.x / G;
   RmsCols<V, G> own{t, (int)p.d};
   A w[HOLD ? K : 1][V], dw[K][V];
@@ -200,6 +206,20 @@ __global__ void __launch_bounds__(norm_block<G>()) rms_grad_kernel(RmsArgs<T, W,
     }
     if (HOLD && own.live(j) && p.w) load_acc<W, A, V>(p.w + own.col(j), w[HOLD ? j : 0]);
   }
+  auto keep = [&](bool take) {
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        A& at = kept[j * V + k][threadIdx.x];
+        if (some) dw[j][k] += at;
+        if (!take) {
+          at = dw[j][k];
+          dw[j][k] = A(0);
+        }
+      }
+    some = true;
+  };
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   const A inv = A(1) / (A)p.d;
   int64_t row = (int64_t)blockIdx.x * GROUPS + group;
@@ -281,8 +301,13 @@ __global__ void __launch_bounds__(norm_block<G>()) rms_grad_kernel(RmsArgs<T, W,
     }
     if (!AHEAD) fetch(next);
     row = next;
+    if (++run == RUN) {
+      run = 0;
+      keep(false);
+    }
   }
   if (!p.part_w) return;
+  if (some) keep(true);
   if constexpr (GROUPS > 1) {
     // the groups of the workgroup one after the other
     for (int i = 0; i < GROUPS; ++i) {
@@ -386,8 +411,13 @@ __global__ void __launch_bounds__(BLOCK) rms_cols_kernel(RmsArgs<T, W, R> p) {
   const int64_t c = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
   if (c >= p.d) return;
   A dw = A(0);
-  for (int64_t row = blockIdx.y; row < p.n; row += gridDim.y)
-    dw = fma_of((A)p.dy[row * p.d + c], rms_total(p, row * p.d + c) * p.rstd[row], dw);
+  for (int64_t row = blockIdx.y; row < p.n;) {
+    A some = A(0);  // of 16 rows (as in rms_grad_kernel)
+#pragma unroll 1
+    for (int i = 0; i < 16 && row < p.n; ++i, row += gridDim.y)
+      some = fma_of((A)p.dy[row * p.d + c], rms_total(p, row * p.d + c) * p.rstd[row], some);
+    dw += some;
+  }
   p.part_w[(int64_t)blockIdx.y * p.d + c] = dw;
 }
 
