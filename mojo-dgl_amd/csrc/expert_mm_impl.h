@@ -195,15 +195,18 @@ __device__ __forceinline__ mm_i32x4 mm_buffer(const char* p, int64_t bytes) {
 
 // 16 (4) bytes a lane from the buffer to consecutive LDS places from `lds` on; zeros
 // where the offset lies behind the buffer. It is waited for with the vector memory
-// counter, which the compiler does not do for it.
+// counter, which the compiler does not do for it. Nor does it keep the distances that the
+// machine asks for in front of it: one wait state behind m0, five behind a vector
+// instruction that wrote a scalar register of `buf` (readlanes, of registers that the
+// compiler keeps in lanes, too). The move and the s_nop are these five.
 __device__ __forceinline__ void mm_load16(mm_i32x4 buf, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                :
                : "v"(off), "s"(buf), "s"(lds)
                : "m0");
 }
 __device__ __forceinline__ void mm_load4(mm_i32x4 buf, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dword %0, %1, 0 offen lds"
                :
                : "v"(off), "s"(buf), "s"(lds)
                : "m0");
