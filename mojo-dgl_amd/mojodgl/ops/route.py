@@ -186,7 +186,7 @@ def dispatch_rows(value, plan):
     Parameters
     ----------
     value : (N, ...) array or tensor, or `Quantized` rows, whose values and scales
-        are both copied
+        are both copied (rows in 8 bits, torch.float8_e4m3fn, have no gradient)
     plan : the `RoutePlan` of the N rows
 
     Returns
@@ -201,6 +201,8 @@ def dispatch_rows(value, plan):
         where = _lib.caller_device(*value)
         return Quantized(*(_lib.hand_back(_dispatch_rows(t, plan), where) for t in value))
     if _autograd.needs_grad(value):
+        if value.dtype is torch.float8_e4m3fn:
+            raise DGLError("dispatch_rows has no gradient for rows in 8 bits")
         return _autograd.DispatchRows.apply(value, plan)
     return _lib.hand_back(_dispatch_rows(value, plan), _lib.caller_device(value))
 
