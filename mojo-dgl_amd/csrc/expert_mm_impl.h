@@ -40,10 +40,11 @@
 // so that the rows and blocks its workgroups share lie in its own L2. Rows behind the
 // last expert's form a group without an inner axis: they are written as zeros.
 //
-// Measured: 8,192 rows by 8,192 by 8,192 in 816 us (bfloat16, b's inner axis contiguous; 850
-// the other way; 866 the gradient of b), where the matrix cores are busy for 55 % of the
-// cycles, and in 528 us in 8 bits. 65,536 rows of 2,048 to 1,536 through 64 experts: 435 us
-// forward, 450 and 450 the gradients. There loads that came from L2 alone would save 11 to
+// Measured: 8,192 rows by 8,192 by 8,192 in 824 us (bfloat16, b's inner axis contiguous; 808
+// the other way; 839 the gradient of b), where the matrix cores are busy for 55 % of the
+// cycles, and in 476 us in 8 bits (normal values; of others up to 528, by what they draw).
+// 65,536 rows of 2,048 to 1,536 through 64 experts: 425 us forward, 450 and 450 the
+// gradients. There loads that came from L2 alone would save 11 to
 // 19 %, no stores 6 to 16 %: the tiles of a round end together, and their results' burst delays
 // the loads behind it. Few rows are bound by reading the experts called: 64 of them by 8
 // rows each in 76 us (5.3 TB/s).
@@ -821,7 +822,8 @@ __device__ __forceinline__ bool mm_apart(float a, float b) {
 }
 // A wavefront's part of a tile that has such, block of 16 by 16 after block, straight from
 // memory: there a block's sum takes one scale after the other, so that 0 stays 0 and what is
-// in float's range stays.
+// in float's range stays. No path for speed: 10,001 rows by 4,096 by 8,192, all of them such,
+// take 20 ms (weights' scales above 1 without such products 373 us, others 318).
 template <class C>
 __device__ __forceinline__ void mm_write_apart(const MmArgs& p, const MmTile<C>& t, int64_t row0,
                                                int64_t n0) {

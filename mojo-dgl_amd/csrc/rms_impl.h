@@ -11,13 +11,14 @@
 // 32,768 rows is off by 2e-7 of its size so, by 1e-5 from a bfloat16 total). Rows lie on
 // threads as layer norm's do (norm_geometry): a group of threads holds a row in
 // registers, so each row is read and written once, with the next one's loads in flight;
-// the weight's gradient is summed in registers, 16 rows at a time, these sums in LDS,
-// one row of sums a workgroup, added by norm_sum_kernel in a fixed order. In 8 bits the 128 columns of a block lie on 128 / V
-// neighbouring lanes, whose maximum goes through DPP.
+// the weight's gradient is summed in registers, 16 rows at a time, these sums in LDS, and
+// one row of sums a workgroup is added by norm_sum_kernel, all in a fixed order. In 8 bits
+// the 128 columns of a block lie on 128 / V neighbouring lanes, whose maximum goes through
+// DPP.
 //
 // Bound by memory: 32,768 bfloat16 rows of 4,096 with a bfloat16 residual take 473 us
 // forward and backward (nine rows of 268 MB read and written, 5.1 TB/s), 200,000 float32
-// rows of 602 without one 457 us (five of 482 MB, 5.3 TB/s), 32,768 rows of 5,120 with
+// rows of 602 without one 463 us (five of 482 MB, 5.3 TB/s), 32,768 rows of 5,120 with
 // a float32 residual in 8 bits 354 us (1.85 GB, 5.2 TB/s), where a copy of 1 GiB runs at
 // 5.2 TB/s.
 #pragma once

@@ -9,9 +9,12 @@ that route_plan puts in order.
 or, with the experts' weights kept in 8 bits,
 
     q = quantize_blocks(w)                                  # once
-    y = combine_rows(scaled_mm(dispatch_rows(x, plan), q, plan), weights, plan)
+    rows = dispatch_rows(quantize_rows(x), plan)            # or of rms_norm(.., quantize=True)
+    y = combine_rows(scaled_mm(rows, q, plan, dtype=x.dtype), weights, plan)
 
-Sums are float32 (float64 for float64 rows) and are rounded to the rows' type once.
+(rows brought to 8 bits in front of the dispatch are N, behind it N * k with the same bits:
+32,768 bfloat16 rows of 4,096 to 2 of 32 experts in 767 us, the other way in 953). Sums are
+float32 (float64 for float64 rows) and are rounded to the rows' type once.
 """
 
 from __future__ import annotations
